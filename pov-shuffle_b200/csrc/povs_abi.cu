@@ -6,8 +6,6 @@
 
 #include <algorithm>
 #include <atomic>
-#include <cstdarg>
-#include <cstdio>
 #include <cstring>
 #include <mutex>
 #include <unordered_map>
@@ -16,35 +14,19 @@
 #include <unistd.h>
 
 #include "../../include/povs.h"
+#include "povs_host.h"
 #include "povs_kernel.cuh"
 #include "povs_metrics.cuh"
 #include "povs_mt19937.h"
 
 using povs::IterParams;
+using povs_host::cuda_fail;
+using povs_host::DeviceGuard;
+using povs_host::fail;
+using povs_host::g_err;
+using povs_host::MAX_DEVICES;
 
 namespace {
-
-thread_local char g_err[512] = "";
-
-int fail(int code, const char* fmt, ...)
-{
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(g_err, sizeof(g_err), fmt, ap);
-    va_end(ap);
-    return code;
-}
-
-int cuda_fail(cudaError_t e, const char* what)
-{
-    return fail(POVS_ERR_CUDA, "%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
-}
-
-#define POVS_CUDA_TRY(expr)                                \
-    do {                                                   \
-        cudaError_t e_ = (expr);                           \
-        if (e_ != cudaSuccess) return cuda_fail(e_, #expr); \
-    } while (0)
 
 bool is_pow2(int64_t x) { return x > 0 && (x & (x - 1)) == 0; }
 
@@ -198,30 +180,9 @@ struct DeviceCtx {
     std::unordered_map<uint64_t, NpTable> np_tables;
 };
 
-constexpr int MAX_DEVICES = 64;
 constexpr int64_t SLAB_FLOOR_BYTES = 2048; // preferred minimum width of a column slab
 DeviceCtx g_ctx[MAX_DEVICES];
 std::mutex g_ctx_mu;
-
-struct DeviceGuard {
-    int prev = -1;
-    bool changed = false;
-    int enter(int dev)
-    {
-        cudaError_t e = cudaGetDevice(&prev);
-        if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
-        if (prev != dev) {
-            e = cudaSetDevice(dev);
-            if (e != cudaSuccess) return cuda_fail(e, "cudaSetDevice");
-            changed = true;
-        }
-        return POVS_OK;
-    }
-    ~DeviceGuard()
-    {
-        if (changed) cudaSetDevice(prev);
-    }
-};
 
 int set_smem_attr_all(int smem)
 {

@@ -11,6 +11,7 @@ import json
 import os
 import shutil
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -21,9 +22,14 @@ LIB_PATH = PKG_DIR / LIB_NAME
 BUILD_PARAMS_PATH = PKG_DIR / "build_params.json"
 CUDA_ARCH = "100a"
 
-SOURCES = [CSRC_DIR / "povs_abi.cu"]
-DEPENDS = [*SOURCES, CSRC_DIR / "povs_kernel.cuh", CSRC_DIR / "povs_rng.cuh", CSRC_DIR / "povs_metrics.cuh",
-           CSRC_DIR / "povs_mt19937.h", INCLUDE_DIR / "povs.h"]
+_HOST = [CSRC_DIR / "povs_host.h", INCLUDE_DIR / "povs.h"]
+# Each source is compiled on its own (the shuffle kernels take minutes, the others seconds), with
+# the headers whose change makes its object stale.
+SOURCES = {
+    CSRC_DIR / "povs_abi.cu": [*_HOST, CSRC_DIR / "povs_kernel.cuh", CSRC_DIR / "povs_rng.cuh",
+                               CSRC_DIR / "povs_metrics.cuh", CSRC_DIR / "povs_mt19937.h"],
+}
+OBJECT_DIR = PKG_DIR.parent / "build"
 
 
 def _nvcc() -> str:
@@ -37,31 +43,23 @@ def _nvcc() -> str:
     return found
 
 
-def nvcc_command(output: Path = LIB_PATH, debug: bool = False) -> list[str]:
-    cmd = [
-        _nvcc(),
-        "-gencode",
-        f"arch=compute_{CUDA_ARCH},code=sm_{CUDA_ARCH}",
-        "-lineinfo",
-        "-std=c++17",
-        "-Xcompiler",
-        "-fPIC",
-        "-shared",
-        "-O3",
-        "-o",
-        str(output),
-        *(str(s) for s in SOURCES),
-    ]
-    if debug:
-        cmd.insert(-len(SOURCES), "-DPOVS_DEBUG=1")
-    return cmd
+def _flags(debug: bool) -> list[str]:
+    flags = ["-gencode", f"arch=compute_{CUDA_ARCH},code=sm_{CUDA_ARCH}", "-lineinfo", "-std=c++17",
+             "-Xcompiler", "-fPIC", "-O3"]
+    return flags + (["-DPOVS_DEBUG=1"] if debug else [])
+
+
+def _object(source: Path, debug: bool) -> Path:
+    return OBJECT_DIR / f"{source.stem}{'_debug' if debug else ''}.o"
+
+
+def _newer(target: Path, deps) -> bool:
+    return target.exists() and all(d.stat().st_mtime <= target.stat().st_mtime for d in deps)
 
 
 def is_stale() -> bool:
-    if not LIB_PATH.exists() or not BUILD_PARAMS_PATH.exists():
-        return True
-    built = LIB_PATH.stat().st_mtime
-    return any(dep.stat().st_mtime > built for dep in DEPENDS)
+    deps = [d for source, headers in SOURCES.items() for d in (source, *headers)]
+    return not BUILD_PARAMS_PATH.exists() or not _newer(LIB_PATH, deps)
 
 
 def write_build_params(debug: bool = False) -> None:
@@ -78,16 +76,27 @@ def write_build_params(debug: bool = False) -> None:
     BUILD_PARAMS_PATH.write_text(json.dumps(params, indent=2) + "\n")
 
 
+def _run(cmd: list[str], output: Path, verbose: bool) -> None:
+    """Run ``cmd + ["-o", <temporary>]`` and move the result to ``output``."""
+    tmp = output.with_suffix(f"{output.suffix}.{os.getpid()}.tmp")
+    cmd = [*cmd, "-o", str(tmp)]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, output)
+
+
 def build(force: bool = False, verbose: bool = False, debug: bool = False) -> Path:
     """Compile the library in place (next to this file) unless it is up to date."""
     if force or is_stale():
-        cmd = nvcc_command(debug=debug)
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        tmp = LIB_PATH.with_suffix(".so.tmp")
-        cmd[cmd.index(str(LIB_PATH))] = str(tmp)
-        subprocess.run(cmd, check=True)
-        os.replace(tmp, LIB_PATH)
+        OBJECT_DIR.mkdir(exist_ok=True)
+        stale = [s for s, headers in SOURCES.items() if force or not _newer(_object(s, debug), [s, *headers])]
+        with ThreadPoolExecutor(max_workers=len(SOURCES)) as pool:
+            jobs = [pool.submit(_run, [_nvcc(), *_flags(debug), "-c", str(s)], _object(s, debug), verbose)
+                    for s in stale]
+            for job in jobs:
+                job.result()
+        _run([_nvcc(), *_flags(debug), "-shared", *(str(_object(s, debug)) for s in SOURCES)], LIB_PATH, verbose)
         write_build_params(debug)
     return LIB_PATH
 
