@@ -356,6 +356,107 @@ int povs_ngram_count_v1(const void* ids, int32_t id_bytes, int64_t n_episodes, i
                         int64_t n_positions, uint64_t* table, int64_t slots, uint64_t* mult, int64_t mult_bins,
                         uint64_t* overflow, int64_t overflow_cap, int32_t device, void* stream);
 
+/*
+ * Row operators whose order follows from scores.  Element types of scores and rows: */
+#define POVS_FLOAT32 0
+#define POVS_BFLOAT16 1
+#define POVS_FLOAT16 2
+
+/*
+ * Draw one id per row from scores (all pointers are device memory; asynchronous on `stream`).
+ * Row r has the scores logits[r * row_stride + i], 0 <= i < width (strides in elements), and the
+ * number uniforms[r] (float or double: uniform_bytes 4 or 8; taken into [0, 1)).  NaN and -infinity
+ * are never drawn.  With the weights w_i = exp((x_i - max x) / temperature) and the ids in
+ * descending order of their score, equal scores by the lowest id:
+ *   top_k > 0   keeps the first top_k ids;
+ *   top_p < 1   keeps, of those, each id before which the kept weights sum to less than top_p of
+ *               their whole sum (the first always);
+ *   min_p > 0   keeps, of those, the ids with w_i >= min_p (the highest score's always).
+ * ids[r] is the lowest id at which the kept weights, summed in id order, exceed uniforms[r] of their
+ * whole sum.  temperature 0 (in the array: any value not above 0, or NaN): the lowest id of the
+ * highest score.  Where some scores are +infinity, they alone have a weight, each the same.  A row without a
+ * number above -infinity gets -1.  temperatures, top_ks, top_ps and min_ps are NULL or hold one value
+ * per row in place of the value beside them.  Sums are whole numbers (weights in units of
+ * 2^-(62 - log2 width), at most 2^-52), so the id is the same on every run.
+ * No reference counterpart: numpy.random.Generator.choice beside its Generator.shuffle baseline.
+ */
+int povs_sample_v1(const void* logits, int32_t dtype, int64_t rows, int64_t width, int64_t row_stride,
+                   const void* uniforms, int32_t uniform_bytes, const float* temperatures, double temperature,
+                   const int32_t* top_ks, int64_t top_k, const float* top_ps, double top_p, const float* min_ps,
+                   double min_p, int64_t* ids, int32_t device, void* stream);
+
+/*
+ * Choose top_k experts for every row from its scores (device memory; asynchronous on `stream`).
+ * Scores s = softmax or sigmoid of the row's logits; choice scores c = s + bias (bias: n_experts
+ * floats or NULL; it moves the choice and not the weights).  With top_groups < n_groups, the experts
+ * form n_groups groups of n_experts / n_groups neighbours; a group scores the sum of its two highest
+ * choice scores (POVS_GROUP_TOP2) or its highest (POVS_GROUP_MAX), and only the top_groups best
+ * groups' experts can be chosen.  experts[r * top_k + j]: the j-th highest c, equal ones by the lowest
+ * index; weights[r * top_k + j] = scale * s of it, divided by the sum of the row's chosen s with
+ * renormalize.  Choices are made on scores computed in 64 bits.  An expert whose logit or choice
+ * score is -infinity is never chosen; a row with fewer than top_k others ends with experts -1 of
+ * weight 0.  A NaN score ranks below every number.  No reference counterpart.
+ */
+#define POVS_SCORE_SOFTMAX 0
+#define POVS_SCORE_SIGMOID 1
+#define POVS_GROUP_TOP2 0
+#define POVS_GROUP_MAX 1
+#define POVS_MAX_ROUTE_EXPERTS 1024
+#define POVS_MAX_TOP_K 32
+int povs_route_v1(const void* logits, int32_t dtype, int64_t rows, int32_t n_experts, int64_t row_stride,
+                  const float* bias, int32_t top_k, int32_t scoring, int32_t n_groups, int32_t top_groups,
+                  int32_t group_score, int32_t renormalize, float scale, int32_t* experts, float* weights,
+                  int32_t device, void* stream);
+
+/* Gradient of povs_route_v1's weights: grad_logits (rows, n_experts), contiguous, of the logits'
+ * type, from `experts` as povs_route_v1 wrote them and grad_weights (rows, top_k). */
+int povs_route_backward_v1(const void* logits, int32_t dtype, int64_t rows, int32_t n_experts, int64_t row_stride,
+                           int32_t top_k, int32_t scoring, int32_t renormalize, float scale, const int32_t* experts,
+                           const float* grad_weights, void* grad_logits, int32_t device, void* stream);
+
+/*
+ * The order that brings rows with the same expert together (device memory; asynchronous on
+ * `stream`): a stable counting sort of n_entries = rows * top_k expert numbers (int32 or int64:
+ * id_bytes 4 or 8).  slots[i]: the place of entry i, sources[slot]: the entry there, offsets[e]: the
+ * first slot of expert e (n_experts + 1 numbers).  Within an expert, entries keep their order.  An
+ * entry outside 0 .. n_experts-1 (-1 by convention) takes no slot: slots -1, and as many sources at
+ * the end are -1.  `workspace` (device) holds povs_plan_rows_workspace_v1 bytes (NULL where that is
+ * 0) and belongs to the call until the stream has run it.  No reference counterpart.
+ */
+#define POVS_MAX_PLAN_EXPERTS 4096
+int64_t povs_plan_rows_workspace_v1(int64_t n_entries, int32_t n_experts);
+int povs_plan_rows_v1(const void* experts, int32_t id_bytes, int64_t n_entries, int32_t n_experts, int32_t* slots,
+                      int32_t* sources, int32_t* offsets, void* workspace, int64_t workspace_bytes, int32_t device,
+                      void* stream);
+
+/*
+ * Copy rows to their slots (device memory; asynchronous on `stream`): row r (row_bytes opaque bytes
+ * at data + r * row_stride, bytes) to out + slot * row_bytes for each of slots[r * top_k ..
+ * + top_k - 1] in 0 .. n_slots-1.  The rows of `out` from *used (device) on are zeroed.  `out`
+ * must not overlap `data`.  No reference counterpart (its moves are in place).
+ */
+int povs_dispatch_rows_v1(const void* data, int64_t rows, int64_t row_bytes, int64_t row_stride,
+                          const int32_t* slots, int32_t top_k, const int32_t* used, void* out, int64_t n_slots,
+                          int32_t device, void* stream);
+
+/*
+ * Weighted sums of slots (device memory; asynchronous on `stream`): out[r] = sum over j of
+ * weights[r * top_k + j] * data[slots[r * top_k + j]] (weights NULL: ones), summed in 32 bits in the
+ * order of j and rounded once.  data: n_slots rows of `width` elements, data_stride elements apart;
+ * out: contiguous.  Slots outside 0 .. n_slots-1 are left out; a row without a slot is 0.
+ * No reference counterpart.
+ */
+int povs_combine_rows_v1(const void* data, int32_t dtype, int64_t n_slots, int64_t width, int64_t data_stride,
+                         const int32_t* slots, int64_t rows, int32_t top_k, const float* weights, void* out,
+                         int32_t device, void* stream);
+
+/* Gradients of povs_combine_rows_v1 from grad (rows, width), contiguous: grad_data (n_slots, width),
+ * contiguous, or NULL, where the slots from *used on are zeroed; grad_weights (rows, top_k), or NULL. */
+int povs_combine_backward_v1(const void* grad, const void* data, int32_t dtype, int64_t n_slots, int64_t width,
+                             int64_t data_stride, const int32_t* slots, int64_t rows, int32_t top_k,
+                             const float* weights, const int32_t* used, void* grad_data, float* grad_weights,
+                             int32_t device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

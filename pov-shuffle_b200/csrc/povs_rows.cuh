@@ -1,0 +1,598 @@
+// Row operators whose order follows from scores: choosing experts for each row (route), the stable
+// counting sort of the choices (plan), and the move of the rows into that order and back (dispatch,
+// combine), with their gradients.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+namespace povs {
+
+// ------------------------------------------------------------------------------------------
+// Element types.
+// ------------------------------------------------------------------------------------------
+
+template <typename T> __device__ __forceinline__ float to_float(T v);
+template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
+
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+// `BYTES` bytes as one load or store; wider than the element's alignment only where the host has
+// checked that every address is a multiple of it.
+template <int BYTES> struct Piece;
+template <> struct Piece<16> { using type = uint4; };
+template <> struct Piece<8> { using type = uint2; };
+template <> struct Piece<4> { using type = uint32_t; };
+template <> struct Piece<2> { using type = uint16_t; };
+template <> struct Piece<1> { using type = uint8_t; };
+
+constexpr unsigned FULL_WARP = 0xffffffffu;
+
+// ------------------------------------------------------------------------------------------
+// Route.
+// ------------------------------------------------------------------------------------------
+
+struct RouteParams {
+    const void* logits; // row r, expert e at logits[r * row_stride + e]
+    const float* bias;  // n_experts, or NULL
+    int64_t rows;
+    int64_t row_stride; // elements
+    int32_t n_experts;
+    int32_t top_k;
+    int32_t sigmoid;
+    int32_t n_groups;
+    int32_t top_groups;
+    int32_t group_max; // a group's score: 1 its highest choice score, 0 the sum of its two highest
+    int32_t renormalize;
+    float scale;
+    int32_t* experts;
+    float* weights;
+    // Backward only.
+    const int32_t* chosen;
+    const float* grad_weights;
+    void* grad_logits; // contiguous
+};
+
+// Order of choice scores as an unsigned number: 0 for what cannot be chosen, 1 for NaN, then the
+// numbers from -infinity up (+0 and -0 are the same number).
+__device__ __forceinline__ uint64_t order_key(double v)
+{
+    if (v != v) return 1;
+    const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v + 0.0));
+    return (b >> 63) ? ~b : (b | 0x8000000000000000ull);
+}
+
+// The largest key of the warp and the lowest index that has it.
+__device__ __forceinline__ void warp_best(uint64_t& key, int& index)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const uint64_t k = __shfl_xor_sync(FULL_WARP, key, o);
+        const int i = __shfl_xor_sync(FULL_WARP, index, o);
+        if (k > key || (k == key && i < index)) {
+            key = k;
+            index = i;
+        }
+    }
+}
+
+// One warp per row, EPL scores per lane (expert lane + 32 * m).
+template <typename T, int EPL>
+__global__ void __launch_bounds__(128) povs_route_kernel(const __grid_constant__ RouteParams p)
+{
+    const int lane = threadIdx.x & 31;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    if (row >= p.rows) return;
+    const T* x = static_cast<const T*>(p.logits) + row * p.row_stride;
+    const int n = p.n_experts;
+
+    double s[EPL];
+    bool open[EPL]; // can be chosen
+#pragma unroll
+    for (int m = 0; m < EPL; ++m) {
+        const int e = lane + 32 * m;
+        s[m] = e < n ? static_cast<double>(to_float(x[e])) : -INFINITY;
+        open[m] = e < n && s[m] != -INFINITY;
+    }
+    if (p.sigmoid) {
+#pragma unroll
+        for (int m = 0; m < EPL; ++m) s[m] = 1.0 / (1.0 + exp(-s[m]));
+    } else {
+        double top = -INFINITY;
+#pragma unroll
+        for (int m = 0; m < EPL; ++m) top = fmax(top, s[m]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(FULL_WARP, top, o));
+        if (top == -INFINITY) top = 0.0; // every expert masked, or NaN: exp(-inf) = 0 and NaN stays
+        double sum = 0.0;
+#pragma unroll
+        for (int m = 0; m < EPL; ++m) {
+            s[m] = exp(s[m] - top);
+            sum += s[m];
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL_WARP, sum, o);
+        const double inv = 1.0 / sum;
+#pragma unroll
+        for (int m = 0; m < EPL; ++m) s[m] = open[m] ? s[m] * inv : 0.0;
+    }
+
+    uint64_t key[EPL];
+#pragma unroll
+    for (int m = 0; m < EPL; ++m) {
+        const int e = lane + 32 * m;
+        const double c = p.bias != nullptr && e < n ? s[m] + static_cast<double>(p.bias[e]) : s[m];
+        key[m] = open[m] && c != -INFINITY ? order_key(c) : 0;
+    }
+    if (p.top_groups < p.n_groups) {
+        // Lane g scores group g.  A masked expert counts as -infinity.
+        const int size = n / p.n_groups;
+        uint64_t mine = 0;
+        for (int g = 0; g < p.n_groups; ++g) {
+            uint64_t first = 0, second = 0;
+            int at = n;
+#pragma unroll
+            for (int m = 0; m < EPL; ++m) {
+                const int e = lane + 32 * m;
+                if (e >= g * size && e < (g + 1) * size) {
+                    if (key[m] > first || at == n) {
+                        second = first;
+                        first = key[m];
+                        at = e;
+                    } else if (key[m] > second) {
+                        second = key[m];
+                    }
+                }
+            }
+            uint64_t best = first;
+            int who = at == n ? n + lane : at;
+            warp_best(best, who);
+            uint64_t other = who == at ? second : first;
+            int unused = 0;
+            warp_best(other, unused);
+            auto value = [](uint64_t k) {
+                return k == 0 ? -INFINITY
+                     : k == 1 ? NAN
+                              : __longlong_as_double(static_cast<long long>((k >> 63) ? k & 0x7fffffffffffffffull : ~k));
+            };
+            const double score = p.group_max || size == 1 ? value(best) : value(best) + value(other);
+            if (lane == g) mine = order_key(score);
+        }
+        int before = 0;
+        for (int g = 0; g < p.n_groups; ++g) {
+            const uint64_t other = __shfl_sync(FULL_WARP, mine, g);
+            before += other > mine || (other == mine && g < lane);
+        }
+        const unsigned kept = __ballot_sync(FULL_WARP, lane < p.n_groups && before < p.top_groups);
+#pragma unroll
+        for (int m = 0; m < EPL; ++m) {
+            const int e = lane + 32 * m;
+            if (e < n && !((kept >> (e / size)) & 1)) key[m] = 0;
+        }
+    }
+
+    int my_expert = -1;
+    double my_score = 0.0, total = 0.0;
+    for (int j = 0; j < p.top_k; ++j) {
+        uint64_t best = 0;
+        int at = n;
+        double value = 0.0;
+#pragma unroll
+        for (int m = 0; m < EPL; ++m)
+            if (key[m] > best) {
+                best = key[m];
+                at = lane + 32 * m;
+                value = s[m];
+            }
+        int who = at;
+        warp_best(best, who);
+        if (best == 0) break;
+        const double score = __shfl_sync(FULL_WARP, value, who & 31);
+#pragma unroll
+        for (int m = 0; m < EPL; ++m)
+            if (lane + 32 * m == who) key[m] = 0;
+        total += score;
+        if (lane == j) {
+            my_expert = who;
+            my_score = score;
+        }
+    }
+    if (lane < p.top_k) {
+        double w = my_expert >= 0 ? my_score * static_cast<double>(p.scale) : 0.0;
+        if (p.renormalize) w = total == 0.0 ? 0.0 : w / total;
+        p.experts[row * p.top_k + lane] = my_expert;
+        p.weights[row * p.top_k + lane] = static_cast<float>(w);
+    }
+}
+
+// Gradient of the weights with respect to the scores' logits, one warp per row.  With f_j the
+// chosen scores, S their sum (1 without renormalisation) and g the weights' gradient:
+//   df_j = scale (g_j - sum_i g_i f_i / S [renormalised]) / S
+//   softmax: dx_i = s_i (df_i - sum_j f_j df_j);  sigmoid: dx_i = s_i (1 - s_i) df_i
+// (df is 0 outside the chosen experts).
+template <typename T>
+__global__ void __launch_bounds__(128) povs_route_backward_kernel(const __grid_constant__ RouteParams p)
+{
+    const int lane = threadIdx.x & 31;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    if (row >= p.rows) return;
+    const T* x = static_cast<const T*>(p.logits) + row * p.row_stride;
+    T* dx = static_cast<T*>(p.grad_logits) + row * p.n_experts;
+    const int n = p.n_experts;
+    int e = -1;
+    float g = 0.0f, v = 0.0f;
+    if (lane < p.top_k) {
+        e = p.chosen[row * p.top_k + lane];
+        if (e < 0 || e >= n) e = -1;
+        if (e >= 0) {
+            g = p.grad_weights[row * p.top_k + lane];
+            v = to_float(x[e]);
+        }
+    }
+    float top = -INFINITY, sum = 0.0f;
+    if (!p.sigmoid) {
+        for (int i = lane; i < n; i += 32) top = fmaxf(top, to_float(x[i]));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL_WARP, top, o));
+        if (top == -INFINITY) top = 0.0f;
+        for (int i = lane; i < n; i += 32) sum += expf(to_float(x[i]) - top);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL_WARP, sum, o);
+    }
+    const float inv = 1.0f / sum;
+    const float f = e < 0 ? 0.0f : p.sigmoid ? 1.0f / (1.0f + expf(-v)) : expf(v - top) * inv;
+    auto warp_sum = [](float a) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(FULL_WARP, a, o);
+        return a;
+    };
+    float df = g * p.scale;
+    if (p.renormalize) {
+        const float total = warp_sum(f);
+        const float w = total == 0.0f ? 0.0f : f / total;
+        const float mean = warp_sum(g * w);
+        df = e < 0 || total == 0.0f ? 0.0f : (g - mean) * p.scale / total;
+    }
+    float mine, common = 0.0f;
+    if (p.sigmoid) {
+        mine = f * (1.0f - f) * df;
+    } else {
+        // Renormalised weights do not depend on a common factor of the scores: the sum is 0 exactly.
+        common = p.renormalize ? 0.0f : warp_sum(f * df);
+        mine = f * (df - common);
+    }
+    for (int i = lane; i < n; i += 32) {
+        const float xi = to_float(x[i]);
+        dx[i] = from_float<T>(common == 0.0f || xi == -INFINITY ? 0.0f : -expf(xi - top) * inv * common);
+    }
+    __syncwarp();
+    if (e >= 0) dx[e] = from_float<T>(mine);
+}
+
+// ------------------------------------------------------------------------------------------
+// Plan: stable counting sort of the chosen experts.
+// ------------------------------------------------------------------------------------------
+
+struct PlanRowsParams {
+    const void* experts; // n entries, int32 or int64
+    int32_t id_bytes;
+    int32_t n_experts;
+    int64_t n;
+    int64_t chunk;       // entries per block
+    int32_t* counts;     // [blocks][n_experts], written by the counting kernel
+    int32_t* slots;      // n
+    int32_t* sources;    // n
+    int32_t* offsets;    // n_experts + 1
+};
+
+constexpr int PLAN_MAX_EXPERTS = 4096;
+constexpr int PLAN_THREADS = 512;
+constexpr int PLAN_WARPS = PLAN_THREADS / 32;
+
+// The entry's expert, or -1 for an entry that takes no slot.
+__device__ __forceinline__ int plan_expert(const PlanRowsParams& p, int64_t i)
+{
+    const int64_t e = p.id_bytes == 4 ? static_cast<int64_t>(static_cast<const int32_t*>(p.experts)[i])
+                                      : static_cast<const int64_t*>(p.experts)[i];
+    return e >= 0 && e < p.n_experts ? static_cast<int>(e) : -1;
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) povs_plan_count_kernel(const __grid_constant__ PlanRowsParams p)
+{
+    extern __shared__ int32_t count[];
+    for (int e = threadIdx.x; e < p.n_experts; e += PLAN_THREADS) count[e] = 0;
+    __syncthreads();
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * p.chunk;
+    const int64_t last = min(first + p.chunk, p.n);
+    for (int64_t i = first + threadIdx.x; i < last; i += PLAN_THREADS) {
+        const int e = plan_expert(p, i);
+        if (e >= 0) atomicAdd(&count[e], 1);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.n_experts; e += PLAN_THREADS)
+        p.counts[static_cast<int64_t>(blockIdx.x) * p.n_experts + e] = count[e];
+}
+
+// Every block places its own entries: a slot is the expert's offset, plus the entries of the
+// blocks before, of the warps before and of the lanes before with the same expert.  Each warp takes
+// a contiguous run of the block's chunk, so the order within an expert is the entries' order
+// whatever the timing.  `warps` warps count (each holds a row of n_experts counters).
+__global__ void __launch_bounds__(PLAN_THREADS) povs_plan_place_kernel(const __grid_constant__ PlanRowsParams p, int warps)
+{
+    extern __shared__ int32_t smem[];
+    int32_t* base = smem;                  // [n_experts]: first slot of this block's entries
+    int32_t* run = smem + p.n_experts;     // [warps][n_experts]
+    __shared__ int32_t warp_total[PLAN_WARPS];
+    __shared__ int32_t used;
+    const int n_e = p.n_experts, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int blocks = gridDim.x;
+
+    for (int i = threadIdx.x; i < warps * n_e; i += PLAN_THREADS) run[i] = 0;
+    __syncthreads();
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * p.chunk;
+    const int64_t last = min(first + p.chunk, p.n);
+    const int64_t per = ((p.chunk + warps - 1) / warps + 31) / 32 * 32;
+    const int64_t w_first = first + warp * per, w_last = min(w_first + per, last);
+    if (warp < warps)
+        for (int64_t i = w_first + lane; i < w_last; i += 32) {
+            const int e = plan_expert(p, i);
+            if (e >= 0) atomicAdd(&run[warp * n_e + e], 1);
+        }
+    __syncthreads();
+
+    // Column sums: entries of the blocks before, and of all blocks.  A single block has its own.
+    for (int e0 = 0; e0 < n_e; e0 += PLAN_THREADS) {
+        const int e = e0 + threadIdx.x;
+        int32_t before = 0, all = 0;
+        if (e < n_e) {
+            if (blocks == 1) {
+                for (int w = 0; w < warps; ++w) all += run[w * n_e + e];
+            } else {
+#pragma unroll 8
+                for (int b = 0; b < blocks; ++b) {
+                    const int32_t c = p.counts[static_cast<int64_t>(b) * n_e + e];
+                    all += c;
+                    if (b < static_cast<int>(blockIdx.x)) before += c;
+                }
+            }
+        }
+        // Exclusive scan of `all` over the experts of this round.
+        int32_t inc = all;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int32_t up = __shfl_up_sync(FULL_WARP, inc, o);
+            if (lane >= o) inc += up;
+        }
+        if (lane == 31) warp_total[warp] = inc;
+        __syncthreads();
+        int32_t start = e0 == 0 ? 0 : used;
+        for (int w = 0; w < warp; ++w) start += warp_total[w];
+        const int32_t offset = start + inc - all;
+        if (e < n_e) {
+            base[e] = offset + before;
+            if (blockIdx.x == 0) {
+                p.offsets[e] = offset;
+                if (e == n_e - 1) p.offsets[n_e] = offset + all;
+            }
+        }
+        __syncthreads();
+        if (threadIdx.x == PLAN_THREADS - 1) used = start + inc;
+        __syncthreads();
+    }
+    // Counters become the first slot of each warp's entries.
+    for (int e = threadIdx.x; e < n_e; e += PLAN_THREADS) {
+        int32_t at = base[e];
+        for (int w = 0; w < warps; ++w) {
+            const int32_t c = run[w * n_e + e];
+            run[w * n_e + e] = at;
+            at += c;
+        }
+    }
+    __syncthreads();
+    if (warp < warps)
+        for (int64_t i0 = w_first; i0 < w_last; i0 += 32) {
+            const int64_t i = i0 + lane;
+            const int e = i < w_last ? plan_expert(p, i) : -1;
+            const unsigned same = __match_any_sync(FULL_WARP, e);
+            const int rank = __popc(same & ((1u << lane) - 1));
+            int slot = -1;
+            if (e >= 0) slot = run[warp * n_e + e] + rank;
+            __syncwarp();
+            if (e >= 0 && rank == 0) run[warp * n_e + e] += __popc(same);
+            __syncwarp();
+            if (i < w_last) {
+                p.slots[i] = slot;
+                if (slot >= 0) p.sources[slot] = static_cast<int32_t>(i);
+            }
+        }
+    // Slots behind the last entry have no source.
+    const int64_t stride = static_cast<int64_t>(blocks) * PLAN_THREADS;
+    for (int64_t i = used + static_cast<int64_t>(blockIdx.x) * PLAN_THREADS + threadIdx.x; i < p.n; i += stride)
+        p.sources[i] = -1;
+}
+
+// ------------------------------------------------------------------------------------------
+// Dispatch: rows copied to their slots.
+// ------------------------------------------------------------------------------------------
+
+struct DispatchParams {
+    const uint8_t* data; // row r at data + r * row_stride
+    uint8_t* out;        // slot s at out + s * row_bytes
+    const int32_t* slots; // rows * top_k
+    const int32_t* used;  // slots in use: the rows of `out` behind them are zeroed
+    int64_t rows;
+    int64_t row_bytes;
+    int64_t row_stride; // bytes
+    int64_t n_slots;
+    int32_t top_k;
+};
+
+// One warp per row and run of 32 * UNROLL pieces: read once, written to each of the row's slots.
+template <int BYTES, int UNROLL>
+__global__ void __launch_bounds__(256) povs_dispatch_kernel(const __grid_constant__ DispatchParams p)
+{
+    using V = typename Piece<BYTES>::type;
+    const int lane = threadIdx.x & 31;
+    const int64_t pieces = p.row_bytes / BYTES;
+    const int64_t runs = (pieces + 32 * UNROLL - 1) / (32 * UNROLL);
+    const int64_t warps = static_cast<int64_t>(gridDim.x) * 8;
+    const int64_t me = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    for (int64_t u = me; u < p.rows * runs; u += warps) {
+        const int64_t row = u / runs, c0 = (u % runs) * 32 * UNROLL + lane;
+        const V* src = reinterpret_cast<const V*>(p.data + row * p.row_stride);
+        V v[UNROLL];
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i)
+            if (c0 + 32 * i < pieces) v[i] = src[c0 + 32 * i];
+        for (int j0 = 0; j0 < p.top_k; j0 += 32) {
+            const int k = min(32, p.top_k - j0);
+            const int mine = lane < k ? p.slots[row * p.top_k + j0 + lane] : -1;
+            for (int j = 0; j < k; ++j) {
+                const int slot = __shfl_sync(FULL_WARP, mine, j);
+                if (slot < 0 || slot >= p.n_slots) continue;
+                V* dst = reinterpret_cast<V*>(p.out + slot * p.row_bytes);
+#pragma unroll
+                for (int i = 0; i < UNROLL; ++i)
+                    if (c0 + 32 * i < pieces) dst[c0 + 32 * i] = v[i];
+            }
+        }
+    }
+    const int64_t used = max(0, *p.used);
+    for (int64_t u = used * runs + me; u < p.n_slots * runs; u += warps) {
+        V* dst = reinterpret_cast<V*>(p.out + (u / runs) * p.row_bytes);
+        const int64_t c0 = (u % runs) * 32 * UNROLL + lane;
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i)
+            if (c0 + 32 * i < pieces) dst[c0 + 32 * i] = V{};
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// Combine: weighted sums of each row's slots, and the gradients.
+// ------------------------------------------------------------------------------------------
+
+struct CombineParams {
+    const void* data;      // slot s at data + s * data_stride elements
+    const int32_t* slots;  // rows * top_k
+    const float* weights;  // rows * top_k, or NULL for ones
+    void* out;             // rows, contiguous
+    int64_t rows;
+    int64_t width;
+    int64_t data_stride;   // elements
+    int64_t n_slots;
+    int32_t top_k;
+    // Backward only.
+    const int32_t* used;
+    const void* grad;      // rows, contiguous
+    void* grad_data;       // n_slots rows, contiguous, or NULL
+    float* grad_weights;   // rows * top_k, or NULL
+};
+
+template <typename T, int N> struct alignas(N * sizeof(T)) Lanes {
+    T v[N];
+};
+
+// One warp per row and run of 32 * N elements; sums in 32 bits, rounded once.
+template <typename T, int N>
+__global__ void __launch_bounds__(256) povs_combine_kernel(const __grid_constant__ CombineParams p)
+{
+    using V = Lanes<T, N>;
+    const int lane = threadIdx.x & 31;
+    const int64_t pieces = p.width / N;
+    const int64_t runs = (pieces + 31) / 32;
+    const int64_t warps = static_cast<int64_t>(gridDim.x) * 8;
+    for (int64_t u = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); u < p.rows * runs; u += warps) {
+        const int64_t row = u / runs, c = (u % runs) * 32 + lane;
+        float sum[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum[i] = 0.0f;
+        for (int j0 = 0; j0 < p.top_k; j0 += 32) {
+            const int k = min(32, p.top_k - j0);
+            int mine = -1;
+            float weight = 1.0f;
+            if (lane < k) {
+                mine = p.slots[row * p.top_k + j0 + lane];
+                if (p.weights != nullptr) weight = p.weights[row * p.top_k + j0 + lane];
+            }
+#pragma unroll 4
+            for (int j = 0; j < k; ++j) {
+                const int slot = __shfl_sync(FULL_WARP, mine, j);
+                const float w = __shfl_sync(FULL_WARP, weight, j);
+                if (slot < 0 || slot >= p.n_slots || c >= pieces) continue;
+                const V y = reinterpret_cast<const V*>(static_cast<const T*>(p.data) + slot * p.data_stride)[c];
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum[i] = fmaf(w, to_float(y.v[i]), sum[i]);
+            }
+        }
+        if (c < pieces) {
+            V o;
+#pragma unroll
+            for (int i = 0; i < N; ++i) o.v[i] = from_float<T>(sum[i]);
+            reinterpret_cast<V*>(static_cast<T*>(p.out) + row * p.width)[c] = o;
+        }
+    }
+}
+
+constexpr int COMBINE_BACKWARD_THREADS = 128;
+
+// One block per row and slot column j: grad_data[slot] = w grad[row], grad_weights = <data[slot], grad[row]>.
+// Behind the rows' blocks come blocks that zero the unused slots of grad_data.
+template <typename T, int N>
+__global__ void __launch_bounds__(COMBINE_BACKWARD_THREADS)
+    povs_combine_backward_kernel(const __grid_constant__ CombineParams p)
+{
+    using V = Lanes<T, N>;
+    __shared__ float part[COMBINE_BACKWARD_THREADS / 32];
+    const int64_t pieces = p.width / N;
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const V* g = reinterpret_cast<const V*>(static_cast<const T*>(p.grad) + row * p.width);
+        for (int j = 0; j < p.top_k; ++j) {
+            const int slot = p.slots[row * p.top_k + j];
+            const bool there = slot >= 0 && slot < p.n_slots;
+            const float w = p.weights != nullptr ? p.weights[row * p.top_k + j] : 1.0f;
+            float dot = 0.0f;
+            if (there)
+                for (int64_t c = threadIdx.x; c < pieces; c += COMBINE_BACKWARD_THREADS) {
+                    const V a = g[c];
+                    if (p.grad_weights != nullptr) {
+                        const V y = reinterpret_cast<const V*>(static_cast<const T*>(p.data) + slot * p.data_stride)[c];
+#pragma unroll
+                        for (int i = 0; i < N; ++i) dot = fmaf(to_float(a.v[i]), to_float(y.v[i]), dot);
+                    }
+                    if (p.grad_data != nullptr) {
+                        V o;
+#pragma unroll
+                        for (int i = 0; i < N; ++i) o.v[i] = from_float<T>(w * to_float(a.v[i]));
+                        reinterpret_cast<V*>(static_cast<T*>(p.grad_data) + slot * p.width)[c] = o;
+                    }
+                }
+            if (p.grad_weights != nullptr) {
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(FULL_WARP, dot, o);
+                if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = dot;
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    float total = 0.0f;
+                    for (int i = 0; i < COMBINE_BACKWARD_THREADS / 32; ++i) total += part[i];
+                    p.grad_weights[row * p.top_k + j] = total;
+                }
+                __syncthreads();
+            }
+        }
+    }
+    if (p.grad_data == nullptr) return;
+    const int64_t used = max(0, *p.used);
+    for (int64_t s = used + blockIdx.x; s < p.n_slots; s += gridDim.x) {
+        V* dst = reinterpret_cast<V*>(static_cast<T*>(p.grad_data) + s * p.width);
+        for (int64_t c = threadIdx.x; c < pieces; c += COMBINE_BACKWARD_THREADS) dst[c] = V{};
+    }
+}
+
+} // namespace povs

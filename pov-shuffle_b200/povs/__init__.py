@@ -6,8 +6,10 @@ and per-vblock permutations, for bit-exact comparison with other implementations
 ``check_device_status``, decks split into shards: ``shuffle_shards`` (one process) and
 ``ShardedDeck`` (one process per GPU, host shards streamed through it by ``shuffle_host_shards``),
 many host decks streamed through the GPU (``shuffle_many``) and many independent CUDA decks
-shuffled together (``shuffle_batch``).  ``povs.eval`` holds the
-shuffle-bias metrics and exercises on the GPU.
+shuffled together (``shuffle_batch``).  Rows ordered by scores instead of a seed: ``sample`` (ids drawn
+from scores), ``route`` (rows to experts), ``plan_rows``, ``dispatch_rows`` and ``combine_rows`` (rows moved into
+the experts' order and back), with gradients.  ``povs.eval`` holds the shuffle-bias metrics and
+exercises on the GPU.
 """
 
 from __future__ import annotations
@@ -22,6 +24,8 @@ from . import torch as povs_torch
 from .common import get_build_params, get_int_seed
 from .distributed import ShardedDeck, shuffle_host_shards, shuffle_shards
 from .injection import apply_randomness
+from .routing import Routing, RowPlan, combine_rows, dispatch_rows, plan_rows, route
+from .sampling import sample
 from .types import BuildParams, Options
 
 __all__ = [
@@ -38,6 +42,13 @@ __all__ = [
     "shuffle_many",
     "shuffle_batch",
     "shuffle_mapped",
+    "sample",
+    "route",
+    "Routing",
+    "RowPlan",
+    "plan_rows",
+    "dispatch_rows",
+    "combine_rows",
 ]
 
 

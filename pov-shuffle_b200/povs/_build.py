@@ -28,6 +28,7 @@ _HOST = [CSRC_DIR / "povs_host.h", INCLUDE_DIR / "povs.h"]
 SOURCES = {
     CSRC_DIR / "povs_abi.cu": [*_HOST, CSRC_DIR / "povs_kernel.cuh", CSRC_DIR / "povs_rng.cuh",
                                CSRC_DIR / "povs_metrics.cuh", CSRC_DIR / "povs_mt19937.h"],
+    CSRC_DIR / "povs_rows_abi.cu": [*_HOST, CSRC_DIR / "povs_rows.cuh", CSRC_DIR / "povs_sample.cuh"],
 }
 OBJECT_DIR = PKG_DIR.parent / "build"
 

@@ -88,6 +88,39 @@ SIGNATURES: dict[str, tuple] = {
         [_c_vp, _c_i32, _c_i64, _c_i64, _c_i64, _c_i64, _c_i32, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64,
          _c_vp, _c_i64, _c_i32, _c_vp],
     ),
+    "povs_sample_v1": (
+        ctypes.c_int,
+        [_c_vp, _c_i32, _c_i64, _c_i64, _c_i64, _c_vp, _c_i32, _c_vp, ctypes.c_double, _c_vp, _c_i64, _c_vp,
+         ctypes.c_double, _c_vp, ctypes.c_double, _c_vp, _c_i32, _c_vp],
+    ),
+    "povs_route_v1": (
+        ctypes.c_int,
+        [_c_vp, _c_i32, _c_i64, _c_i32, _c_i64, _c_vp, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, ctypes.c_float,
+         _c_vp, _c_vp, _c_i32, _c_vp],
+    ),
+    "povs_route_backward_v1": (
+        ctypes.c_int,
+        [_c_vp, _c_i32, _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, ctypes.c_float, _c_vp, _c_vp, _c_vp, _c_i32,
+         _c_vp],
+    ),
+    "povs_plan_rows_workspace_v1": (ctypes.c_int64, [_c_i64, _c_i32]),
+    "povs_plan_rows_v1": (
+        ctypes.c_int,
+        [_c_vp, _c_i32, _c_i64, _c_i32, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i32, _c_vp],
+    ),
+    "povs_dispatch_rows_v1": (
+        ctypes.c_int,
+        [_c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_i32, _c_vp, _c_vp, _c_i64, _c_i32, _c_vp],
+    ),
+    "povs_combine_rows_v1": (
+        ctypes.c_int,
+        [_c_vp, _c_i32, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_i32, _c_vp, _c_vp, _c_i32, _c_vp],
+    ),
+    "povs_combine_backward_v1": (
+        ctypes.c_int,
+        [_c_vp, _c_vp, _c_i32, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_i32, _c_vp, _c_vp, _c_vp, _c_vp, _c_i32,
+         _c_vp],
+    ),
     "povs_numpy_path_perm_v1": (ctypes.c_int, [_c_u32, _c_i32, _c_vp]),
     "povs_set_peer_wait_limit_v1": (ctypes.c_int, [_c_u64]),
     "povs_apply_static_v1": (
@@ -272,6 +305,152 @@ def ngram_count(ids: torch.Tensor, n: int, step: int, positions: torch.Tensor | 
     if status:
         raise RuntimeError(f"device status 0x{status:x} after povs_ngram_count_v1 (8: the hash table was full)")
     return m, overflow[: int(m[0])].cpu().numpy().astype(np.uint64)
+
+
+# Limits and element types of the row operators (include/povs.h).
+MAX_ROUTE_EXPERTS, MAX_TOP_K, MAX_PLAN_EXPERTS = 1024, 32, 4096
+_SCORE_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def score_dtype(t: torch.Tensor) -> int:
+    """The C ABI's number of a floating element type; TypeError for one that has no kernels."""
+    code = _SCORE_DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"dtype must be float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _row_elements(data: torch.Tensor) -> int:
+    n = 1
+    for d in data.shape[1:]:
+        n *= d
+    return n
+
+
+def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature, top_k, top_p, min_p) -> torch.Tensor:
+    """``povs_sample_v1``: one int64 id per row; the four settings are numbers or per-row tensors."""
+    dev = logits.device
+    rows, width = logits.shape
+    ids = torch.empty(rows, dtype=torch.int64, device=dev)
+    per_row = [v.data_ptr() if isinstance(v, torch.Tensor) else None for v in (temperature, top_k, top_p, min_p)]
+    number = [0 if p is not None else v for p, v in zip(per_row, (temperature, top_k, top_p, min_p))]
+    check(
+        load().povs_sample_v1(
+            logits.data_ptr(), _SCORE_DTYPES[logits.dtype], rows, width, logits.stride(0), uniforms.data_ptr(),
+            uniforms.element_size(), per_row[0], number[0], per_row[1], int(number[1]), per_row[2], number[2],
+            per_row[3], number[3], ids.data_ptr(), dev.index, current_stream_handle(dev),
+        ),
+        "povs_sample_v1",
+    )
+    return ids
+
+
+def route(logits: torch.Tensor, bias: torch.Tensor | None, top_k: int, scoring: int, n_groups: int, top_groups: int,
+          group_score: int, renormalize: bool, scale: float) -> tuple[torch.Tensor, torch.Tensor]:
+    """``povs_route_v1``: (experts int32, weights float32), both (rows, top_k)."""
+    dev = logits.device
+    rows, n = logits.shape
+    experts = torch.empty((rows, top_k), dtype=torch.int32, device=dev)
+    weights = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
+    check(
+        load().povs_route_v1(
+            logits.data_ptr(), _SCORE_DTYPES[logits.dtype], rows, n, logits.stride(0),
+            None if bias is None else bias.data_ptr(), top_k, scoring, n_groups, top_groups, group_score, renormalize,
+            scale, experts.data_ptr(), weights.data_ptr(), dev.index, current_stream_handle(dev),
+        ),
+        "povs_route_v1",
+    )
+    return experts, weights
+
+
+def route_backward(logits: torch.Tensor, experts: torch.Tensor, grad_weights: torch.Tensor, scoring: int,
+                   renormalize: bool, scale: float) -> torch.Tensor:
+    """``povs_route_backward_v1``: the gradient of the logits, contiguous."""
+    dev = logits.device
+    rows, n = logits.shape
+    grad = torch.empty((rows, n), dtype=logits.dtype, device=dev)
+    check(
+        load().povs_route_backward_v1(
+            logits.data_ptr(), _SCORE_DTYPES[logits.dtype], rows, n, logits.stride(0), experts.shape[1], scoring,
+            renormalize, scale, experts.data_ptr(), grad_weights.data_ptr(), grad.data_ptr(), dev.index,
+            current_stream_handle(dev),
+        ),
+        "povs_route_backward_v1",
+    )
+    return grad
+
+
+def plan_rows(experts: torch.Tensor, n_experts: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``povs_plan_rows_v1``: (slots, sources, offsets) as int32 tensors."""
+    lib = load()
+    dev = experts.device
+    n = experts.numel()
+    slots = torch.empty(experts.shape, dtype=torch.int32, device=dev)
+    sources = torch.empty(n, dtype=torch.int32, device=dev)
+    offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=dev)
+    need = lib.povs_plan_rows_workspace_v1(n, n_experts)
+    check(need, "povs_plan_rows_workspace_v1")
+    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    check(
+        lib.povs_plan_rows_v1(
+            experts.data_ptr(), experts.element_size(), n, n_experts, slots.data_ptr(), sources.data_ptr(),
+            offsets.data_ptr(), None if work is None else work.data_ptr(), need, dev.index, current_stream_handle(dev),
+        ),
+        "povs_plan_rows_v1",
+    )
+    return slots, sources, offsets
+
+
+def dispatch_rows(data: torch.Tensor, slots: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    """``povs_dispatch_rows_v1``: the rows of ``data`` in the order of ``slots``, zeros behind ``offsets[-1]``."""
+    dev = data.device
+    rows, k = slots.shape
+    size = data.element_size()
+    out = torch.empty((rows * k, *data.shape[1:]), dtype=data.dtype, device=dev)
+    check(
+        load().povs_dispatch_rows_v1(
+            data.data_ptr(), rows, _row_elements(data) * size, data.stride(0) * size, slots.data_ptr(), k,
+            offsets.data_ptr() + 4 * (offsets.numel() - 1), out.data_ptr(), rows * k, dev.index,
+            current_stream_handle(dev),
+        ),
+        "povs_dispatch_rows_v1",
+    )
+    return out
+
+
+def combine_rows(data: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor | None) -> torch.Tensor:
+    """``povs_combine_rows_v1``: weighted sums of each row's slots."""
+    dev = data.device
+    rows, k = slots.shape
+    out = torch.empty((rows, *data.shape[1:]), dtype=data.dtype, device=dev)
+    check(
+        load().povs_combine_rows_v1(
+            data.data_ptr(), _SCORE_DTYPES[data.dtype], data.shape[0], _row_elements(data), data.stride(0),
+            slots.data_ptr(), rows, k, None if weights is None else weights.data_ptr(), out.data_ptr(), dev.index,
+            current_stream_handle(dev),
+        ),
+        "povs_combine_rows_v1",
+    )
+    return out
+
+
+def combine_backward(grad: torch.Tensor, data: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor | None,
+                     offsets: torch.Tensor, need_data: bool, need_weights: bool):
+    """``povs_combine_backward_v1``: the gradients of ``data`` and ``weights`` (None where not needed)."""
+    dev = grad.device
+    rows, k = slots.shape
+    grad_data = torch.empty(data.shape, dtype=data.dtype, device=dev) if need_data else None
+    grad_weights = torch.empty((rows, k), dtype=torch.float32, device=dev) if need_weights else None
+    check(
+        load().povs_combine_backward_v1(
+            grad.data_ptr(), data.data_ptr(), _SCORE_DTYPES[data.dtype], data.shape[0], _row_elements(data),
+            data.stride(0), slots.data_ptr(), rows, k, None if weights is None else weights.data_ptr(),
+            offsets.data_ptr() + 4 * (offsets.numel() - 1), None if grad_data is None else grad_data.data_ptr(),
+            None if grad_weights is None else grad_weights.data_ptr(), dev.index, current_stream_handle(dev),
+        ),
+        "povs_combine_backward_v1",
+    )
+    return grad_data, grad_weights
 
 
 def shuffle_host(
