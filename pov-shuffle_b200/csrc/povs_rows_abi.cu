@@ -158,6 +158,29 @@ int check_combine(const povs::CombineParams& p, int32_t dtype)
     return POVS_OK;
 }
 
+// Blocks per row: as many as the GPU holds at once for these rows (four per SM), of 2048 ids or more.
+int sample_cluster(int64_t rows, int64_t width, int sms)
+{
+    int c = 1;
+    while (2 * c <= povs::SAMPLE_MAX_CLUSTER && rows * 2 * c <= 4 * static_cast<int64_t>(sms) && width / (2 * c) >= 2048) c *= 2;
+    return c;
+}
+
+template <typename T> cudaError_t launch_sample(const povs::SampleParams& p, cudaStream_t s)
+{
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(p.rows * p.cluster));
+    config.blockDim = dim3(povs::SAMPLE_THREADS);
+    config.stream = s;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = static_cast<unsigned>(p.cluster);
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = p.cluster > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&config, povs::povs_sample_kernel<T>, p);
+}
+
 } // namespace
 
 extern "C" int povs_sample_v1(const void* logits, int32_t dtype, int64_t rows, int64_t width, int64_t row_stride,
@@ -206,11 +229,12 @@ extern "C" int povs_sample_v1(const void* logits, int32_t dtype, int64_t rows, i
     p.min_p = min_p;
     p.ids = ids;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const unsigned grid = static_cast<unsigned>(rows);
-    if (dtype == POVS_FLOAT32) povs::povs_sample_kernel<float><<<grid, povs::SAMPLE_THREADS, 0, s>>>(p);
-    else if (dtype == POVS_BFLOAT16) povs::povs_sample_kernel<__nv_bfloat16><<<grid, povs::SAMPLE_THREADS, 0, s>>>(p);
-    else povs::povs_sample_kernel<__half><<<grid, povs::SAMPLE_THREADS, 0, s>>>(p);
-    return launched("sample kernel");
+    p.cluster = sample_cluster(rows, width, sms);
+    cudaError_t e;
+    if (dtype == POVS_FLOAT32) e = launch_sample<float>(p, s);
+    else if (dtype == POVS_BFLOAT16) e = launch_sample<__nv_bfloat16>(p, s);
+    else e = launch_sample<__half>(p, s);
+    return e == cudaSuccess ? launched("sample kernel") : cuda_fail(e, "sample kernel");
 }
 
 extern "C" int povs_route_v1(const void* logits, int32_t dtype, int64_t rows, int32_t n_experts, int64_t row_stride,
