@@ -13,6 +13,7 @@
 
 #include <cfloat>
 #include <cstdint>
+#include <type_traits>
 
 #include "povs_rows.cuh"
 
@@ -174,6 +175,9 @@ struct SampleShared {
     double part_mass[SAMPLE_WARPS];
     unsigned int probe_counts[16];
     uint32_t probe_low;
+    uint32_t lowest;
+    int few;
+    int few_at[32];
     unsigned long long found;
     unsigned long long left;
 };
@@ -390,36 +394,28 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
         for (int w = 0; w < SAMPLE_WARPS; ++w) s += sh.part[w];
         return s;
     };
-    // The first of `bins` bins, from the top, at which the running sum reaches `want`; its number in
-    // sh.found (-1: never) and what is left of `want` in it in sh.left.
-    auto crossing = [&](int bins, bool descending, unsigned long long want) {
-        if (warp == 0) {
-            const int per = bins / 32;
-            unsigned long long mine = 0;
-            for (int b = 0; b < per; ++b) {
-                const int at = lane * per + b;
-                mine += sh.bins[descending ? bins - 1 - at : at];
-            }
-            const unsigned long long upto = warp_inclusive(mine, lane);
-            const unsigned hit = __ballot_sync(FULL_WARP, upto >= want);
-            if (hit == 0) {
-                if (lane == 0) sh.found = ~0ull;
-            } else if (lane == __ffs(hit) - 1) {
-                unsigned long long left = want - (upto - mine);
-                for (int b = 0; b < per; ++b) {
-                    const int at = descending ? bins - 1 - (lane * per + b) : lane * per + b;
-                    if (sh.bins[at] >= left) {
-                        sh.found = at;
-                        break;
-                    }
-                    left -= sh.bins[at];
-                }
-                sh.left = left;
-            }
+    // The first bin at which the running sum over sh.bins reaches `want`: its number in sh.found (~0:
+    // none) and what is left of `want` in it in sh.left.
+    auto crossing = [&](auto bins, unsigned long long want) {
+        constexpr int PER = decltype(bins)::value / SAMPLE_THREADS;
+        unsigned long long mine = 0;
+#pragma unroll
+        for (int b = 0; b < PER; ++b) mine += sh.bins[t * PER + b];
+        unsigned long long upto = warp_inclusive(mine, lane);
+        if (lane == 31) sh.part[warp] = upto;
+        if (t == 0) sh.found = ~0ull;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) upto += sh.part[w];
+        if (upto >= want && upto - mine < want) {
+            unsigned long long left = want - (upto - mine);
+            int at = t * PER;
+            while (sh.bins[at] < left) left -= sh.bins[at++];
+            sh.found = at;
+            sh.left = left;
         }
         __syncthreads();
     };
-    // Of the list's members, from the highest entry down, the one at which the running sum of `amount`
+    // Of the list's first n entries, from the highest down, the one at which the running sum of `amount`
     // reaches `want`, digit by digit; 0 where the whole sum stays below.  by_id looks at the lower
     // half (~id) alone: ids in ascending order.
     auto select = [&](int n, bool by_id, unsigned long long want, auto&& amount) -> unsigned long long {
@@ -435,16 +431,59 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
                 const unsigned long long c = by_id ? sh.list[i] & 0xffffffffull : sh.list[i];
                 if (shift < 56 && (c >> (shift + 8)) != prefix) continue;
                 const unsigned long long a = amount(i);
-                if (a != 0) atomicAdd(&sh.bins[(c >> shift) & 255], a);
+                if (a != 0) atomicAdd(&sh.bins[255 - ((c >> shift) & 255)], a);
             }
             __syncthreads();
-            crossing(256, true, want);
-            if (sh.found == ~0ull) return 0;
-            prefix = (prefix << 8) | sh.found;
+            crossing(std::integral_constant<int, 256>{}, want);
+            const unsigned long long found = sh.found;
             want = sh.left;
             __syncthreads();
+            if (found == ~0ull) return 0;
+            prefix = (prefix << 8) | (255 - found);
         }
         return prefix;
+    };
+    // The same by bins of a number that does not rise along the order (bin_of: a bin for an entry): one
+    // round of sums, then the few entries of the bin that holds the border.  Where those are more than
+    // a warp has lanes, digit by digit.
+    auto border_of = [&](int n, bool by_id, unsigned long long want, auto&& bin_of, auto&& amount) -> unsigned long long {
+        for (int b = t; b < SAMPLE_BINS; b += SAMPLE_THREADS) sh.bins[b] = 0;
+        if (t == 0) sh.few = 0;
+        __syncthreads();
+        for (int i = t; i < n; i += SAMPLE_THREADS) {
+            const unsigned long long a = amount(i);
+            if (a != 0) atomicAdd(&sh.bins[bin_of(sh.list[i])], a);
+        }
+        __syncthreads();
+        crossing(std::integral_constant<int, SAMPLE_BINS>{}, want);
+        const unsigned long long found = sh.found, left = sh.left;
+        if (found == ~0ull) {
+            __syncthreads();
+            return 0;
+        }
+        for (int i = t; i < n; i += SAMPLE_THREADS)
+            if (bin_of(sh.list[i]) == static_cast<int>(found) && amount(i) != 0) {
+                const int at = atomicAdd(&sh.few, 1);
+                if (at < 32) sh.few_at[at] = i;
+            }
+        __syncthreads();
+        const int few = sh.few;
+        if (few > 32) return select(n, by_id, left, [&](int i) { return bin_of(sh.list[i]) == static_cast<int>(found) ? amount(i) : 0ull; });
+        if (warp == 0) {
+            const int i = lane < few ? sh.few_at[lane] : 0;
+            const unsigned long long c = by_id ? sh.list[i] & 0xffffffffull : sh.list[i];
+            const unsigned long long a = lane < few ? static_cast<unsigned long long>(amount(i)) : 0;
+            unsigned long long before = 0;
+            for (int o = 0; o < few; ++o) {
+                const unsigned long long other = __shfl_sync(FULL_WARP, c, o), b = __shfl_sync(FULL_WARP, a, o);
+                if (other > c) before += b;
+            }
+            if (lane < few && before < left && before + a >= left) sh.found = c;
+        }
+        __syncthreads();
+        const unsigned long long entry = sh.found;
+        __syncthreads();
+        return entry;
     };
     // The other blocks' listed entries, appended to this block's (rank 0).
     auto gather = [&] {
@@ -463,13 +502,30 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
             const int n = static_cast<int>(listed);
             const bool complete = threshold == LOWEST_KEY;
             gather();
-            for (int i = t; i < n; i += SAMPLE_THREADS)
-                sh.weight[i] = score_weight(key_score(static_cast<uint32_t>(sh.list[i] >> 32)), top, inv);
+            if (t == 0) sh.lowest = 0xffffffffu;
             __syncthreads();
+            uint32_t lowest = 0xffffffffu;
+            for (int i = t; i < n; i += SAMPLE_THREADS) {
+                const uint32_t k = static_cast<uint32_t>(sh.list[i] >> 32);
+                lowest = min(lowest, k);
+                sh.weight[i] = score_weight(key_score(k), top, inv);
+            }
+            lowest = __reduce_min_sync(FULL_WARP, lowest);
+            if (lane == 0) atomicMin(&sh.lowest, lowest);
+            __syncthreads();
+            const float spread = top - key_score(sh.lowest);
+            const float per_score = spread > 0.0f ? SAMPLE_BINS / spread : 0.0f;
+            const float per_id = static_cast<float>(SAMPLE_BINS) / static_cast<float>(p.width);
+            auto score_bin = [&](unsigned long long c) {
+                return min(SAMPLE_BINS - 1, static_cast<int>((top - key_score(static_cast<uint32_t>(c >> 32))) * per_score));
+            };
+            auto id_bin = [&](unsigned long long c) {
+                return min(SAMPLE_BINS - 1, static_cast<int>(static_cast<float>(~static_cast<uint32_t>(c)) * per_id));
+            };
             bool resolved = true;
             unsigned long long cut = 0; // kept are the entries from here up
             if (top_k > 0) {
-                if (n >= top_k) cut = select(n, false, static_cast<unsigned long long>(top_k), [](int) { return 1ull; });
+                if (n >= top_k) cut = border_of(n, false, static_cast<unsigned long long>(top_k), score_bin, [](int) { return 1ull; });
                 else resolved = complete;
             }
             if (resolved && nucleus) {
@@ -481,8 +537,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
                 }
                 const double want = ceil(top_p * mass * unit);
                 const unsigned long long from = cut;
-                const unsigned long long border = select(n, false, want > 1.0 ? static_cast<unsigned long long>(want) : 1ull,
-                                                         [&](int i) { return sh.list[i] >= from ? whole(sh.weight[i]) : 0ull; });
+                const unsigned long long border = border_of(n, false, want > 1.0 ? static_cast<unsigned long long>(want) : 1ull, score_bin,
+                                                            [&](int i) { return sh.list[i] >= from ? whole(sh.weight[i]) : 0ull; });
                 if (border != 0) cut = border;
                 else if (top_k == 0) resolved = complete; // every listed id is in the nucleus, and more may be
             }
@@ -500,7 +556,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
                 m = block_total(m);
                 const double target = u * static_cast<double>(m);
                 const unsigned long long want = target < static_cast<double>(m) ? min(static_cast<unsigned long long>(target) + 1, m) : m;
-                const unsigned long long at = select(n, true, want, kept);
+                const unsigned long long at = border_of(n, true, want, id_bin, kept);
                 if (t == 0) p.ids[row] = static_cast<int64_t>(~static_cast<uint32_t>(at));
             }
             if (t == 0) sh.outcome = resolved;
@@ -590,7 +646,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
             });
             __syncthreads();
             cluster_bins();
-            crossing(SAMPLE_BINS, false, left);
+            crossing(std::integral_constant<int, SAMPLE_BINS>{}, left);
             const unsigned long long found = sh.found;
             if (found == ~0ull) { // first round only: the ids above the cut do not reach `want`
                 unsigned long long sum = 0;
