@@ -228,6 +228,8 @@ extern "C" int povs_sample_v1(const void* logits, int32_t dtype, int64_t rows, i
     p.top_p = top_p;
     p.min_p = min_p;
     p.ids = ids;
+    double term = 1.0;
+    for (int i = 0; i < 5; ++i) p.taylor[i] = term *= 0.69314718055994530942 / (i + 1);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     p.cluster = sample_cluster(rows, width, sms);
     cudaError_t e;

@@ -40,6 +40,7 @@ struct SampleParams {
     double min_p;
     int64_t top_k;
     int64_t* ids;
+    double taylor[5]; // (ln 2)^i / i!, i = 1 .. 5: in constant memory, where an operand costs no register
 };
 
 constexpr int SAMPLE_THREADS = 256;
@@ -63,40 +64,50 @@ __device__ __forceinline__ float key_score(uint32_t k) { return __uint_as_float(
 
 constexpr uint32_t LOWEST_KEY = 0x00800000u; // the lowest finite score's
 
-// Weights of many scores, for loops that a whole warp runs together: exp((v - reference) * inv) to
-// 2^-48 relative.  With z = (v - reference) * inv / ln 2 = n / 32 + r, |r| <= 1/64, it is
-// 2^(n >> 5) * 2^((n & 31) / 32) * 2^r: the second factor sits in the lanes' registers (one shuffle in place of a
-// table in memory, whose banks would clash), and 2^r is its Taylor polynomial of degree 5 (the next
-// term is (r ln 2)^6 / 720 < 2.3e-15).  12 operations in 64 bits a score, about what the scores' 4
-// bytes cost to read.
+// A highest score below this, or +infinity, leaves weights to the scores equal to it alone: float's
+// next lower score is 2^104 away, which the highest temperature that counts (1e28) makes 2000.
+constexpr float LONE = -3.0e38f;
+
+// Weights of many scores, for loops that a whole warp runs together: exp((v - reference) * inv) up to
+// a factor common to all, to 2^-48 relative.  With z = v * inv / ln 2 = n / 32 + r, |r| <= 1/64, and n0
+// the n of the reference, the weight is 2^((n - n0) >> 5) * 2^(((n - n0) & 31) / 32) * 2^r: the second
+// factor sits in the lanes' registers (one shuffle in place of a table in memory, whose banks would
+// clash), and 2^r is its Taylor polynomial of degree 5 (the next term is (r ln 2)^6 / 720 < 2.3e-15).
+// The products with inv / ln 2 are exact in both fused operations, so large scores lose nothing.
+// Ten operations in 64 bits a score: at half the rate of 32 bits about what its 4 bytes cost to read.
+// Scores 500 or more below the reference in z, NaN and -infinity weigh 2^-500 to 2^-1000: nothing beside
+// the highest score's.  References stay above LONE, where the float 500 below exists.
 struct WarpExp {
-    double step;  // 2^(lane / 32)
-    double scale; // inv / ln 2
-    float scale_f;
-    __device__ WarpExp(double inv_temperature, int lane)
+    double step;   // 2^(lane / 32)
+    double scale;  // inv / ln 2, or so much that one of float's steps at the reference makes 250
+    double magic;  // rounds to steps of 1/32, less n0
+    double factor; // times this, a weight is relative to the reference
+    float floor;
+    __device__ WarpExp(int lane) : step(exp2(lane * 0.03125)), scale(0.0), magic(0.0), factor(0.0), floor(-INFINITY) {}
+    __device__ __forceinline__ void refer(float reference, double inv)
     {
-        step = exp2(lane * 0.03125);
-        scale = inv_temperature * 1.4426950408889634074;
-        scale_f = static_cast<float>(scale);
-    }
-    // 0 for NaN, -infinity and what is below 2^-1000.
-    __device__ __forceinline__ double operator()(float v, float reference) const
-    {
-        constexpr double L = 0.69314718055994530942; // ln 2
         constexpr double MAGIC = 6755399441055744.0 / 32; // 1.5 * 2^52 steps of 1/32
-        const bool there = (v - reference) * scale_f >= -1000.0f;
-        const double d = static_cast<double>(v) - static_cast<double>(reference);
-        const double t = fma(d, scale, MAGIC);
-        const double r = fma(d, scale, -(t - MAGIC));
+        const double here = static_cast<double>(reference);
+        const double spacing = fmax(fabs(here) * 5.9604644775390625e-8, 1.401298464324817e-45);
+        scale = fmin(inv * 1.4426950408889634074, 250.0 / spacing);
+        const double n0 = rint(here * scale * 32.0);
+        magic = MAGIC - n0 * 0.03125;
+        factor = exp2(fma(-here, scale, n0 * 0.03125));
+        floor = __double2float_rd(here - 500.0 / scale);
+    }
+    __device__ __forceinline__ double operator()(float v, const double* __restrict__ taylor) const
+    {
+        const double x = static_cast<double>(fmaxf(v, floor));
+        const double t = fma(x, scale, magic);
+        const double r = fma(x, scale, magic - t);
         const int n = __double2loint(t);
-        double q = fma(r, L * L * L * L * L / 120, L * L * L * L / 24);
-        q = fma(r, q, L * L * L / 6);
-        q = fma(r, q, L * L / 2);
-        q = fma(r, q, L);
-        const double base = __shfl_sync(FULL_WARP, step, n & 31);
-        const double w = fma(base * r, q, base);
-        const int hi = __double2hiint(w) + ((n >> 5) << 20);
-        return __hiloint2double(there ? hi : 0, there ? __double2loint(w) : 0);
+        double q = fma(r, taylor[4], taylor[3]);
+        q = fma(r, q, taylor[2]);
+        q = fma(r, q, taylor[1]);
+        q = fma(r, q, taylor[0]);
+        const double at = __shfl_sync(FULL_WARP, step, n & 31);
+        const double base = __hiloint2double(__double2hiint(at) + (n & ~31) * (1 << 15), __double2loint(at));
+        return fma(base * r, q, base);
     }
 };
 
@@ -173,6 +184,7 @@ struct SampleShared {
     // This block's own.
     unsigned long long part[SAMPLE_WARPS];
     double part_mass[SAMPLE_WARPS];
+    double listed_mass;
     unsigned int probe_counts[16];
     uint32_t probe_low;
     uint32_t lowest;
@@ -201,7 +213,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
     const int64_t top_k_given = p.top_ks != nullptr ? p.top_ks[row] : p.top_k;
     const int64_t top_k = top_k_given > 0 && top_k_given < p.width ? top_k_given : 0;
     const bool greedy = !(temperature > 0.0);
-    const double inv = fmin(1.0 / temperature, 1e36); // so that 0 * inv stays 0
+    const double inv = fmin(fmax(1.0 / temperature, 1e-28), 1e36); // so that 0 * inv stays 0
     const bool nucleus = top_p < 1.0, floor_p = min_p > 0.0;
     const bool filtered = !greedy && (nucleus || floor_p || top_k > 0);
     // The sum of all weights: without a filter, or for a nucleus of the whole row.
@@ -267,10 +279,10 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
         }
         threshold = max(found, LOWEST_KEY);
     }
-    const float list_from = listing ? key_score(threshold) : INFINITY; // +infinity: see `top_inf` below
+    const float list_from = listing ? key_score(threshold) : INFINITY; // +infinity: see `lone` below
 
     // The stream.
-    const WarpExp weight_of(inv, lane);
+    WarpExp weight_of(lane);
     {
         float top = -INFINITY, reference = -INFINITY, limit = -INFINITY;
         int top_group = 0;
@@ -313,12 +325,14 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
                         float higher = most;
 #pragma unroll
                         for (int o = 16; o > 0; o >>= 1) higher = fmaxf(higher, __shfl_xor_sync(FULL_WARP, higher, o));
-                        if (reference > -INFINITY) sum *= score_weight(reference, higher, inv);
+                        const double old_factor = weight_of.factor;
+                        weight_of.refer(higher, inv);
+                        sum = reference > LONE ? sum * old_factor * score_weight(reference, higher, inv) / weight_of.factor : 0.0;
                         reference = higher;
                         limit = static_cast<float>(static_cast<double>(reference) + 64.0 / inv);
                     }
 #pragma unroll
-                    for (int j = 0; j < N; ++j) sum += weight_of(v[u][j], reference);
+                    for (int j = 0; j < N; ++j) sum += weight_of(v[u][j], p.taylor);
                 }
             }
         }
@@ -337,7 +351,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
         sum = warp_sum(sum);
         if (lane == 0) {
             sh.best[warp] = best;
-            sh.mass[warp] = sum;
+            sh.mass[warp] = reference > LONE ? sum * weight_of.factor : 0.0;
             sh.reference[warp] = reference;
         }
     }
@@ -358,11 +372,11 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
         everyone();
         return;
     }
-    const bool top_inf = top == INFINITY; // those scores alone have a weight: no list, no sums
+    const bool lone = top == INFINITY || top < LONE; // no list, no sums
     double part_mass[2] = {0.0, 0.0};
     unsigned long long part_ties[2] = {0, 0};
     double total = 0.0; // sum of all weights, relative to the highest score
-    if (need_mass && !top_inf) {
+    if (need_mass && !lone) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int e = 2 * lane + h;
@@ -497,7 +511,9 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
         __syncthreads();
     };
 
-    if (listing && !top_inf && listed <= SAMPLE_LIST) {
+    double listed_mass = 0.0; // weight of the scores from `below` up
+    float below = INFINITY;
+    if (listing && !lone && listed <= SAMPLE_LIST) {
         if (rank == 0) {
             const int n = static_cast<int>(listed);
             const bool complete = threshold == LOWEST_KEY;
@@ -559,10 +575,18 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
                 const unsigned long long at = border_of(n, true, want, id_bin, kept);
                 if (t == 0) p.ids[row] = static_cast<int64_t>(~static_cast<uint32_t>(at));
             }
+            if (!resolved) {
+                unsigned long long m = 0;
+                for (int i = t; i < n; i += SAMPLE_THREADS) m += whole(sh.weight[i]);
+                m = block_total(m);
+                if (t == 0) sh.listed_mass = static_cast<double>(m) / unit;
+            }
             if (t == 0) sh.outcome = resolved;
         }
         everyone();
         const bool done = block_at(0).outcome != 0;
+        listed_mass = block_at(0).listed_mass;
+        below = key_score(threshold);
         everyone();
         if (done) return;
     }
@@ -731,36 +755,174 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
         }
     };
 
-    bool searched = false;
-    if (top_inf) {
+    // Whether part_mass and part_ties hold what each warp's ids keep (without a filter the stream left it).
+    bool summed = !filtered && !lone;
+    if (lone) {
         unsigned long long c = 0;
         each([&](float, uint32_t k, uint32_t) { c += k == top_key; });
         c = cluster_total(c);
         if (top_k > 0) c = min(c, static_cast<unsigned long long>(top_k));
-        if (nucleus) c = static_cast<unsigned long long>(fmax(1.0, ceil(top_p * static_cast<double>(c))));
+        if (filtered && nucleus) c = static_cast<unsigned long long>(fmax(1.0, ceil(top_p * static_cast<double>(c))));
         cut = top_key;
         ties = c;
-        searched = true;
-    } else if (filtered) {
-        if (top_k > 0) narrow(false, static_cast<unsigned long long>(top_k));
+    } else if (filtered && top_k > 0) {
+        narrow(false, static_cast<unsigned long long>(top_k));
         if (nucleus) {
-            double mass = total * unit;
-            if (top_k > 0) {
-                unsigned long long m = 0;
-                each([&](float v, uint32_t k, uint32_t) { m += k > cut ? whole(score_weight(v, top, inv)) : 0; });
-                m = cluster_total(m);
-                if (cut != 0) m += ties * whole(score_weight(key_score(cut), top, inv));
-                mass = static_cast<double>(m);
-            }
-            const double want = ceil(top_p * mass);
+            unsigned long long m = 0;
+            each([&](float v, uint32_t k, uint32_t) { m += k > cut ? whole(score_weight(v, top, inv)) : 0; });
+            m = cluster_total(m);
+            if (cut != 0) m += ties * whole(score_weight(key_score(cut), top, inv));
+            const double want = ceil(top_p * static_cast<double>(m));
             narrow(true, want > 1.0 ? static_cast<unsigned long long>(want) : 1ull);
         }
-        searched = true;
+    } else if (filtered && nucleus) {
+        // The border lies below the list.  Counts of the scores below it by bins of their distance from the
+        // top, each taken at its bin's middle, place the border to a small part of a bin; the next
+        // reading sums the weights above a window around that place and lists the window, and the
+        // border is found inside.  Should it lie outside, it is narrowed down from the top instead.
+        const double need = top_p * total;
+        const float range = static_cast<float>(fmin(static_cast<double>(top) - static_cast<double>(key_score(sh.probe_low)), 45.0 / inv));
+        const float per = range > 0.0f ? SAMPLE_BINS / range : 0.0f;
+        for (int b = t; b < SAMPLE_BINS; b += SAMPLE_THREADS) {
+            sh.bins[b] = 0;
+            sh.counts[b] = 0;
+        }
+        __syncthreads();
+        for (int g = first_group + t; g < last_group; g += SAMPLE_THREADS) {
+            float v[N];
+            x.load(g, v);
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (v[j] < below && v[j] > -INFINITY)
+                    atomicAdd(&sh.counts[static_cast<int>(fminf((top - v[j]) * per, SAMPLE_BINS - 1))], 1u);
+        }
+        __syncthreads();
+        cluster_bins();
+        for (int b = t; b < SAMPLE_BINS; b += SAMPLE_THREADS)
+            sh.bins[b] = whole(exp(-(b + 0.5) / per * inv)) * sh.counts[b];
+        __syncthreads();
+        const double wanted = (need - listed_mass) * unit;
+        crossing(std::integral_constant<int, SAMPLE_BINS>{}, wanted > 1.0 ? static_cast<unsigned long long>(wanted) : 1ull);
+        const unsigned long long found = sh.found;
+        bool settled = found != ~0ull;
+        if (settled) {
+            const float count = static_cast<float>(sh.counts[found]);
+            const float place = static_cast<float>(found) + static_cast<float>(static_cast<double>(sh.left) / static_cast<double>(sh.bins[found]));
+            const float half = fminf(1.0f, 700.0f / count);
+            const float from = place - half, to = place + half;
+            if (t == 0) sh.listed = 0;
+            __syncthreads();
+            double sum = 0.0;
+            weight_of.refer(top, inv);
+            for (int g0 = warp_first; g0 < warp_last; g0 += 32) {
+                const int g = g0 + lane;
+                float v[N];
+                if (g < warp_last) {
+                    x.load(g, v);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < N; ++j) v[j] = -INFINITY;
+                }
+                bool any = false;
+                const uint32_t id = static_cast<uint32_t>(x.id(g));
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const float y = (top - v[j]) * per;
+                    if (y < from) {
+                        any = true;
+                    } else {
+                        if (y <= to && v[j] > -INFINITY) {
+                            const unsigned int at = atomicAdd(&sh.listed, 1u);
+                            if (at < SAMPLE_LIST) sh.list[at] = (static_cast<unsigned long long>(score_key(v[j])) << 32) | ~(id + j);
+                        }
+                        v[j] = -INFINITY;
+                    }
+                }
+                if (__any_sync(FULL_WARP, any)) {
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        const double w = weight_of(v[j], p.taylor);
+                        if (v[j] > -INFINITY) sum += w;
+                    }
+                }
+            }
+            sum = warp_sum(sum);
+            if (lane == 0) sh.mass[warp] = sum * weight_of.factor;
+            everyone();
+            listed = 0;
+            for (int r = 0; r < blocks; ++r) listed += block_at(r).listed;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int e = 2 * lane + h;
+                part_mass[h] = e < parts ? block_at(e / SAMPLE_WARPS).mass[e % SAMPLE_WARPS] : 0.0;
+            }
+            const double rest = (need - warp_sum(part_mass[0] + part_mass[1])) * unit;
+            settled = listed <= SAMPLE_LIST && rest >= 1.0;
+            if (settled && rank == 0) {
+                const int n = static_cast<int>(listed);
+                gather();
+                for (int i = t; i < n; i += SAMPLE_THREADS)
+                    sh.weight[i] = score_weight(key_score(static_cast<uint32_t>(sh.list[i] >> 32)), top, inv);
+                __syncthreads();
+                const float finer = SAMPLE_BINS / (to - from);
+                auto bin_of = [&](unsigned long long c) {
+                    const float y = (top - key_score(static_cast<uint32_t>(c >> 32))) * per;
+                    return static_cast<int>(fminf(fmaxf(y - from, 0.0f) * finer, SAMPLE_BINS - 1));
+                };
+                const unsigned long long border = border_of(n, false, static_cast<unsigned long long>(ceil(rest)), bin_of,
+                                                            [&](int i) { return whole(sh.weight[i]); });
+                for (int e = t; e < SAMPLE_BINS; e += SAMPLE_THREADS) {
+                    sh.bins[e] = 0;
+                    sh.counts[e] = 0;
+                }
+                if (t == 0) sh.few = 0;
+                __syncthreads();
+                const uint32_t key = static_cast<uint32_t>(border >> 32);
+                for (int i = t; i < n; i += SAMPLE_THREADS) {
+                    const unsigned long long c = sh.list[i];
+                    const uint32_t k = static_cast<uint32_t>(c >> 32);
+                    if (k < key) continue;
+                    // The warp whose ids hold it.
+                    const int g = static_cast<int>((static_cast<int64_t>(~static_cast<uint32_t>(c)) + x.lead) / N);
+                    const int e = g / per_block * SAMPLE_WARPS + g % per_block / per_warp;
+                    if (k > key) atomicAdd(&sh.bins[e], whole(sh.weight[i]));
+                    else atomicAdd(&sh.counts[e], 1u);
+                    if (k == key && c >= border) atomicAdd(&sh.few, 1);
+                }
+                __syncthreads();
+                if (t == 0) {
+                    sh.cut = key;
+                    sh.cut_ties = sh.few;
+                }
+            }
+            everyone();
+            if (settled) {
+                cut = block_at(0).cut;
+                ties = block_at(0).cut_ties;
+                settled = cut != 0;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int e = 2 * lane + h;
+                    if (e < parts) {
+                        part_mass[h] += static_cast<double>(block_at(0).bins[e]) / unit;
+                        part_ties[h] = block_at(0).counts[e];
+                    }
+                }
+                summed = settled && !floor_p;
+            }
+            everyone();
+        }
+        if (!settled) {
+            const double want = ceil(need * unit);
+            narrow(true, want > 1.0 ? static_cast<unsigned long long>(want) : 1ull);
+        }
     }
 
-    // Each warp's kept weight, ties apart (without a filter the stream has left it).
+    // Each warp's kept weight, ties apart.
     const double cut_weight = cut != 0 ? score_weight(key_score(cut), top, inv) : 0.0;
-    if (searched) {
+    weight_of.refer(lone ? 0.0f : top, inv);
+    const double min_weight = min_p / weight_of.factor; // in the units of weight_of
+    if (!summed) {
         double sum = 0.0;
         unsigned int equal = 0;
         for (int g0 = warp_first; g0 < warp_last; g0 += 32) {
@@ -783,12 +945,12 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
             if (__any_sync(FULL_WARP, any)) {
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
-                    const double w = weight_of(v[j], top);
-                    if (w >= min_p || v[j] == top) sum += w;
+                    const double w = weight_of(v[j], p.taylor);
+                    if (v[j] > -INFINITY && (w >= min_weight || v[j] == top)) sum += w;
                 }
             }
         }
-        sum = warp_sum(sum);
+        sum = warp_sum(sum) * weight_of.factor;
         equal = __reduce_add_sync(FULL_WARP, equal);
         if (lane == 0) {
             sh.mass[warp] = sum;
@@ -858,10 +1020,11 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
             const uint32_t k = score_key(v[j]);
             if (cut != 0 && k == cut) ++equal;
             if (k <= cut) v[j] = -INFINITY;
-            const double w = weight_of(v[j], top);
-            if (w >= min_p || v[j] == top) sum += w;
+            const double w = weight_of(v[j], p.taylor);
+            if (v[j] > -INFINITY && (w >= min_weight || v[j] == top)) sum += w;
         }
     }
+    sum *= weight_of.factor;
     // Running sums over the block: of the ties, then of the weights with the ties that are kept.
     const unsigned long long equal_upto = warp_inclusive(equal, lane);
     __syncthreads();

@@ -118,6 +118,44 @@ def test_sample_rows_with_masks(dtype, kw):
     np.testing.assert_array_equal(_host(povs.sample(x, u, **kw)), _sample_wanted(x, u, **kw))
 
 
+@pytest.mark.parametrize("kw", [{"top_p": 0.9}, {"top_p": 0.999}, {"top_p": 0.6, "min_p": 1e-4}, {"top_k": 5000},
+                                {"top_k": 30_000, "top_p": 0.95}, {"min_p": 1e-4}, {"top_p": 0.9, "temperature": 30.0},
+                                {"top_p": 0.95, "temperature": 0.01}, {"top_p": 0.5, "temperature": 1e28}], ids=str)
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("rows", [3, 40])
+def test_sample_wide_nuclei(rows, dtype, kw):
+    """Kept sets of thousands of ids: flat scores, scores tied by the thousand, masked runs, few and many
+    blocks per row."""
+    width = 40_009
+    g = torch.Generator().manual_seed(rows)
+    x = (torch.randn(rows, width, generator=g) * 0.7).to(dtype).to(DEV)
+    x[0] = (x[0] * 2).round() / 2
+    x[1, 1000:30_000] = -float("inf")
+    x[2] = torch.where(torch.arange(width, device=DEV) < 9000, 3.0, x[2])
+    u = _uniforms(rows, seed=11)
+    np.testing.assert_array_equal(_host(povs.sample(x, u, **kw)), _sample_wanted(x, u, **kw))
+
+
+def test_sample_scores_at_the_ends_of_float():
+    """Rows of the lowest and highest floats, and temperatures at and beyond both ends."""
+    low, high = torch.finfo(torch.float32).min, torch.finfo(torch.float32).max
+    width = 3001
+    x = torch.full((8, width), low, device=DEV)
+    x[1, 7::9] = -float("inf")
+    x[2, 3::2] = high
+    x[3] = torch.linspace(-1e-30, 1e-30, width, device=DEV)
+    x[4] = torch.linspace(low / 2, high / 2, width, device=DEV)
+    x[5, :1500] = -float("inf")
+    x[5, 2000] = -3.2e38
+    x[6] = 1.0
+    x[6, 5] = torch.nextafter(torch.tensor(1.0), torch.tensor(2.0))
+    u = _uniforms(8, seed=2)
+    for temperature in (1e-30, 1e-7, 1.0, 1e10, 1e20):
+        for kw in ({}, {"top_p": 0.5}, {"top_k": 50}, {"min_p": 0.3}):
+            kw = dict(kw, temperature=temperature)
+            np.testing.assert_array_equal(_host(povs.sample(x, u, **kw)), _sample_wanted(x, u, **kw), err_msg=str(kw))
+
+
 def test_sample_uniforms_at_and_beyond_their_ends():
     x = _scores(6, 301, torch.float32, seed=1)
     x[:, 280:] = -float("inf")
