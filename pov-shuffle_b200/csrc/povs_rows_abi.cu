@@ -228,8 +228,13 @@ extern "C" int povs_sample_v1(const void* logits, int32_t dtype, int64_t rows, i
     p.top_p = top_p;
     p.min_p = min_p;
     p.ids = ids;
-    double term = 1.0;
-    for (int i = 0; i < 5; ++i) p.taylor[i] = term *= 0.69314718055994530942 / (i + 1);
+    // 2^r = 1 + r (poly[0] + r (poly[1] + ...)): Taylor terms (ln 2)^i / i!, the fifth economised for
+    // |r| <= h: r^5 = 5/4 h^2 r^3 - 5/16 h^4 r, up to h^5 / 16.
+    const double ln2 = 0.69314718055994530942, h2 = 1.0 / (64 * 64), fifth = ln2 * ln2 * ln2 * ln2 * ln2 / 120;
+    p.poly[0] = ln2 - 0.3125 * h2 * h2 * fifth;
+    p.poly[1] = ln2 * ln2 / 2;
+    p.poly[2] = ln2 * ln2 * ln2 / 6 + 1.25 * h2 * fifth;
+    p.poly[3] = ln2 * ln2 * ln2 * ln2 / 24;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     p.cluster = sample_cluster(rows, width, sms);
     cudaError_t e;

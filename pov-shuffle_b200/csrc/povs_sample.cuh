@@ -13,7 +13,7 @@
 
 #include <cfloat>
 #include <cstdint>
-#include <type_traits>
+#include <cstring>
 
 #include "povs_rows.cuh"
 
@@ -40,7 +40,7 @@ struct SampleParams {
     double min_p;
     int64_t top_k;
     int64_t* ids;
-    double taylor[5]; // (ln 2)^i / i!, i = 1 .. 5: in constant memory, where an operand costs no register
+    double poly[4]; // WarpExp's polynomial from r on: in constant memory, where an operand costs no register
 };
 
 constexpr int SAMPLE_THREADS = 256;
@@ -69,12 +69,13 @@ constexpr uint32_t LOWEST_KEY = 0x00800000u; // the lowest finite score's
 constexpr float LONE = -3.0e38f;
 
 // Weights of many scores, for loops that a whole warp runs together: exp((v - reference) * inv) up to
-// a factor common to all, to 2^-48 relative.  With z = v * inv / ln 2 = n / 32 + r, |r| <= 1/64, and n0
+// a factor common to all, to 2^-43 relative.  With z = v * inv / ln 2 = n / 32 + r, |r| <= 1/64, and n0
 // the n of the reference, the weight is 2^((n - n0) >> 5) * 2^(((n - n0) & 31) / 32) * 2^r: the second
 // factor sits in the lanes' registers (one shuffle in place of a table in memory, whose banks would
-// clash), and 2^r is its Taylor polynomial of degree 5 (the next term is (r ln 2)^6 / 720 < 2.3e-15).
+// clash), and 2^r is its Taylor polynomial of degree 5 with the last term economised into the lower
+// ones by the Chebyshev polynomial T5, which leaves (ln 2)^5 / 120 / 64^5 / 16 < 2^-43.
 // The products with inv / ln 2 are exact in both fused operations, so large scores lose nothing.
-// Ten operations in 64 bits a score: at half the rate of 32 bits about what its 4 bytes cost to read.
+// Nine operations in 64 bits a score: at half the rate of 32 bits about what its 4 bytes cost to read.
 // Scores 500 or more below the reference in z, NaN and -infinity weigh 2^-500 to 2^-1000: nothing beside
 // the highest score's.  References stay above LONE, where the float 500 below exists.
 struct WarpExp {
@@ -95,16 +96,15 @@ struct WarpExp {
         factor = exp2(fma(-here, scale, n0 * 0.03125));
         floor = __double2float_rd(here - 500.0 / scale);
     }
-    __device__ __forceinline__ double operator()(float v, const double* __restrict__ taylor) const
+    __device__ __forceinline__ double operator()(float v, const double* __restrict__ poly) const
     {
         const double x = static_cast<double>(fmaxf(v, floor));
         const double t = fma(x, scale, magic);
         const double r = fma(x, scale, magic - t);
         const int n = __double2loint(t);
-        double q = fma(r, taylor[4], taylor[3]);
-        q = fma(r, q, taylor[2]);
-        q = fma(r, q, taylor[1]);
-        q = fma(r, q, taylor[0]);
+        double q = fma(r, poly[3], poly[2]);
+        q = fma(r, q, poly[1]);
+        q = fma(r, q, poly[0]);
         const double at = __shfl_sync(FULL_WARP, step, n & 31);
         const double base = __hiloint2double(__double2hiint(at) + (n & ~31) * (1 << 15), __double2loint(at));
         return fma(base * r, q, base);
@@ -148,17 +148,27 @@ template <typename T> struct RowGroups {
         groups = static_cast<int>((width + lead + N - 1) / N);
     }
     __device__ __forceinline__ int64_t id(int g) const { return static_cast<int64_t>(g) * N - lead; }
+    __device__ __forceinline__ void unpack(const uint4& raw, float (&v)[N]) const
+    {
+        T e[N];
+        memcpy(e, &raw, sizeof(raw));
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = to_float(e[j]);
+    }
+    __device__ __forceinline__ void load_if(bool there, int g, float (&v)[N]) const
+    {
+        if (there) {
+            load(g, v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = -INFINITY;
+        }
+    }
     __device__ __forceinline__ void load(int g, float (&v)[N]) const
     {
         const int64_t i = id(g);
         if (i >= 0 && i + N <= width) {
-            union {
-                uint4 raw;
-                T e[N];
-            } u;
-            u.raw = __ldg(reinterpret_cast<const uint4*>(x + i));
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = to_float(u.e[j]);
+            unpack(__ldg(reinterpret_cast<const uint4*>(x + i)), v);
         } else {
 #pragma unroll
             for (int j = 0; j < N; ++j) v[j] = i + j >= 0 && i + j < width ? to_float(x[i + j]) : -INFINITY;
@@ -172,7 +182,7 @@ struct SampleShared {
     unsigned long long bins[SAMPLE_BINS];
     unsigned int counts[SAMPLE_BINS];
     // Read by the other blocks of the cluster.
-    unsigned long long best[SAMPLE_WARPS]; // highest key << 32 | ~lowest id that has it
+    uint32_t best[SAMPLE_WARPS]; // each warp's highest key
     double mass[SAMPLE_WARPS];             // of each warp's ids, which follow one another
     float reference[SAMPLE_WARPS];
     unsigned int ties[SAMPLE_WARPS];
@@ -194,408 +204,107 @@ struct SampleShared {
     unsigned long long left;
 };
 
-// Grid: rows * cluster blocks, `cluster` neighbours per row.
-template <typename T>
-__global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __grid_constant__ SampleParams p)
-{
-    constexpr int N = RowGroups<T>::N;
-    constexpr int UNROLL = 4;
-    __shared__ SampleShared sh;
-    cg::cluster_group cluster = cg::this_cluster();
-    const int blocks = p.cluster, rank = blockIdx.x % blocks;
-    const int64_t row = blockIdx.x / blocks;
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const RowGroups<T> x(static_cast<const T*>(p.logits) + row * p.row_stride, p.width);
+// One block's share of the work on a row.  All blocks of the row's cluster take the same steps: what
+// decides them is worked out by each from the same numbers.
+template <typename T> struct SampleRow {
+    using Groups = RowGroups<T>;
+    static constexpr int N = Groups::N;
+    using Entry = unsigned long long; // an entry of the list
+    using Whole = unsigned long long; // a weight in units of 2^-weight_bits, or a count
 
-    const double temperature = p.temperatures != nullptr ? p.temperatures[row] : p.temperature;
-    const double top_p = p.top_ps != nullptr ? p.top_ps[row] : p.top_p;
-    const double min_p = p.min_ps != nullptr ? p.min_ps[row] : p.min_p;
-    const int64_t top_k_given = p.top_ks != nullptr ? p.top_ks[row] : p.top_k;
-    const int64_t top_k = top_k_given > 0 && top_k_given < p.width ? top_k_given : 0;
-    const bool greedy = !(temperature > 0.0);
-    const double inv = fmin(fmax(1.0 / temperature, 1e-28), 1e36); // so that 0 * inv stays 0
-    const bool nucleus = top_p < 1.0, floor_p = min_p > 0.0;
-    const bool filtered = !greedy && (nucleus || floor_p || top_k > 0);
-    // The sum of all weights: without a filter, or for a nucleus of the whole row.
-    const bool need_mass = !greedy && top_k == 0 && (nucleus || !floor_p);
-
+    const SampleParams& p;
+    SampleShared& sh;
+    cg::cluster_group cluster;
+    Groups x;
+    WarpExp weight_of;
+    int blocks, rank, t, lane, warp;
     // This block's groups, and within them each warp's, in id order.
-    const int per_block = (x.groups + blocks - 1) / blocks;
-    const int first_group = min(rank * per_block, x.groups), last_group = min(first_group + per_block, x.groups);
-    const int per_warp = (per_block + SAMPLE_WARPS - 1) / SAMPLE_WARPS;
-    const int warp_first = min(first_group + warp * per_warp, last_group), warp_last = min(warp_first + per_warp, last_group);
+    int per_block, per_warp, first_group, last_group, warp_first, warp_last;
+    int parts; // warps of the cluster
+    // The row's settings.
+    int64_t top_k;
+    double top_p, min_p, inv, u;
+    bool nucleus, floor_p, filtered, need_mass;
+    double unit;
+    int id_bits;
+    // The list's threshold (`list_from` +infinity: no list).
+    uint32_t threshold;
+    float list_from;
+    bool listing;
+    // What the stream leaves.
+    float top, warp_top, reference;
+    double warp_mass;
+    uint32_t top_key;
+    // Kept are the keys above `cut` and, in id order, the first `ties` of those equal to it (0: all).
+    uint32_t cut = 0;
+    Whole ties = 0;
+    int parity = 0;
+    // Warps 2 lane and 2 lane + 1 of the cluster, which follow one another in id order.
+    double part_mass[2] = {0.0, 0.0};
+    Whole part_ties[2] = {0, 0};
 
-    auto everyone = [&] {
+    __device__ __forceinline__ SampleRow(const SampleParams& p_, SampleShared& sh_, int64_t row)
+        : p(p_), sh(sh_), cluster(cg::this_cluster()), x(static_cast<const T*>(p_.logits) + row * p_.row_stride, p_.width),
+          weight_of(threadIdx.x & 31)
+    {
+        blocks = p.cluster;
+        rank = blockIdx.x % blocks;
+        t = threadIdx.x;
+        lane = t & 31;
+        warp = t >> 5;
+        per_block = (x.groups + blocks - 1) / blocks;
+        per_warp = (per_block + SAMPLE_WARPS - 1) / SAMPLE_WARPS;
+        first_group = min(rank * per_block, x.groups);
+        last_group = min(first_group + per_block, x.groups);
+        warp_first = min(first_group + warp * per_warp, last_group);
+        warp_last = min(warp_first + per_warp, last_group);
+        parts = blocks * SAMPLE_WARPS;
+        const double temperature = p.temperatures != nullptr ? p.temperatures[row] : p.temperature;
+        top_p = p.top_ps != nullptr ? p.top_ps[row] : p.top_p;
+        min_p = p.min_ps != nullptr ? p.min_ps[row] : p.min_p;
+        top_k = p.top_ks != nullptr ? p.top_ks[row] : p.top_k;
+        inv = fmin(fmax(1.0 / temperature, 1e-28), 1e36); // so that 0 * inv stays 0
+        nucleus = top_p < 1.0;
+        floor_p = min_p > 0.0;
+        if (!(temperature > 0.0)) { // the highest score's lowest id is the draw at top_k = 1, at any temperature
+            inv = 1.0;
+            top_k = 1;
+            nucleus = floor_p = false;
+        }
+        if (!floor_p) min_p = 0.0;
+        if (top_k < 0 || top_k >= p.width) top_k = 0;
+        filtered = nucleus || floor_p || top_k > 0;
+        // The sum of all weights: without a filter, or for a nucleus of the whole row.
+        need_mass = top_k == 0 && (nucleus || !floor_p);
+        u = p.uniform_bytes == 4 ? static_cast<const float*>(p.uniforms)[row] : static_cast<const double*>(p.uniforms)[row];
+        u = u > 0.0 ? u : 0.0;
+        unit = static_cast<double>(1ull << p.weight_bits);
+        id_bits = 0;
+        while (id_bits < 32 && (p.width - 1) >> id_bits) ++id_bits;
+    }
+
+    __device__ __forceinline__ void everyone()
+    {
         if (blocks > 1) cluster.sync();
         else __syncthreads();
-    };
-    auto block_at = [&](int r) -> SampleShared& { return blocks > 1 ? *cluster.map_shared_rank(&sh, r) : sh; };
-
-    if (t == 0) sh.listed = 0;
-    if (t < 16) sh.probe_counts[t] = 0;
-    if (t == 0) sh.probe_low = 0xffffffffu;
-    __syncthreads();
-
-    // The probe: scores spread evenly over the row.  Its rank that corresponds to the ids wanted,
-    // with four standard deviations to spare where top_k must be met, gives the list's threshold (its
-    // upper 16 bits, found bit by bit).  Every block of the row finds the same one.
-    uint32_t threshold = LOWEST_KEY;
-    bool listing = filtered;
-    if (filtered && p.width > SAMPLE_LIST) {
-        constexpr int PER = SAMPLE_PROBE / SAMPLE_THREADS;
-        uint32_t k[PER];
-        uint32_t low = 0xffffffffu;
-#pragma unroll
-        for (int m = 0; m < PER / N; ++m) {
-            float v[N];
-            x.load(static_cast<int>(static_cast<int64_t>(m * SAMPLE_THREADS + t) * x.groups / (SAMPLE_PROBE / N)), v);
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                k[m * N + j] = score_key(v[j]);
-                if (k[m * N + j] != 0) low = min(low, k[m * N + j]);
-            }
-        }
-        low = __reduce_min_sync(FULL_WARP, low);
-        if (lane == 0) atomicMin(&sh.probe_low, low);
-        const double share = static_cast<double>(SAMPLE_PROBE) / static_cast<double>(p.width);
-        const double room = 0.8 * SAMPLE_LIST * share;
-        double want = SAMPLE_TARGET * share;
-        if (top_k > 0) {
-            want = static_cast<double>(top_k) * share;
-            if (want > room) listing = false;
-            want = fmin(want + 4.0 * sqrt(want) + 6.0, room);
-        }
-        const unsigned int rank_wanted = static_cast<unsigned int>(fmax(want, 1.0));
-        uint32_t found = 0;
-        for (int bit = 31; bit >= 16; --bit) {
-            const uint32_t candidate = found | (1u << bit);
-            unsigned int c = 0;
-#pragma unroll
-            for (int m = 0; m < PER; ++m) c += k[m] >= candidate;
-            c = __reduce_add_sync(FULL_WARP, c);
-            if (lane == 0) atomicAdd(&sh.probe_counts[bit - 16], c);
-            __syncthreads();
-            if (sh.probe_counts[bit - 16] >= rank_wanted) found = candidate;
-        }
-        threshold = max(found, LOWEST_KEY);
     }
-    const float list_from = listing ? key_score(threshold) : INFINITY; // +infinity: see `lone` below
+    __device__ __forceinline__ SampleShared& block_at(int r) { return blocks > 1 ? *cluster.map_shared_rank(&sh, r) : sh; }
+    __device__ __forceinline__ Whole whole(double w) const { return static_cast<Whole>(llrint(w * unit)); }
+    __device__ __forceinline__ static float score_of(Entry c) { return key_score(static_cast<uint32_t>(c >> 32)); }
 
-    // The stream.
-    WarpExp weight_of(lane);
+    __device__ __forceinline__ Whole block_total(Whole v)
     {
-        float top = -INFINITY, reference = -INFINITY, limit = -INFINITY;
-        int top_group = 0;
-        double sum = 0.0;
-        for (int g0 = warp_first; g0 < warp_last; g0 += 32 * UNROLL) {
-            float v[UNROLL][N];
-#pragma unroll
-            for (int u = 0; u < UNROLL; ++u) {
-                const int g = g0 + 32 * u + lane;
-                if (g < warp_last) {
-                    x.load(g, v[u]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < N; ++j) v[u][j] = -INFINITY;
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < UNROLL; ++u) {
-                const int g = g0 + 32 * u + lane;
-                float most = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < N; ++j) most = fmaxf(most, v[u][j]);
-                if (most > top) {
-                    top = most;
-                    top_group = g;
-                }
-                if (most >= list_from) {
-                    const uint32_t id = static_cast<uint32_t>(x.id(g));
-#pragma unroll
-                    for (int j = 0; j < N; ++j)
-                        if (v[u][j] >= list_from) {
-                            const unsigned int at = atomicAdd(&sh.listed, 1u);
-                            if (at < SAMPLE_LIST)
-                                sh.list[at] = (static_cast<unsigned long long>(score_key(v[u][j])) << 32) | (~(id + j));
-                        }
-                }
-                if (need_mass) {
-                    // The reference is the first scores' highest, renewed only when a weight would pass e^64.
-                    if (__any_sync(FULL_WARP, most > limit)) {
-                        float higher = most;
-#pragma unroll
-                        for (int o = 16; o > 0; o >>= 1) higher = fmaxf(higher, __shfl_xor_sync(FULL_WARP, higher, o));
-                        const double old_factor = weight_of.factor;
-                        weight_of.refer(higher, inv);
-                        sum = reference > LONE ? sum * old_factor * score_weight(reference, higher, inv) / weight_of.factor : 0.0;
-                        reference = higher;
-                        limit = static_cast<float>(static_cast<double>(reference) + 64.0 / inv);
-                    }
-#pragma unroll
-                    for (int j = 0; j < N; ++j) sum += weight_of(v[u][j], p.taylor);
-                }
-            }
-        }
-        // The warp's highest score and the lowest id that has it.
-        unsigned long long best = 0;
-        if (top > -INFINITY) {
-            float v[N];
-            x.load(top_group, v);
-#pragma unroll
-            for (int j = N - 1; j >= 0; --j)
-                if (v[j] == top)
-                    best = (static_cast<unsigned long long>(score_key(top)) << 32) | ~static_cast<uint32_t>(x.id(top_group) + j);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(FULL_WARP, best, o));
-        sum = warp_sum(sum);
-        if (lane == 0) {
-            sh.best[warp] = best;
-            sh.mass[warp] = reference > LONE ? sum * weight_of.factor : 0.0;
-            sh.reference[warp] = reference;
-        }
-    }
-    everyone();
-
-    // Every warp of every block works out the row's totals for itself: lane l takes the warps 2 l and
-    // 2 l + 1 of the cluster, which follow one another in id order.
-    const int parts = blocks * SAMPLE_WARPS;
-    unsigned long long best = 0;
-    unsigned int listed = 0;
-    for (int e = lane; e < parts; e += 32) best = max(best, block_at(e / SAMPLE_WARPS).best[e % SAMPLE_WARPS]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(FULL_WARP, best, o));
-    const uint32_t top_key = static_cast<uint32_t>(best >> 32);
-    const float top = key_score(top_key);
-    if (top_key == 0 || greedy) {
-        if (rank == 0 && t == 0) p.ids[row] = top_key == 0 ? -1 : static_cast<int64_t>(~static_cast<uint32_t>(best));
-        everyone();
-        return;
-    }
-    const bool lone = top == INFINITY || top < LONE; // no list, no sums
-    double part_mass[2] = {0.0, 0.0};
-    unsigned long long part_ties[2] = {0, 0};
-    double total = 0.0; // sum of all weights, relative to the highest score
-    if (need_mass && !lone) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int e = 2 * lane + h;
-            if (e < parts) {
-                SampleShared& from = block_at(e / SAMPLE_WARPS);
-                const double m = from.mass[e % SAMPLE_WARPS];
-                if (m > 0.0) part_mass[h] = m / score_weight(top, from.reference[e % SAMPLE_WARPS], inv);
-            }
-        }
-        total = warp_sum(part_mass[0] + part_mass[1]);
-    }
-    for (int r = 0; r < blocks; ++r) listed += block_at(r).listed;
-
-    double u = p.uniform_bytes == 4 ? static_cast<const float*>(p.uniforms)[row]
-                                    : static_cast<const double*>(p.uniforms)[row];
-    u = u > 0.0 ? u : 0.0;
-    const double unit = static_cast<double>(1ull << p.weight_bits);
-    auto whole = [&](double w) { return static_cast<unsigned long long>(llrint(w * unit)); };
-    int id_bits = 0;
-    while (id_bits < 32 && (p.width - 1) >> id_bits) ++id_bits;
-
-    auto block_total = [&](unsigned long long v) {
         v = warp_sum(v);
         __syncthreads();
         if (lane == 0) sh.part[warp] = v;
         __syncthreads();
-        unsigned long long s = 0;
+        Whole s = 0;
 #pragma unroll
         for (int w = 0; w < SAMPLE_WARPS; ++w) s += sh.part[w];
         return s;
-    };
-    // The first bin at which the running sum over sh.bins reaches `want`: its number in sh.found (~0:
-    // none) and what is left of `want` in it in sh.left.
-    auto crossing = [&](auto bins, unsigned long long want) {
-        constexpr int PER = decltype(bins)::value / SAMPLE_THREADS;
-        unsigned long long mine = 0;
-#pragma unroll
-        for (int b = 0; b < PER; ++b) mine += sh.bins[t * PER + b];
-        unsigned long long upto = warp_inclusive(mine, lane);
-        if (lane == 31) sh.part[warp] = upto;
-        if (t == 0) sh.found = ~0ull;
-        __syncthreads();
-        for (int w = 0; w < warp; ++w) upto += sh.part[w];
-        if (upto >= want && upto - mine < want) {
-            unsigned long long left = want - (upto - mine);
-            int at = t * PER;
-            while (sh.bins[at] < left) left -= sh.bins[at++];
-            sh.found = at;
-            sh.left = left;
-        }
-        __syncthreads();
-    };
-    // Of the list's first n entries, from the highest down, the one at which the running sum of `amount`
-    // reaches `want`, digit by digit; 0 where the whole sum stays below.  by_id looks at the lower
-    // half (~id) alone: ids in ascending order.
-    auto select = [&](int n, bool by_id, unsigned long long want, auto&& amount) -> unsigned long long {
-        unsigned long long prefix = 0;
-        for (int shift = by_id ? 24 : 56; shift >= 0; shift -= 8) {
-            if (shift < 32 && shift >= id_bits) { // ~id has ones there
-                prefix = (prefix << 8) | 255;
-                continue;
-            }
-            sh.bins[t] = 0;
-            __syncthreads();
-            for (int i = t; i < n; i += SAMPLE_THREADS) {
-                const unsigned long long c = by_id ? sh.list[i] & 0xffffffffull : sh.list[i];
-                if (shift < 56 && (c >> (shift + 8)) != prefix) continue;
-                const unsigned long long a = amount(i);
-                if (a != 0) atomicAdd(&sh.bins[255 - ((c >> shift) & 255)], a);
-            }
-            __syncthreads();
-            crossing(std::integral_constant<int, 256>{}, want);
-            const unsigned long long found = sh.found;
-            want = sh.left;
-            __syncthreads();
-            if (found == ~0ull) return 0;
-            prefix = (prefix << 8) | (255 - found);
-        }
-        return prefix;
-    };
-    // The same by bins of a number that does not rise along the order (bin_of: a bin for an entry): one
-    // round of sums, then the few entries of the bin that holds the border.  Where those are more than
-    // a warp has lanes, digit by digit.
-    auto border_of = [&](int n, bool by_id, unsigned long long want, auto&& bin_of, auto&& amount) -> unsigned long long {
-        for (int b = t; b < SAMPLE_BINS; b += SAMPLE_THREADS) sh.bins[b] = 0;
-        if (t == 0) sh.few = 0;
-        __syncthreads();
-        for (int i = t; i < n; i += SAMPLE_THREADS) {
-            const unsigned long long a = amount(i);
-            if (a != 0) atomicAdd(&sh.bins[bin_of(sh.list[i])], a);
-        }
-        __syncthreads();
-        crossing(std::integral_constant<int, SAMPLE_BINS>{}, want);
-        const unsigned long long found = sh.found, left = sh.left;
-        if (found == ~0ull) {
-            __syncthreads();
-            return 0;
-        }
-        for (int i = t; i < n; i += SAMPLE_THREADS)
-            if (bin_of(sh.list[i]) == static_cast<int>(found) && amount(i) != 0) {
-                const int at = atomicAdd(&sh.few, 1);
-                if (at < 32) sh.few_at[at] = i;
-            }
-        __syncthreads();
-        const int few = sh.few;
-        if (few > 32) return select(n, by_id, left, [&](int i) { return bin_of(sh.list[i]) == static_cast<int>(found) ? amount(i) : 0ull; });
-        if (warp == 0) {
-            const int i = lane < few ? sh.few_at[lane] : 0;
-            const unsigned long long c = by_id ? sh.list[i] & 0xffffffffull : sh.list[i];
-            const unsigned long long a = lane < few ? static_cast<unsigned long long>(amount(i)) : 0;
-            unsigned long long before = 0;
-            for (int o = 0; o < few; ++o) {
-                const unsigned long long other = __shfl_sync(FULL_WARP, c, o), b = __shfl_sync(FULL_WARP, a, o);
-                if (other > c) before += b;
-            }
-            if (lane < few && before < left && before + a >= left) sh.found = c;
-        }
-        __syncthreads();
-        const unsigned long long entry = sh.found;
-        __syncthreads();
-        return entry;
-    };
-    // The other blocks' listed entries, appended to this block's (rank 0).
-    auto gather = [&] {
-        unsigned int at = min(sh.listed, static_cast<unsigned int>(SAMPLE_LIST));
-        for (int r = 1; r < blocks; ++r) {
-            SampleShared& from = block_at(r);
-            const unsigned int c = from.listed;
-            for (unsigned int i = t; i < c && at + i < SAMPLE_LIST; i += SAMPLE_THREADS) sh.list[at + i] = from.list[i];
-            at += c;
-        }
-        __syncthreads();
-    };
-
-    double listed_mass = 0.0; // weight of the scores from `below` up
-    float below = INFINITY;
-    if (listing && !lone && listed <= SAMPLE_LIST) {
-        if (rank == 0) {
-            const int n = static_cast<int>(listed);
-            const bool complete = threshold == LOWEST_KEY;
-            gather();
-            if (t == 0) sh.lowest = 0xffffffffu;
-            __syncthreads();
-            uint32_t lowest = 0xffffffffu;
-            for (int i = t; i < n; i += SAMPLE_THREADS) {
-                const uint32_t k = static_cast<uint32_t>(sh.list[i] >> 32);
-                lowest = min(lowest, k);
-                sh.weight[i] = score_weight(key_score(k), top, inv);
-            }
-            lowest = __reduce_min_sync(FULL_WARP, lowest);
-            if (lane == 0) atomicMin(&sh.lowest, lowest);
-            __syncthreads();
-            const float spread = top - key_score(sh.lowest);
-            const float per_score = spread > 0.0f ? SAMPLE_BINS / spread : 0.0f;
-            const float per_id = static_cast<float>(SAMPLE_BINS) / static_cast<float>(p.width);
-            auto score_bin = [&](unsigned long long c) {
-                return min(SAMPLE_BINS - 1, static_cast<int>((top - key_score(static_cast<uint32_t>(c >> 32))) * per_score));
-            };
-            auto id_bin = [&](unsigned long long c) {
-                return min(SAMPLE_BINS - 1, static_cast<int>(static_cast<float>(~static_cast<uint32_t>(c)) * per_id));
-            };
-            bool resolved = true;
-            unsigned long long cut = 0; // kept are the entries from here up
-            if (top_k > 0) {
-                if (n >= top_k) cut = border_of(n, false, static_cast<unsigned long long>(top_k), score_bin, [](int) { return 1ull; });
-                else resolved = complete;
-            }
-            if (resolved && nucleus) {
-                double mass = total;
-                if (top_k > 0) {
-                    unsigned long long m = 0;
-                    for (int i = t; i < n; i += SAMPLE_THREADS) m += sh.list[i] >= cut ? whole(sh.weight[i]) : 0;
-                    mass = static_cast<double>(block_total(m)) / unit;
-                }
-                const double want = ceil(top_p * mass * unit);
-                const unsigned long long from = cut;
-                const unsigned long long border = border_of(n, false, want > 1.0 ? static_cast<unsigned long long>(want) : 1ull, score_bin,
-                                                            [&](int i) { return sh.list[i] >= from ? whole(sh.weight[i]) : 0ull; });
-                if (border != 0) cut = border;
-                else if (top_k == 0) resolved = complete; // every listed id is in the nucleus, and more may be
-            }
-            // min_p alone ends inside the list where the threshold's own weight is below it.
-            if (floor_p && !resolved && top_k == 0) resolved = score_weight(key_score(threshold), top, inv) < min_p;
-            else if (floor_p && !nucleus && top_k == 0) resolved = complete || score_weight(key_score(threshold), top, inv) < min_p;
-            if (resolved) {
-                auto kept = [&](int i) -> unsigned long long {
-                    const unsigned long long c = sh.list[i];
-                    const double w = sh.weight[i];
-                    return c >= cut && (w >= min_p || static_cast<uint32_t>(c >> 32) == top_key) ? whole(w) : 0;
-                };
-                unsigned long long m = 0;
-                for (int i = t; i < n; i += SAMPLE_THREADS) m += kept(i);
-                m = block_total(m);
-                const double target = u * static_cast<double>(m);
-                const unsigned long long want = target < static_cast<double>(m) ? min(static_cast<unsigned long long>(target) + 1, m) : m;
-                const unsigned long long at = border_of(n, true, want, id_bin, kept);
-                if (t == 0) p.ids[row] = static_cast<int64_t>(~static_cast<uint32_t>(at));
-            }
-            if (!resolved) {
-                unsigned long long m = 0;
-                for (int i = t; i < n; i += SAMPLE_THREADS) m += whole(sh.weight[i]);
-                m = block_total(m);
-                if (t == 0) sh.listed_mass = static_cast<double>(m) / unit;
-            }
-            if (t == 0) sh.outcome = resolved;
-        }
-        everyone();
-        const bool done = block_at(0).outcome != 0;
-        listed_mass = block_at(0).listed_mass;
-        below = key_score(threshold);
-        everyone();
-        if (done) return;
     }
-
-    // From here on all blocks of the row work together, each on its own groups.
-    uint32_t cut = 0;            // kept are the keys above, and, in id order, the first `ties` of those equal to it
-    unsigned long long ties = 0; // (0: every key is kept)
-    int parity = 0;
-    auto cluster_total = [&](unsigned long long v) {
+    __device__ __forceinline__ Whole cluster_total(Whole v)
+    {
         v = block_total(v);
         if (blocks == 1) return v;
         if (t == 0) sh.exchange[parity] = v;
@@ -604,8 +313,320 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
         for (int r = 0; r < blocks; ++r) v += block_at(r).exchange[parity];
         parity ^= 1;
         return v;
-    };
-    auto each = [&](auto&& f) {
+    }
+
+    // --- The probe: scores spread evenly over the row.  Its rank that corresponds to the ids wanted,
+    // with four standard deviations to spare where top_k must be met, gives the list's threshold (its
+    // upper 16 bits, found bit by bit).  Every block of the row finds the same one.
+    __device__ __forceinline__ void probe()
+    {
+        threshold = LOWEST_KEY;
+        listing = filtered;
+        if (filtered && p.width > SAMPLE_LIST) {
+            constexpr int PER = SAMPLE_PROBE / SAMPLE_THREADS;
+            uint32_t k[PER];
+            uint32_t low = 0xffffffffu;
+#pragma unroll
+            for (int m = 0; m < PER / N; ++m) {
+                float v[N];
+                x.load(static_cast<int>(static_cast<int64_t>(m * SAMPLE_THREADS + t) * x.groups / (SAMPLE_PROBE / N)), v);
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    k[m * N + j] = score_key(v[j]);
+                    if (k[m * N + j] != 0) low = min(low, k[m * N + j]);
+                }
+            }
+            low = __reduce_min_sync(FULL_WARP, low);
+            if (lane == 0) atomicMin(&sh.probe_low, low);
+            const double share = static_cast<double>(SAMPLE_PROBE) / static_cast<double>(p.width);
+            const double room = 0.8 * SAMPLE_LIST * share;
+            double want = SAMPLE_TARGET * share;
+            if (top_k > 0) {
+                want = static_cast<double>(top_k) * share;
+                if (want > room) listing = false;
+                want = fmin(want + 4.0 * sqrt(want) + 6.0, room);
+            }
+            const unsigned int rank_wanted = static_cast<unsigned int>(fmax(want, 1.0));
+            uint32_t found = 0;
+            for (int bit = 31; bit >= 16; --bit) {
+                const uint32_t candidate = found | (1u << bit);
+                unsigned int c = 0;
+#pragma unroll
+                for (int m = 0; m < PER; ++m) c += k[m] >= candidate;
+                c = __reduce_add_sync(FULL_WARP, c);
+                if (lane == 0) atomicAdd(&sh.probe_counts[bit - 16], c);
+                __syncthreads();
+                if (sh.probe_counts[bit - 16] >= rank_wanted) found = candidate;
+            }
+            threshold = max(found, LOWEST_KEY);
+        }
+        list_from = listing ? key_score(threshold) : INFINITY;
+    }
+
+    // --- The stream.
+    // One batch: MANY vectors of this lane, vector u being group g + 32 u.
+    template <bool MASS, bool LIST, int MANY>
+    __device__ __forceinline__ void take(const float (&v)[MANY][N], int g, float& limit, double (&sums)[2])
+    {
+        float most = v[0][0];
+#pragma unroll
+        for (int i = 0; i < MANY; ++i)
+#pragma unroll
+            for (int j = 0; j < N; ++j) most = fmaxf(most, v[i][j]);
+        warp_top = fmaxf(warp_top, most);
+        if (LIST && most >= list_from) {
+#pragma unroll
+            for (int i = 0; i < MANY; ++i) {
+                const uint32_t id = static_cast<uint32_t>(x.id(g + 32 * i));
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (v[i][j] >= list_from) {
+                        const unsigned int at = atomicAdd(&sh.listed, 1u);
+                        if (at < SAMPLE_LIST) sh.list[at] = (static_cast<Entry>(score_key(v[i][j])) << 32) | ~(id + j);
+                    }
+            }
+        }
+        if (MASS) {
+            // The reference is the first scores' highest, renewed only when a weight would pass e^64.
+            if (__any_sync(FULL_WARP, most > limit)) {
+                float higher = most > -INFINITY ? most : -INFINITY;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) higher = fmaxf(higher, __shfl_xor_sync(FULL_WARP, higher, o));
+                const double old_factor = weight_of.factor;
+                weight_of.refer(higher, inv);
+                const bool keep = reference > LONE;
+                const double rescale = keep ? old_factor * score_weight(reference, higher, inv) / weight_of.factor : 0.0;
+                sums[0] = keep ? sums[0] * rescale : 0.0;
+                sums[1] = keep ? sums[1] * rescale : 0.0;
+                reference = higher;
+                limit = static_cast<float>(static_cast<double>(reference) + 64.0 / inv);
+            }
+#pragma unroll
+            for (int i = 0; i < MANY; ++i)
+#pragma unroll
+                for (int j = 0; j < N; ++j) sums[j & 1] += weight_of(v[i][j], p.poly);
+        }
+    }
+    // Groups wholly inside the row are read UNROLL vectors a lane at a time; the row's first and last
+    // group, which may reach outside, go by themselves.
+    template <bool MASS, bool LIST> __device__ __forceinline__ void stream()
+    {
+        constexpr int UNROLL = 16 / N;
+        float limit = -INFINITY;
+        double sums[2] = {0.0, 0.0};
+        warp_top = reference = -INFINITY;
+        const int full_first = max(warp_first, x.lead > 0 ? 1 : 0);
+        const int full_last = min(warp_last, static_cast<int>((x.width + x.lead) / N));
+        const uint4* vectors = reinterpret_cast<const uint4*>(x.x - x.lead);
+        int g = full_first + lane;
+        for (; g - lane + 32 * UNROLL <= full_last; g += 32 * UNROLL) {
+            uint4 raw[UNROLL];
+            float v[UNROLL][N];
+#pragma unroll
+            for (int i = 0; i < UNROLL; ++i) raw[i] = __ldg(vectors + g + 32 * i);
+#pragma unroll
+            for (int i = 0; i < UNROLL; ++i) x.unpack(raw[i], v[i]);
+            take<MASS, LIST, UNROLL>(v, g, limit, sums);
+        }
+        for (; g - lane < full_last; g += 32) {
+            float v[1][N];
+            x.load_if(g < full_last, g, v[0]);
+            take<MASS, LIST, 1>(v, g, limit, sums);
+        }
+#pragma unroll 1
+        for (int end = 0; end < 2; ++end) {
+            const int at = end == 0 ? 0 : x.groups - 1;
+            const bool outside = end == 0 ? x.lead > 0 : at >= full_last && (at > 0 || x.lead == 0);
+            if (outside && warp_first <= at && at < warp_last) {
+                float v[1][N];
+                x.load_if(lane == 0, at, v[0]);
+                take<MASS, LIST, 1>(v, at, limit, sums);
+            }
+        }
+        warp_mass = sums[0] + sums[1];
+    }
+
+    // --- Work on a list of n entries in sh.list, their weights in sh.weight.
+    // The first of BINS bins at which the running sum over sh.bins reaches `want`: its number in sh.found
+    // (~0: none) and what is left of `want` in it in sh.left.
+    template <int BINS> __device__ __forceinline__ void crossing(Whole want)
+    {
+        constexpr int PER = BINS / SAMPLE_THREADS;
+        Whole mine = 0;
+#pragma unroll
+        for (int b = 0; b < PER; ++b) mine += sh.bins[t * PER + b];
+        Whole upto = warp_inclusive(mine, lane);
+        if (lane == 31) sh.part[warp] = upto;
+        if (t == 0) sh.found = ~0ull;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) upto += sh.part[w];
+        if (upto >= want && upto - mine < want) {
+            Whole left = want - (upto - mine);
+            int at = t * PER;
+            while (sh.bins[at] < left) left -= sh.bins[at++];
+            sh.found = at;
+            sh.left = left;
+        }
+        __syncthreads();
+    }
+    // From the highest entry down, the one at which the running sum of `amount` reaches `want`, digit by
+    // digit; 0 where the whole sum stays below.  BY_ID looks at the lower half (~id) alone: ids in
+    // ascending order.
+    template <bool BY_ID, typename Amount> __device__ __forceinline__ Entry select(int n, Whole want, Amount amount)
+    {
+        Entry prefix = 0;
+        for (int shift = BY_ID ? 24 : 56; shift >= 0; shift -= 8) {
+            if (shift < 32 && shift >= id_bits) { // ~id has ones there
+                prefix = (prefix << 8) | 255;
+                continue;
+            }
+            sh.bins[t] = 0;
+            __syncthreads();
+            for (int i = t; i < n; i += SAMPLE_THREADS) {
+                const Entry c = BY_ID ? sh.list[i] & 0xffffffffull : sh.list[i];
+                if (shift < 56 && (c >> (shift + 8)) != prefix) continue;
+                const Whole a = amount(i);
+                if (a != 0) atomicAdd(&sh.bins[255 - ((c >> shift) & 255)], a);
+            }
+            __syncthreads();
+            crossing<256>(want);
+            const Whole found = sh.found;
+            want = sh.left;
+            __syncthreads();
+            if (found == ~0ull) return 0;
+            prefix = (prefix << 8) | (255 - found);
+        }
+        return prefix;
+    }
+    // The same by bins of a number that does not fall along the order (bin_of: an entry's bin): one
+    // round of sums, then the few entries of the bin that holds the border.  Where those are more than
+    // a warp has lanes, digit by digit.
+    template <bool BY_ID, typename BinOf, typename Amount>
+    __device__ __forceinline__ Entry border_of(int n, Whole want, BinOf bin_of, Amount amount)
+    {
+        for (int b = t; b < SAMPLE_BINS; b += SAMPLE_THREADS) sh.bins[b] = 0;
+        if (t == 0) sh.few = 0;
+        __syncthreads();
+        for (int i = t; i < n; i += SAMPLE_THREADS) {
+            const Whole a = amount(i);
+            if (a != 0) atomicAdd(&sh.bins[bin_of(sh.list[i])], a);
+        }
+        __syncthreads();
+        crossing<SAMPLE_BINS>(want);
+        const Whole found = sh.found, left = sh.left;
+        if (found == ~0ull) {
+            __syncthreads();
+            return 0;
+        }
+        const int bin = static_cast<int>(found);
+        for (int i = t; i < n; i += SAMPLE_THREADS)
+            if (bin_of(sh.list[i]) == bin && amount(i) != 0) {
+                const int at = atomicAdd(&sh.few, 1);
+                if (at < 32) sh.few_at[at] = i;
+            }
+        __syncthreads();
+        const int few = sh.few;
+        if (few > 32) return select<BY_ID>(n, left, [&](int i) { return bin_of(sh.list[i]) == bin ? amount(i) : Whole{0}; });
+        if (warp == 0) {
+            const int i = lane < few ? sh.few_at[lane] : 0;
+            const Entry c = BY_ID ? sh.list[i] & 0xffffffffull : sh.list[i];
+            const Whole a = lane < few ? amount(i) : Whole{0};
+            Whole before = 0;
+            for (int o = 0; o < few; ++o) {
+                const Entry other = __shfl_sync(FULL_WARP, c, o);
+                const Whole b = __shfl_sync(FULL_WARP, a, o);
+                if (other > c) before += b;
+            }
+            if (lane < few && before < left && before + a >= left) sh.found = c;
+        }
+        __syncthreads();
+        const Entry entry = sh.found;
+        __syncthreads();
+        return entry;
+    }
+    // The other blocks' listed entries, appended to rank 0's, and all their weights.
+    __device__ __forceinline__ void gather(int n)
+    {
+        unsigned int at = min(sh.listed, static_cast<unsigned int>(SAMPLE_LIST));
+        for (int r = 1; r < blocks; ++r) {
+            SampleShared& from = block_at(r);
+            const unsigned int c = from.listed;
+            for (unsigned int i = t; i < c && at + i < SAMPLE_LIST; i += SAMPLE_THREADS) sh.list[at + i] = from.list[i];
+            at += c;
+        }
+        if (t == 0) sh.lowest = 0xffffffffu;
+        __syncthreads();
+        uint32_t lowest = 0xffffffffu;
+        for (int i = t; i < n; i += SAMPLE_THREADS) {
+            const uint32_t k = static_cast<uint32_t>(sh.list[i] >> 32);
+            lowest = min(lowest, k);
+            sh.weight[i] = score_weight(key_score(k), top, inv);
+        }
+        lowest = __reduce_min_sync(FULL_WARP, lowest);
+        if (lane == 0) atomicMin(&sh.lowest, lowest);
+        __syncthreads();
+    }
+    // Rank 0: the filters and the draw on the list, which holds every score from the threshold up; false
+    // where they reach below it.
+    __device__ __forceinline__ bool draw_from_list(int n, double total, int64_t row)
+    {
+        const bool complete = threshold == LOWEST_KEY;
+        gather(n);
+        const float spread = top - key_score(sh.lowest);
+        const float per_score = spread > 0.0f ? SAMPLE_BINS / spread : 0.0f;
+        const float per_id = static_cast<float>(SAMPLE_BINS) / static_cast<float>(p.width);
+        auto score_bin = [&](Entry c) { return static_cast<int>(fminf((top - score_of(c)) * per_score, SAMPLE_BINS - 1)); };
+        auto id_bin = [&](Entry c) {
+            return static_cast<int>(fminf(static_cast<float>(~static_cast<uint32_t>(c)) * per_id, SAMPLE_BINS - 1));
+        };
+        bool resolved = true;
+        Entry border = 0; // kept are the entries from here up
+        if (top_k > 0) {
+            if (n >= top_k) border = border_of<false>(n, static_cast<Whole>(top_k), score_bin, [](int) { return Whole{1}; });
+            else resolved = complete;
+        }
+        if (resolved && nucleus) {
+            double mass = total * unit;
+            if (top_k > 0) {
+                Whole m = 0;
+                for (int i = t; i < n; i += SAMPLE_THREADS) m += sh.list[i] >= border ? whole(sh.weight[i]) : Whole{0};
+                mass = static_cast<double>(block_total(m));
+            }
+            const double want = ceil(top_p * mass);
+            const Entry from = border;
+            const Entry at = border_of<false>(n, want > 1.0 ? static_cast<Whole>(want) : Whole{1}, score_bin,
+                                              [&](int i) { return sh.list[i] >= from ? whole(sh.weight[i]) : Whole{0}; });
+            if (at != 0) border = at;
+            else if (top_k == 0) resolved = complete; // every listed id is in the nucleus, and more may be
+        }
+        // min_p ends inside the list where the threshold's own weight is below it.
+        if (floor_p && top_k == 0 && (!resolved || !nucleus))
+            resolved = complete || score_weight(key_score(threshold), top, inv) < min_p;
+        if (!resolved) {
+            Whole m = 0;
+            for (int i = t; i < n; i += SAMPLE_THREADS) m += whole(sh.weight[i]);
+            m = block_total(m);
+            if (t == 0) sh.listed_mass = static_cast<double>(m) / unit;
+            return false;
+        }
+        const Entry from = border;
+        auto kept = [&](int i) {
+            const double w = sh.weight[i];
+            return sh.list[i] >= from && (w >= min_p || static_cast<uint32_t>(sh.list[i] >> 32) == top_key) ? whole(w) : Whole{0};
+        };
+        Whole m = 0;
+        for (int i = t; i < n; i += SAMPLE_THREADS) m += kept(i);
+        m = block_total(m);
+        const double target = u * static_cast<double>(m);
+        const Whole want = target < static_cast<double>(m) ? min(static_cast<Whole>(target) + 1, m) : m;
+        const Entry at = border_of<true>(n, want, id_bin, kept);
+        if (t == 0) p.ids[row] = static_cast<int64_t>(~static_cast<uint32_t>(at));
+        return true;
+    }
+
+    // --- Rows that are read again, all blocks together, each on its own groups.
+    template <typename F> __device__ __forceinline__ void each(F f)
+    {
         for (int g = first_group + t; g < last_group; g += SAMPLE_THREADS) {
             float v[N];
             x.load(g, v);
@@ -615,13 +636,23 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
                 if (k != 0) f(v[j], k, static_cast<uint32_t>(x.id(g) + j));
             }
         }
-    };
-    // Sum over the cluster's bins and counts, in every block.
-    auto cluster_bins = [&] {
+    }
+    __device__ __forceinline__ void clear_bins()
+    {
+        for (int b = t; b < SAMPLE_BINS; b += SAMPLE_THREADS) {
+            sh.bins[b] = 0;
+            sh.counts[b] = 0;
+        }
+        __syncthreads();
+    }
+    // Sums of the cluster's bins and counts, in every block.
+    __device__ __forceinline__ void cluster_bins()
+    {
+        __syncthreads();
         if (blocks == 1) return;
         cluster.sync();
         constexpr int PER = SAMPLE_BINS / SAMPLE_THREADS;
-        unsigned long long b[PER];
+        Whole b[PER];
         unsigned int c[PER];
 #pragma unroll
         for (int m = 0; m < PER; ++m) {
@@ -640,70 +671,67 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
             sh.counts[m * SAMPLE_THREADS + t] = c[m];
         }
         __syncthreads();
-    };
+    }
+    __device__ __forceinline__ unsigned int cluster_listed()
+    {
+        unsigned int n = 0;
+        for (int r = 0; r < blocks; ++r) n += block_at(r).listed;
+        return n;
+    }
     // Narrows `cut` and `ties` to the ids before which the running sum, from the highest score down, is
-    // below `want` (counts, or weights with by_mass).
-    auto narrow = [&](bool by_mass, unsigned long long want) {
+    // below `want` (counts, or weights with BY_MASS), by bins of the distance from the highest score.
+    // A round parts the lowest from the highest score of its range, and cuts the range of evenly spread
+    // scores 1024-fold; float's exponents end it within 40 rounds.
+    template <bool BY_MASS> __device__ __forceinline__ void narrow(Whole want)
+    {
         float hi = top, lo = -FLT_MAX;
-        unsigned long long left = want;
+        Whole left = want;
         double range = static_cast<double>(top) - static_cast<double>(key_score(sh.probe_low));
-        if (by_mass) range = fmin(range, 45.0 / inv); // weights further down are below 2^-64
-        // A round parts the lowest from the highest score of its range, and cuts the range of evenly
-        // spread scores 1024-fold; float's exponents end it within 40 rounds.
+        if (BY_MASS) range = fmin(range, 45.0 / inv); // weights further down are below 2^-64
         for (int round = 0; round < 64; ++round) {
             const double scale = range > 0.0 ? SAMPLE_BINS / range : 0.0;
             auto bin_of = [&](float v) {
                 const double b = (static_cast<double>(hi) - static_cast<double>(v)) * scale;
                 return b < SAMPLE_BINS - 1 ? static_cast<int>(b) : SAMPLE_BINS - 1;
             };
-            for (int b = t; b < SAMPLE_BINS; b += SAMPLE_THREADS) {
-                sh.bins[b] = 0;
-                sh.counts[b] = 0;
-            }
-            __syncthreads();
+            clear_bins();
             each([&](float v, uint32_t k, uint32_t) {
                 if (k <= cut || v > hi || v < lo) return;
                 const int b = bin_of(v);
-                const unsigned long long a = by_mass ? whole(score_weight(v, top, inv)) : 1ull;
+                const Whole a = BY_MASS ? whole(score_weight(v, top, inv)) : Whole{1};
                 if (a != 0) atomicAdd(&sh.bins[b], a);
                 atomicAdd(&sh.counts[b], 1u);
             });
-            __syncthreads();
             cluster_bins();
-            crossing(std::integral_constant<int, SAMPLE_BINS>{}, left);
-            const unsigned long long found = sh.found;
+            crossing<SAMPLE_BINS>(left);
+            const Whole found = sh.found;
             if (found == ~0ull) { // first round only: the ids above the cut do not reach `want`
-                unsigned long long sum = 0;
+                Whole sum = 0;
                 for (int b = t; b < SAMPLE_BINS; b += SAMPLE_THREADS) sum += sh.bins[b];
                 sum = block_total(sum);
-                if (cut != 0 && by_mass) {
-                    const unsigned long long w = whole(score_weight(key_score(cut), top, inv));
+                if (cut != 0 && BY_MASS) {
+                    const Whole w = whole(score_weight(key_score(cut), top, inv));
                     if (w != 0) ties = min(ties, (left - sum + w - 1) / w);
                 }
                 return;
             }
-            const int b = static_cast<int>(found);
+            const int bin = static_cast<int>(found);
             left = sh.left;
-            const unsigned int in_bin = sh.counts[b];
+            const unsigned int in_bin = sh.counts[bin];
+            if (t == 0) sh.listed = 0;
             __syncthreads();
             if (in_bin <= SAMPLE_LIST) {
-                if (t == 0) sh.listed = 0;
-                __syncthreads();
                 each([&](float v, uint32_t k, uint32_t id) {
-                    if (k <= cut || v > hi || v < lo || bin_of(v) != b) return;
+                    if (k <= cut || v > hi || v < lo || bin_of(v) != bin) return;
                     const unsigned int at = atomicAdd(&sh.listed, 1u);
-                    if (at < SAMPLE_LIST) sh.list[at] = (static_cast<unsigned long long>(k) << 32) | ~id;
+                    if (at < SAMPLE_LIST) sh.list[at] = (static_cast<Entry>(k) << 32) | ~id;
                 });
                 everyone();
                 if (rank == 0) {
                     const int n = static_cast<int>(in_bin);
-                    gather();
-                    for (int i = t; i < n; i += SAMPLE_THREADS)
-                        sh.weight[i] = score_weight(key_score(static_cast<uint32_t>(sh.list[i] >> 32)), top, inv);
-                    __syncthreads();
-                    const unsigned long long border =
-                        select(n, false, left, [&](int i) { return by_mass ? whole(sh.weight[i]) : 1ull; });
-                    unsigned long long equal = 0;
+                    gather(n);
+                    const Entry border = select<false>(n, left, [&](int i) { return BY_MASS ? whole(sh.weight[i]) : Whole{1}; });
+                    Whole equal = 0;
                     for (int i = t; i < n; i += SAMPLE_THREADS) equal += sh.list[i] >= border && (sh.list[i] >> 32) == (border >> 32);
                     equal = block_total(equal);
                     if (t == 0) {
@@ -720,23 +748,23 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
             // Too many for the list: the bin's own lowest and highest score bound the next round.
             uint32_t low = 0xffffffffu, high = 0;
             each([&](float v, uint32_t k, uint32_t) {
-                if (k <= cut || v > hi || v < lo || bin_of(v) != b) return;
+                if (k <= cut || v > hi || v < lo || bin_of(v) != bin) return;
                 low = min(low, k);
                 high = max(high, k);
             });
             low = __reduce_min_sync(FULL_WARP, low);
             high = __reduce_max_sync(FULL_WARP, high);
-            if (lane == 0) sh.part[warp] = (static_cast<unsigned long long>(~low) << 32) | high;
+            if (lane == 0) sh.part[warp] = (static_cast<Whole>(~low) << 32) | high;
             __syncthreads();
             for (int w = 0; w < SAMPLE_WARPS; ++w) {
                 low = min(low, ~static_cast<uint32_t>(sh.part[w] >> 32));
                 high = max(high, static_cast<uint32_t>(sh.part[w]));
             }
             if (blocks > 1) {
-                if (t == 0) sh.exchange[parity] = (static_cast<unsigned long long>(~low) << 32) | high;
+                if (t == 0) sh.exchange[parity] = (static_cast<Whole>(~low) << 32) | high;
                 cluster.sync();
                 for (int r = 0; r < blocks; ++r) {
-                    const unsigned long long e = block_at(r).exchange[parity];
+                    const Whole e = block_at(r).exchange[parity];
                     low = min(low, ~static_cast<uint32_t>(e >> 32));
                     high = max(high, static_cast<uint32_t>(e));
                 }
@@ -744,7 +772,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
             }
             __syncthreads();
             if (low == high) { // one score, many ids
-                const unsigned long long w = by_mass ? whole(score_weight(key_score(low), top, inv)) : 1ull;
+                const Whole w = BY_MASS ? whole(score_weight(key_score(low), top, inv)) : Whole{1};
                 cut = low;
                 ties = (left + w - 1) / w;
                 return;
@@ -753,41 +781,16 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
             lo = key_score(low);
             range = static_cast<double>(hi) - static_cast<double>(lo);
         }
-    };
-
-    // Whether part_mass and part_ties hold what each warp's ids keep (without a filter the stream left it).
-    bool summed = !filtered && !lone;
-    if (lone) {
-        unsigned long long c = 0;
-        each([&](float, uint32_t k, uint32_t) { c += k == top_key; });
-        c = cluster_total(c);
-        if (top_k > 0) c = min(c, static_cast<unsigned long long>(top_k));
-        if (filtered && nucleus) c = static_cast<unsigned long long>(fmax(1.0, ceil(top_p * static_cast<double>(c))));
-        cut = top_key;
-        ties = c;
-    } else if (filtered && top_k > 0) {
-        narrow(false, static_cast<unsigned long long>(top_k));
-        if (nucleus) {
-            unsigned long long m = 0;
-            each([&](float v, uint32_t k, uint32_t) { m += k > cut ? whole(score_weight(v, top, inv)) : 0; });
-            m = cluster_total(m);
-            if (cut != 0) m += ties * whole(score_weight(key_score(cut), top, inv));
-            const double want = ceil(top_p * static_cast<double>(m));
-            narrow(true, want > 1.0 ? static_cast<unsigned long long>(want) : 1ull);
-        }
-    } else if (filtered && nucleus) {
-        // The border lies below the list.  Counts of the scores below it by bins of their distance from the
-        // top, each taken at its bin's middle, place the border to a small part of a bin; the next
-        // reading sums the weights above a window around that place and lists the window, and the
-        // border is found inside.  Should it lie outside, it is narrowed down from the top instead.
-        const double need = top_p * total;
+    }
+    // A nucleus whose border lies below the list (scores from `below` up weigh listed_mass).  Counts of
+    // the scores below it by bins of their distance from the top, each taken at its bin's middle, place
+    // the border to a small part of a bin; the next reading sums the weights above a window around
+    // that place and lists the window, and the border is found inside, with each warp's kept weight.  False where it lies outside.
+    __device__ __forceinline__ bool border_in_window(double need, double listed_mass, float below)
+    {
         const float range = static_cast<float>(fmin(static_cast<double>(top) - static_cast<double>(key_score(sh.probe_low)), 45.0 / inv));
         const float per = range > 0.0f ? SAMPLE_BINS / range : 0.0f;
-        for (int b = t; b < SAMPLE_BINS; b += SAMPLE_THREADS) {
-            sh.bins[b] = 0;
-            sh.counts[b] = 0;
-        }
-        __syncthreads();
+        clear_bins();
         for (int g = first_group + t; g < last_group; g += SAMPLE_THREADS) {
             float v[N];
             x.load(g, v);
@@ -796,171 +799,153 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
                 if (v[j] < below && v[j] > -INFINITY)
                     atomicAdd(&sh.counts[static_cast<int>(fminf((top - v[j]) * per, SAMPLE_BINS - 1))], 1u);
         }
-        __syncthreads();
         cluster_bins();
-        for (int b = t; b < SAMPLE_BINS; b += SAMPLE_THREADS)
-            sh.bins[b] = whole(exp(-(b + 0.5) / per * inv)) * sh.counts[b];
+        for (int b = t; b < SAMPLE_BINS; b += SAMPLE_THREADS) sh.bins[b] = whole(exp(-(b + 0.5) / per * inv)) * sh.counts[b];
         __syncthreads();
         const double wanted = (need - listed_mass) * unit;
-        crossing(std::integral_constant<int, SAMPLE_BINS>{}, wanted > 1.0 ? static_cast<unsigned long long>(wanted) : 1ull);
-        const unsigned long long found = sh.found;
-        bool settled = found != ~0ull;
-        if (settled) {
-            const float count = static_cast<float>(sh.counts[found]);
-            const float place = static_cast<float>(found) + static_cast<float>(static_cast<double>(sh.left) / static_cast<double>(sh.bins[found]));
-            const float half = fminf(1.0f, 700.0f / count);
-            const float from = place - half, to = place + half;
-            if (t == 0) sh.listed = 0;
+        crossing<SAMPLE_BINS>(wanted > 1.0 ? static_cast<Whole>(wanted) : Whole{1});
+        const Whole found = sh.found;
+        if (found == ~0ull) {
             __syncthreads();
-            double sum = 0.0;
-            weight_of.refer(top, inv);
-            for (int g0 = warp_first; g0 < warp_last; g0 += 32) {
-                const int g = g0 + lane;
-                float v[N];
-                if (g < warp_last) {
-                    x.load(g, v);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < N; ++j) v[j] = -INFINITY;
-                }
-                bool any = false;
-                const uint32_t id = static_cast<uint32_t>(x.id(g));
-#pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const float y = (top - v[j]) * per;
-                    if (y < from) {
-                        any = true;
-                    } else {
-                        if (y <= to && v[j] > -INFINITY) {
-                            const unsigned int at = atomicAdd(&sh.listed, 1u);
-                            if (at < SAMPLE_LIST) sh.list[at] = (static_cast<unsigned long long>(score_key(v[j])) << 32) | ~(id + j);
-                        }
-                        v[j] = -INFINITY;
-                    }
-                }
-                if (__any_sync(FULL_WARP, any)) {
-#pragma unroll
-                    for (int j = 0; j < N; ++j) {
-                        const double w = weight_of(v[j], p.taylor);
-                        if (v[j] > -INFINITY) sum += w;
-                    }
-                }
-            }
-            sum = warp_sum(sum);
-            if (lane == 0) sh.mass[warp] = sum * weight_of.factor;
-            everyone();
-            listed = 0;
-            for (int r = 0; r < blocks; ++r) listed += block_at(r).listed;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int e = 2 * lane + h;
-                part_mass[h] = e < parts ? block_at(e / SAMPLE_WARPS).mass[e % SAMPLE_WARPS] : 0.0;
-            }
-            const double rest = (need - warp_sum(part_mass[0] + part_mass[1])) * unit;
-            settled = listed <= SAMPLE_LIST && rest >= 1.0;
-            if (settled && rank == 0) {
-                const int n = static_cast<int>(listed);
-                gather();
-                for (int i = t; i < n; i += SAMPLE_THREADS)
-                    sh.weight[i] = score_weight(key_score(static_cast<uint32_t>(sh.list[i] >> 32)), top, inv);
-                __syncthreads();
-                const float finer = SAMPLE_BINS / (to - from);
-                auto bin_of = [&](unsigned long long c) {
-                    const float y = (top - key_score(static_cast<uint32_t>(c >> 32))) * per;
-                    return static_cast<int>(fminf(fmaxf(y - from, 0.0f) * finer, SAMPLE_BINS - 1));
-                };
-                const unsigned long long border = border_of(n, false, static_cast<unsigned long long>(ceil(rest)), bin_of,
-                                                            [&](int i) { return whole(sh.weight[i]); });
-                for (int e = t; e < SAMPLE_BINS; e += SAMPLE_THREADS) {
-                    sh.bins[e] = 0;
-                    sh.counts[e] = 0;
-                }
-                if (t == 0) sh.few = 0;
-                __syncthreads();
-                const uint32_t key = static_cast<uint32_t>(border >> 32);
-                for (int i = t; i < n; i += SAMPLE_THREADS) {
-                    const unsigned long long c = sh.list[i];
-                    const uint32_t k = static_cast<uint32_t>(c >> 32);
-                    if (k < key) continue;
-                    // The warp whose ids hold it.
-                    const int g = static_cast<int>((static_cast<int64_t>(~static_cast<uint32_t>(c)) + x.lead) / N);
-                    const int e = g / per_block * SAMPLE_WARPS + g % per_block / per_warp;
-                    if (k > key) atomicAdd(&sh.bins[e], whole(sh.weight[i]));
-                    else atomicAdd(&sh.counts[e], 1u);
-                    if (k == key && c >= border) atomicAdd(&sh.few, 1);
-                }
-                __syncthreads();
-                if (t == 0) {
-                    sh.cut = key;
-                    sh.cut_ties = sh.few;
-                }
-            }
-            everyone();
-            if (settled) {
-                cut = block_at(0).cut;
-                ties = block_at(0).cut_ties;
-                settled = cut != 0;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int e = 2 * lane + h;
-                    if (e < parts) {
-                        part_mass[h] += static_cast<double>(block_at(0).bins[e]) / unit;
-                        part_ties[h] = block_at(0).counts[e];
-                    }
-                }
-                summed = settled && !floor_p;
-            }
-            everyone();
+            return false;
         }
-        if (!settled) {
-            const double want = ceil(need * unit);
-            narrow(true, want > 1.0 ? static_cast<unsigned long long>(want) : 1ull);
-        }
-    }
-
-    // Each warp's kept weight, ties apart.
-    const double cut_weight = cut != 0 ? score_weight(key_score(cut), top, inv) : 0.0;
-    weight_of.refer(lone ? 0.0f : top, inv);
-    const double min_weight = min_p / weight_of.factor; // in the units of weight_of
-    if (!summed) {
+        const float place = static_cast<float>(found) + static_cast<float>(static_cast<double>(sh.left) / static_cast<double>(sh.bins[found]));
+        const float half = fminf(1.0f, 700.0f / static_cast<float>(sh.counts[found]));
+        const float from = place - half, to = place + half;
+        if (t == 0) sh.listed = 0;
+        __syncthreads();
         double sum = 0.0;
-        unsigned int equal = 0;
         for (int g0 = warp_first; g0 < warp_last; g0 += 32) {
             const int g = g0 + lane;
             float v[N];
-            if (g < warp_last) {
-                x.load(g, v);
-            } else {
-#pragma unroll
-                for (int j = 0; j < N; ++j) v[j] = -INFINITY;
-            }
+            x.load_if(g < warp_last, g, v);
             bool any = false;
+            const uint32_t id = static_cast<uint32_t>(x.id(g));
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const uint32_t k = score_key(v[j]);
-                if (cut != 0 && k == cut) ++equal;
-                if (k <= cut) v[j] = -INFINITY;
-                any |= k > cut;
+                const float y = (top - v[j]) * per;
+                if (y < from) {
+                    any = true;
+                } else {
+                    if (y <= to && v[j] > -INFINITY) {
+                        const unsigned int at = atomicAdd(&sh.listed, 1u);
+                        if (at < SAMPLE_LIST) sh.list[at] = (static_cast<Entry>(score_key(v[j])) << 32) | ~(id + j);
+                    }
+                    v[j] = -INFINITY;
+                }
             }
             if (__any_sync(FULL_WARP, any)) {
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
-                    const double w = weight_of(v[j], p.taylor);
-                    if (v[j] > -INFINITY && (w >= min_weight || v[j] == top)) sum += w;
+                    const double w = weight_of(v[j], p.poly);
+                    if (v[j] > -INFINITY) sum += w;
                 }
             }
         }
+        sum = warp_sum(sum);
+        if (lane == 0) sh.mass[warp] = sum * weight_of.factor;
+        everyone();
+        const unsigned int listed = cluster_listed();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int e = 2 * lane + h;
+            part_mass[h] = e < parts ? block_at(e / SAMPLE_WARPS).mass[e % SAMPLE_WARPS] : 0.0;
+        }
+        const double rest = (need - warp_sum(part_mass[0] + part_mass[1])) * unit;
+        const bool inside = listed <= SAMPLE_LIST && rest >= 1.0;
+        if (inside && rank == 0) {
+            const int n = static_cast<int>(listed);
+            gather(n);
+            const float finer = SAMPLE_BINS / (to - from);
+            auto bin_of = [&](Entry c) {
+                const float y = (top - score_of(c)) * per;
+                return static_cast<int>(fminf(fmaxf(y - from, 0.0f) * finer, SAMPLE_BINS - 1));
+            };
+            const Entry border = border_of<false>(n, static_cast<Whole>(ceil(rest)), bin_of, [&](int i) { return whole(sh.weight[i]); });
+            clear_bins();
+            if (t == 0) sh.few = 0;
+            __syncthreads();
+            const uint32_t key = static_cast<uint32_t>(border >> 32);
+            for (int i = t; i < n; i += SAMPLE_THREADS) {
+                const Entry c = sh.list[i];
+                const uint32_t k = static_cast<uint32_t>(c >> 32);
+                if (k < key) continue;
+                // The warp whose ids hold it.
+                const int g = static_cast<int>((static_cast<int64_t>(~static_cast<uint32_t>(c)) + x.lead) / N);
+                const int e = g / per_block * SAMPLE_WARPS + g % per_block / per_warp;
+                if (k > key) atomicAdd(&sh.bins[e], whole(sh.weight[i]));
+                else atomicAdd(&sh.counts[e], 1u);
+                if (c >= border && k == key) atomicAdd(&sh.few, 1);
+            }
+            __syncthreads();
+            if (t == 0) {
+                sh.cut = key;
+                sh.cut_ties = sh.few;
+            }
+        }
+        everyone();
+        if (inside) {
+            cut = block_at(0).cut;
+            ties = block_at(0).cut_ties;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int e = 2 * lane + h;
+                if (e < parts) {
+                    part_mass[h] += static_cast<double>(block_at(0).bins[e]) / unit;
+                    part_ties[h] = block_at(0).counts[e];
+                }
+            }
+        }
+        everyone();
+        return inside && cut != 0;
+    }
+
+    // --- The draw in id order, with `cut` and `ties` settled.
+    // Weight of `have` ids equal to the cut, `before` of them before.
+    __device__ __forceinline__ double tied(Whole before, Whole have, double cut_weight) const
+    {
+        return before >= ties ? 0.0 : static_cast<double>(min(have, ties - before)) * cut_weight;
+    }
+    // Adds a group's kept weights, ties apart, in units of weight_of.  The whole warp takes part.
+    __device__ __forceinline__ void add_kept(float (&v)[N], double min_weight, double& sum, Whole& equal)
+    {
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint32_t k = score_key(v[j]);
+            equal += cut != 0 && k == cut;
+            if (k <= cut) v[j] = -INFINITY;
+            any |= k > cut;
+        }
+        if (__any_sync(FULL_WARP, any)) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const double w = weight_of(v[j], p.poly);
+                if (v[j] > -INFINITY && (w >= min_weight || v[j] == top)) sum += w;
+            }
+        }
+    }
+    __device__ __forceinline__ void sum_parts(double min_weight)
+    {
+        double sum = 0.0;
+        Whole equal = 0;
+        for (int g0 = warp_first; g0 < warp_last; g0 += 32) {
+            float v[N];
+            x.load_if(g0 + lane < warp_last, g0 + lane, v);
+            add_kept(v, min_weight, sum, equal);
+        }
         sum = warp_sum(sum) * weight_of.factor;
-        equal = __reduce_add_sync(FULL_WARP, equal);
+        equal = warp_sum(equal);
         if (lane == 0) {
             sh.mass[warp] = sum;
-            sh.ties[warp] = equal;
+            sh.ties[warp] = static_cast<unsigned int>(equal);
         }
         everyone();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int e = 2 * lane + h;
             part_mass[h] = 0.0;
+            part_ties[h] = 0;
             if (e < parts) {
                 SampleShared& from = block_at(e / SAMPLE_WARPS);
                 part_mass[h] = from.mass[e % SAMPLE_WARPS];
@@ -968,106 +953,186 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __
             }
         }
     }
-    everyone(); // the last look at the other blocks
+    __device__ __forceinline__ void draw(int64_t row, double min_weight)
+    {
+        const double w_cut = cut != 0 ? score_weight(key_score(cut), top, inv) : 0.0;
+        const double cut_weight = cut == top_key || w_cut >= min_p ? w_cut : 0.0;
+        const Whole two_ties = part_ties[0] + part_ties[1];
+        const Whole ties_before = warp_inclusive(two_ties, lane) - two_ties;
+        part_mass[0] += tied(ties_before, part_ties[0], cut_weight);
+        part_mass[1] += tied(ties_before + part_ties[0], part_ties[1], cut_weight);
+        const double two = part_mass[0] + part_mass[1];
+        const double upto = warp_inclusive(two, lane);
+        const double target = u * __shfl_sync(FULL_WARP, upto, 31);
+        // The pair that holds the target; where rounding leaves none, the last one with a weight.
+        const unsigned above = __ballot_sync(FULL_WARP, upto > target && two > 0.0), some = __ballot_sync(FULL_WARP, two > 0.0);
+        const int pair = above != 0 ? __ffs(above) - 1 : 31 - __clz(some);
+        const double before_pair = __shfl_sync(FULL_WARP, upto - two, pair);
+        const double even = __shfl_sync(FULL_WARP, part_mass[0], pair), odd = __shfl_sync(FULL_WARP, part_mass[1], pair);
+        const Whole pair_ties = __shfl_sync(FULL_WARP, ties_before, pair), even_ties = __shfl_sync(FULL_WARP, part_ties[0], pair);
+        const bool second = !(even > 0.0 && before_pair + even > target) && odd > 0.0;
+        const int part = 2 * pair + second;
+        if (some == 0 || part / SAMPLE_WARPS != rank) return;
 
-    const bool ties_drawn = cut != 0 && (cut_weight >= min_p || cut == top_key);
-    auto clipped = [&](unsigned long long before, unsigned long long have) -> double {
-        if (!ties_drawn || before >= ties) return 0.0;
-        return static_cast<double>(min(have, ties - before)) * cut_weight;
-    };
-    const unsigned long long two_ties = part_ties[0] + part_ties[1];
-    const unsigned long long ties_before = warp_inclusive(two_ties, lane) - two_ties;
-    part_mass[0] += clipped(ties_before, part_ties[0]);
-    part_mass[1] += clipped(ties_before + part_ties[0], part_ties[1]);
-    const double upto = warp_inclusive(part_mass[0] + part_mass[1], lane);
-    const double all = __shfl_sync(FULL_WARP, upto, 31);
-    const double target = u * all;
-    // The part that holds the target; where rounding leaves none, the last one with a weight.
-    auto first_above = [&](double sum_upto, double own) {
-        unsigned hit = __ballot_sync(FULL_WARP, sum_upto > target && own > 0.0);
-        if (hit != 0) return __ffs(hit) - 1;
-        hit = __ballot_sync(FULL_WARP, own > 0.0);
-        return 31 - __clz(hit);
-    };
-    const int pair = first_above(upto, part_mass[0] + part_mass[1]);
-    const double pair_before = __shfl_sync(FULL_WARP, upto - part_mass[0] - part_mass[1], pair);
-    const double even = __shfl_sync(FULL_WARP, part_mass[0], pair), odd = __shfl_sync(FULL_WARP, part_mass[1], pair);
-    const unsigned long long pair_ties = __shfl_sync(FULL_WARP, ties_before, pair);
-    const unsigned long long even_ties = __shfl_sync(FULL_WARP, part_ties[0], pair);
-    const bool second = !(even > 0.0 && pair_before + even > target) && odd > 0.0;
-    const int part = 2 * pair + second;
-    if (part / SAMPLE_WARPS != rank) return;
+        // This block holds it: its threads share the part's groups, each a run of them in id order.
+        const double rest = target - (before_pair + (second ? even : 0.0));
+        const int part_first = min(first_group + (part % SAMPLE_WARPS) * per_warp, last_group);
+        const int part_last = min(part_first + per_warp, last_group);
+        const int per_thread = (part_last - part_first + SAMPLE_THREADS - 1) / SAMPLE_THREADS;
+        const int mine_first = min(part_first + t * per_thread, part_last), mine_last = min(mine_first + per_thread, part_last);
+        double sum = 0.0;
+        Whole equal = 0;
+        for (int i = 0; i < per_thread; ++i) { // the same count for every lane: weights are worked out together
+            float v[N];
+            x.load_if(mine_first + i < mine_last, mine_first + i, v);
+            add_kept(v, min_weight, sum, equal);
+        }
+        // Running sums over the block: of the ties, then of the weights with the ties that are kept.
+        const Whole equal_upto = warp_inclusive(equal, lane);
+        __syncthreads();
+        if (lane == 31) sh.part[warp] = equal_upto;
+        __syncthreads();
+        Whole seen = pair_ties + (second ? even_ties : 0) + equal_upto - equal;
+        for (int w = 0; w < warp; ++w) seen += sh.part[w];
+        const double mine = sum * weight_of.factor + tied(seen, equal, cut_weight);
+        const double mine_upto = warp_inclusive(mine, lane);
+        if (lane == 31) sh.part_mass[warp] = mine_upto;
+        if (t == 0) sh.found = ~0ull;
+        __syncthreads();
+        double before = 0.0;
+        for (int w = 0; w < warp; ++w) before += sh.part_mass[w];
+        // The lowest thread whose running sum passes the rest, else the last one with a weight.
+        const Whole ticket = before + mine_upto > rest ? t : 2 * SAMPLE_THREADS - t;
+        if (mine > 0.0) atomicMin(&sh.found, ticket);
+        __syncthreads();
+        if (!(mine > 0.0) || sh.found != ticket) return;
+        double running = before + mine_upto - mine;
+        int64_t id = -1;
+        for (int g = mine_first; g < mine_last; ++g) {
+            float v[N];
+            x.load(g, v);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const uint32_t k = score_key(v[j]);
+                if (k == 0 || k < cut) continue;
+                if (cut != 0 && k == cut && seen++ >= ties) continue;
+                const double w = score_weight(v[j], top, inv);
+                if (!(w >= min_p || k == top_key) || w == 0.0 || running > rest) continue;
+                id = x.id(g) + j;
+                running += w;
+            }
+            if (running > rest) break;
+        }
+        p.ids[row] = id;
+    }
 
-    // This block holds it: its threads share the part's groups, each a run of them in id order.
-    const double rest = target - (pair_before + (second ? even : 0.0));
-    const unsigned long long seen_before = pair_ties + (second ? even_ties : 0);
-    const int part_first = min(first_group + (part % SAMPLE_WARPS) * per_warp, last_group);
-    const int part_last = min(part_first + per_warp, last_group);
-    const int per_thread = (part_last - part_first + SAMPLE_THREADS - 1) / SAMPLE_THREADS;
-    const int mine_first = min(part_first + t * per_thread, part_last), mine_last = min(mine_first + per_thread, part_last);
-    double sum = 0.0;
-    unsigned long long equal = 0;
-    for (int i = 0; i < per_thread; ++i) { // the same count for every lane: weights are worked out together
-        float v[N];
-        if (mine_first + i < mine_last) {
-            x.load(mine_first + i, v);
-        } else {
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = -INFINITY;
+    __device__ __forceinline__ void run(int64_t row)
+    {
+        if (t == 0) {
+            sh.listed = 0;
+            sh.probe_low = 0xffffffffu;
         }
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const uint32_t k = score_key(v[j]);
-            if (cut != 0 && k == cut) ++equal;
-            if (k <= cut) v[j] = -INFINITY;
-            const double w = weight_of(v[j], p.taylor);
-            if (v[j] > -INFINITY && (w >= min_weight || v[j] == top)) sum += w;
-        }
-    }
-    sum *= weight_of.factor;
-    // Running sums over the block: of the ties, then of the weights with the ties that are kept.
-    const unsigned long long equal_upto = warp_inclusive(equal, lane);
-    __syncthreads();
-    if (lane == 31) sh.part[warp] = equal_upto;
-    __syncthreads();
-    unsigned long long seen = seen_before + equal_upto - equal;
-    for (int w = 0; w < warp; ++w) seen += sh.part[w];
-    const double mine = sum + clipped(seen, equal);
-    const double mine_upto = warp_inclusive(mine, lane);
-    if (lane == 31) sh.part_mass[warp] = mine_upto;
-    if (t == 0) sh.found = ~0ull;
-    __syncthreads();
-    double before = 0.0;
-    for (int w = 0; w < warp; ++w) before += sh.part_mass[w];
-    // The lowest thread whose running sum passes the rest, else the last one with a weight.
-    if (mine > 0.0) {
-        const bool passes = before + mine_upto > rest;
-        atomicMin(&sh.found, passes ? static_cast<unsigned long long>(t) : static_cast<unsigned long long>(2 * SAMPLE_THREADS - t));
-    }
-    __syncthreads();
-    const unsigned long long chosen = sh.found;
-    if (chosen != static_cast<unsigned long long>(t) && chosen != static_cast<unsigned long long>(2 * SAMPLE_THREADS - t)) return;
-    if (!(mine > 0.0)) return;
-    double running = before + mine_upto - mine;
-    int64_t id = -1;
-    for (int g = mine_first; g < mine_last; ++g) {
-        float v[N];
-        x.load(g, v);
-        for (int j = 0; j < N; ++j) {
-            const uint32_t k = score_key(v[j]);
-            if (k == 0 || k < cut) continue;
-            if (cut != 0 && k == cut && seen++ >= ties) continue;
-            const double w = score_weight(v[j], top, inv);
-            if (!(w >= min_p || k == top_key) || w == 0.0) continue;
-            id = x.id(g) + j;
-            running += w;
-            if (running > rest) {
-                p.ids[row] = id;
-                return;
+        if (t < 16) sh.probe_counts[t] = 0;
+        __syncthreads();
+        probe();
+        if (listing && need_mass) stream<true, true>();
+        else if (listing) stream<false, true>();
+        else if (need_mass) stream<true, false>();
+        else stream<false, false>();
+        {
+            const uint32_t key = __reduce_max_sync(FULL_WARP, score_key(warp_top));
+            const double sum = warp_sum(warp_mass);
+            if (lane == 0) {
+                sh.best[warp] = key;
+                sh.mass[warp] = reference > LONE ? sum * weight_of.factor : 0.0;
+                sh.reference[warp] = reference;
             }
         }
+        everyone();
+
+        // Every warp of every block works out the row's totals for itself.
+        top_key = 0;
+        for (int e = lane; e < parts; e += 32) top_key = max(top_key, block_at(e / SAMPLE_WARPS).best[e % SAMPLE_WARPS]);
+        top_key = __reduce_max_sync(FULL_WARP, top_key);
+        top = key_score(top_key);
+        const unsigned int listed = cluster_listed();
+        const bool lone = top == INFINITY || top < LONE; // no list, no sums
+        double total = 0.0; // sum of all weights, relative to the highest score
+        if (top_key != 0 && !lone && need_mass) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int e = 2 * lane + h;
+                if (e < parts) {
+                    SampleShared& from = block_at(e / SAMPLE_WARPS);
+                    const double m = from.mass[e % SAMPLE_WARPS];
+                    if (m > 0.0) part_mass[h] = m / score_weight(top, from.reference[e % SAMPLE_WARPS], inv);
+                }
+            }
+            total = warp_sum(part_mass[0] + part_mass[1]);
+        }
+        if (top_key == 0) {
+            if (rank == 0 && t == 0) p.ids[row] = -1;
+            everyone(); // the last look at the other blocks
+            return;
+        }
+        double listed_mass = 0.0; // weight of the scores from `below` up
+        float below = INFINITY;
+        if (listing && !lone && listed <= SAMPLE_LIST) {
+            if (rank == 0) {
+                const bool done = draw_from_list(static_cast<int>(listed), total, row);
+                if (t == 0) sh.outcome = done;
+            }
+            everyone();
+            const bool done = block_at(0).outcome != 0;
+            listed_mass = block_at(0).listed_mass;
+            below = key_score(threshold);
+            everyone();
+            if (done) return;
+        }
+
+        weight_of.refer(lone ? 0.0f : top, inv);
+        const double min_weight = min_p / weight_of.factor; // in the units of weight_of
+        bool summed = !filtered && !lone; // part_mass and part_ties hold what each warp's ids keep
+        if (lone) {
+            Whole c = 0;
+            each([&](float, uint32_t k, uint32_t) { c += k == top_key; });
+            c = cluster_total(c);
+            if (top_k > 0) c = min(c, static_cast<Whole>(top_k));
+            if (nucleus) c = static_cast<Whole>(fmax(1.0, ceil(top_p * static_cast<double>(c))));
+            cut = top_key;
+            ties = c;
+        } else if (top_k > 0) {
+            narrow<false>(static_cast<Whole>(top_k));
+            if (nucleus) {
+                Whole m = 0;
+                each([&](float v, uint32_t k, uint32_t) { m += k > cut ? whole(score_weight(v, top, inv)) : Whole{0}; });
+                m = cluster_total(m);
+                if (cut != 0) m += ties * whole(score_weight(key_score(cut), top, inv));
+                const double want = ceil(top_p * static_cast<double>(m));
+                narrow<true>(want > 1.0 ? static_cast<Whole>(want) : Whole{1});
+            }
+        } else if (nucleus) {
+            const double need = top_p * total;
+            if (border_in_window(need, listed_mass, below)) {
+                summed = !floor_p;
+            } else {
+                const double want = ceil(need * unit);
+                narrow<true>(want > 1.0 ? static_cast<Whole>(want) : Whole{1});
+            }
+        }
+        if (!summed) sum_parts(min_weight);
+        everyone(); // the last look at the other blocks
+        draw(row, min_weight);
     }
-    p.ids[row] = id;
+};
+
+// Grid: rows * cluster blocks, `cluster` neighbours per row.
+template <typename T>
+__global__ void __launch_bounds__(SAMPLE_THREADS, 4) povs_sample_kernel(const __grid_constant__ SampleParams p)
+{
+    __shared__ SampleShared sh;
+    const int64_t row = blockIdx.x / p.cluster;
+    SampleRow<T>(p, sh, row).run(row);
 }
 
 } // namespace povs
