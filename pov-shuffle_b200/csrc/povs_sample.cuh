@@ -50,6 +50,7 @@ constexpr int SAMPLE_LIST = 2048;   // listed scores per block, and per row
 constexpr int SAMPLE_TARGET = 1024; // listed scores aimed at where no top_k says how many
 constexpr int SAMPLE_PROBE = 4096;  // scores probed
 constexpr int SAMPLE_BINS = 1024;
+constexpr int SAMPLE_PARTS = 64; // runs of ids whose weights are summed apart, per row
 
 // Order of scores as an unsigned number: 0 for what is never drawn (NaN, -infinity), then the
 // numbers from the lowest up (+0 and -0 are the same number).
@@ -183,9 +184,9 @@ struct SampleShared {
     unsigned int counts[SAMPLE_BINS];
     // Read by the other blocks of the cluster.
     uint32_t best[SAMPLE_WARPS]; // each warp's highest key
-    double mass[SAMPLE_WARPS];             // of each warp's ids, which follow one another
-    float reference[SAMPLE_WARPS];
-    unsigned int ties[SAMPLE_WARPS];
+    double mass[SAMPLE_PARTS];     // of each of this block's parts, which follow one another in id order
+    float reference[SAMPLE_PARTS]; // that the mass is relative to
+    unsigned int ties[SAMPLE_PARTS];
     unsigned long long exchange[2];
     unsigned int listed;
     int outcome;
@@ -218,9 +219,9 @@ template <typename T> struct SampleRow {
     Groups x;
     WarpExp weight_of;
     int blocks, rank, t, lane, warp;
-    // This block's groups, and within them each warp's, in id order.
-    int per_block, per_warp, first_group, last_group, warp_first, warp_last;
-    int parts; // warps of the cluster
+    // This block's groups, and within them its parts' (as many to each warp), in id order.
+    int per_block, per_part, first_group, last_group;
+    int parts, warp_parts; // of this block, of each warp
     // The row's settings.
     int64_t top_k;
     double top_p, min_p, inv, u;
@@ -233,13 +234,12 @@ template <typename T> struct SampleRow {
     bool listing;
     // What the stream leaves.
     float top, warp_top, reference;
-    double warp_mass;
     uint32_t top_key;
     // Kept are the keys above `cut` and, in id order, the first `ties` of those equal to it (0: all).
     uint32_t cut = 0;
     Whole ties = 0;
     int parity = 0;
-    // Warps 2 lane and 2 lane + 1 of the cluster, which follow one another in id order.
+    // Parts 2 lane and 2 lane + 1 of the row.
     double part_mass[2] = {0.0, 0.0};
     Whole part_ties[2] = {0, 0};
 
@@ -253,12 +253,11 @@ template <typename T> struct SampleRow {
         lane = t & 31;
         warp = t >> 5;
         per_block = (x.groups + blocks - 1) / blocks;
-        per_warp = (per_block + SAMPLE_WARPS - 1) / SAMPLE_WARPS;
+        parts = SAMPLE_PARTS / blocks;
+        warp_parts = parts / SAMPLE_WARPS;
+        per_part = (per_block + parts - 1) / parts;
         first_group = min(rank * per_block, x.groups);
         last_group = min(first_group + per_block, x.groups);
-        warp_first = min(first_group + warp * per_warp, last_group);
-        warp_last = min(warp_first + per_warp, last_group);
-        parts = blocks * SAMPLE_WARPS;
         const double temperature = p.temperatures != nullptr ? p.temperatures[row] : p.temperature;
         top_p = p.top_ps != nullptr ? p.top_ps[row] : p.top_p;
         min_p = p.min_ps != nullptr ? p.min_ps[row] : p.min_p;
@@ -289,6 +288,7 @@ template <typename T> struct SampleRow {
         else __syncthreads();
     }
     __device__ __forceinline__ SampleShared& block_at(int r) { return blocks > 1 ? *cluster.map_shared_rank(&sh, r) : sh; }
+    __device__ __forceinline__ int part_first(int q) const { return min(first_group + q * per_part, last_group); }
     __device__ __forceinline__ Whole whole(double w) const { return static_cast<Whole>(llrint(w * unit)); }
     __device__ __forceinline__ static float score_of(Entry c) { return key_score(static_cast<uint32_t>(c >> 32)); }
 
@@ -413,37 +413,47 @@ template <typename T> struct SampleRow {
     {
         constexpr int UNROLL = 16 / N;
         float limit = -INFINITY;
-        double sums[2] = {0.0, 0.0};
         warp_top = reference = -INFINITY;
-        const int full_first = max(warp_first, x.lead > 0 ? 1 : 0);
-        const int full_last = min(warp_last, static_cast<int>((x.width + x.lead) / N));
         const uint4* vectors = reinterpret_cast<const uint4*>(x.x - x.lead);
-        int g = full_first + lane;
-        for (; g - lane + 32 * UNROLL <= full_last; g += 32 * UNROLL) {
-            uint4 raw[UNROLL];
-            float v[UNROLL][N];
+        // Without sums to keep apart, a warp's parts are one run.
+        for (int q = warp * warp_parts; q < (warp + 1) * warp_parts; q += MASS ? 1 : warp_parts) {
+            double sums[2] = {0.0, 0.0};
+            const int from = part_first(q), to = part_first(MASS ? q + 1 : q + warp_parts);
+            const int full_first = max(from, x.lead > 0 ? 1 : 0);
+            const int full_last = min(to, static_cast<int>((x.width + x.lead) / N));
+            int g = full_first + lane;
+            for (; g - lane + 32 * UNROLL <= full_last; g += 32 * UNROLL) {
+                uint4 raw[UNROLL];
+                float v[UNROLL][N];
 #pragma unroll
-            for (int i = 0; i < UNROLL; ++i) raw[i] = __ldg(vectors + g + 32 * i);
+                for (int i = 0; i < UNROLL; ++i) raw[i] = __ldg(vectors + g + 32 * i);
 #pragma unroll
-            for (int i = 0; i < UNROLL; ++i) x.unpack(raw[i], v[i]);
-            take<MASS, LIST, UNROLL>(v, g, limit, sums);
-        }
-        for (; g - lane < full_last; g += 32) {
-            float v[1][N];
-            x.load_if(g < full_last, g, v[0]);
-            take<MASS, LIST, 1>(v, g, limit, sums);
-        }
-#pragma unroll 1
-        for (int end = 0; end < 2; ++end) {
-            const int at = end == 0 ? 0 : x.groups - 1;
-            const bool outside = end == 0 ? x.lead > 0 : at >= full_last && (at > 0 || x.lead == 0);
-            if (outside && warp_first <= at && at < warp_last) {
+                for (int i = 0; i < UNROLL; ++i) x.unpack(raw[i], v[i]);
+                take<MASS, LIST, UNROLL>(v, g, limit, sums);
+            }
+            for (; g - lane < full_last; g += 32) {
                 float v[1][N];
-                x.load_if(lane == 0, at, v[0]);
-                take<MASS, LIST, 1>(v, at, limit, sums);
+                x.load_if(g < full_last, g, v[0]);
+                take<MASS, LIST, 1>(v, g, limit, sums);
+            }
+#pragma unroll 1
+            for (int end = 0; end < 2; ++end) {
+                const int at = end == 0 ? 0 : x.groups - 1;
+                const bool outside = end == 0 ? x.lead > 0 : at >= full_last && (at > 0 || x.lead == 0);
+                if (outside && from <= at && at < to) {
+                    float v[1][N];
+                    x.load_if(lane == 0, at, v[0]);
+                    take<MASS, LIST, 1>(v, at, limit, sums);
+                }
+            }
+            if (MASS) {
+                const double sum = warp_sum(sums[0] + sums[1]);
+                if (lane == 0) {
+                    sh.mass[q] = reference > LONE && sum > 1e-90 ? sum * weight_of.factor : 0.0; // masked scores alone: 0
+                    sh.reference[q] = reference;
+                }
             }
         }
-        warp_mass = sums[0] + sums[1];
     }
 
     // --- Work on a list of n entries in sh.list, their weights in sh.weight.
@@ -785,7 +795,7 @@ template <typename T> struct SampleRow {
     // A nucleus whose border lies below the list (scores from `below` up weigh listed_mass).  Counts of
     // the scores below it by bins of their distance from the top, each taken at its bin's middle, place
     // the border to a small part of a bin; the next reading sums the weights above a window around
-    // that place and lists the window, and the border is found inside, with each warp's kept weight.  False where it lies outside.
+    // that place and lists the window, and the border is found inside, with each part's kept weight.  False where it lies outside.
     __device__ __forceinline__ bool border_in_window(double need, double listed_mass, float below)
     {
         const float range = static_cast<float>(fmin(static_cast<double>(top) - static_cast<double>(key_score(sh.probe_low)), 45.0 / inv));
@@ -814,42 +824,45 @@ template <typename T> struct SampleRow {
         const float from = place - half, to = place + half;
         if (t == 0) sh.listed = 0;
         __syncthreads();
-        double sum = 0.0;
-        for (int g0 = warp_first; g0 < warp_last; g0 += 32) {
-            const int g = g0 + lane;
-            float v[N];
-            x.load_if(g < warp_last, g, v);
-            bool any = false;
-            const uint32_t id = static_cast<uint32_t>(x.id(g));
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const float y = (top - v[j]) * per;
-                if (y < from) {
-                    any = true;
-                } else {
-                    if (y <= to && v[j] > -INFINITY) {
-                        const unsigned int at = atomicAdd(&sh.listed, 1u);
-                        if (at < SAMPLE_LIST) sh.list[at] = (static_cast<Entry>(score_key(v[j])) << 32) | ~(id + j);
-                    }
-                    v[j] = -INFINITY;
-                }
-            }
-            if (__any_sync(FULL_WARP, any)) {
+        for (int q = warp * warp_parts; q < (warp + 1) * warp_parts; ++q) {
+            double sum = 0.0;
+            const int last = part_first(q + 1);
+            for (int g0 = part_first(q); g0 < last; g0 += 32) {
+                const int g = g0 + lane;
+                float v[N];
+                x.load_if(g < last, g, v);
+                bool any = false;
+                const uint32_t id = static_cast<uint32_t>(x.id(g));
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
-                    const double w = weight_of(v[j], p.poly);
-                    if (v[j] > -INFINITY) sum += w;
+                    const float y = (top - v[j]) * per;
+                    if (y < from) {
+                        any = true;
+                    } else {
+                        if (y <= to && v[j] > -INFINITY) {
+                            const unsigned int at = atomicAdd(&sh.listed, 1u);
+                            if (at < SAMPLE_LIST) sh.list[at] = (static_cast<Entry>(score_key(v[j])) << 32) | ~(id + j);
+                        }
+                        v[j] = -INFINITY;
+                    }
+                }
+                if (__any_sync(FULL_WARP, any)) {
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        const double w = weight_of(v[j], p.poly);
+                        if (v[j] > -INFINITY) sum += w;
+                    }
                 }
             }
+            sum = warp_sum(sum);
+            if (lane == 0) sh.mass[q] = sum * weight_of.factor;
         }
-        sum = warp_sum(sum);
-        if (lane == 0) sh.mass[warp] = sum * weight_of.factor;
         everyone();
         const unsigned int listed = cluster_listed();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int e = 2 * lane + h;
-            part_mass[h] = e < parts ? block_at(e / SAMPLE_WARPS).mass[e % SAMPLE_WARPS] : 0.0;
+            part_mass[h] = block_at(e / parts).mass[e % parts];
         }
         const double rest = (need - warp_sum(part_mass[0] + part_mass[1])) * unit;
         const bool inside = listed <= SAMPLE_LIST && rest >= 1.0;
@@ -870,9 +883,9 @@ template <typename T> struct SampleRow {
                 const Entry c = sh.list[i];
                 const uint32_t k = static_cast<uint32_t>(c >> 32);
                 if (k < key) continue;
-                // The warp whose ids hold it.
+                // The part that holds it.
                 const int g = static_cast<int>((static_cast<int64_t>(~static_cast<uint32_t>(c)) + x.lead) / N);
-                const int e = g / per_block * SAMPLE_WARPS + g % per_block / per_warp;
+                const int e = g / per_block * parts + g % per_block / per_part;
                 if (k > key) atomicAdd(&sh.bins[e], whole(sh.weight[i]));
                 else atomicAdd(&sh.counts[e], 1u);
                 if (c >= border && k == key) atomicAdd(&sh.few, 1);
@@ -890,10 +903,8 @@ template <typename T> struct SampleRow {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int e = 2 * lane + h;
-                if (e < parts) {
-                    part_mass[h] += static_cast<double>(block_at(0).bins[e]) / unit;
-                    part_ties[h] = block_at(0).counts[e];
-                }
+                part_mass[h] += static_cast<double>(block_at(0).bins[e]) / unit;
+                part_ties[h] = block_at(0).counts[e];
             }
         }
         everyone();
@@ -927,30 +938,29 @@ template <typename T> struct SampleRow {
     }
     __device__ __forceinline__ void sum_parts(double min_weight)
     {
-        double sum = 0.0;
-        Whole equal = 0;
-        for (int g0 = warp_first; g0 < warp_last; g0 += 32) {
-            float v[N];
-            x.load_if(g0 + lane < warp_last, g0 + lane, v);
-            add_kept(v, min_weight, sum, equal);
-        }
-        sum = warp_sum(sum) * weight_of.factor;
-        equal = warp_sum(equal);
-        if (lane == 0) {
-            sh.mass[warp] = sum;
-            sh.ties[warp] = static_cast<unsigned int>(equal);
+        for (int q = warp * warp_parts; q < (warp + 1) * warp_parts; ++q) {
+            double sum = 0.0;
+            Whole equal = 0;
+            const int last = part_first(q + 1);
+            for (int g0 = part_first(q); g0 < last; g0 += 32) {
+                float v[N];
+                x.load_if(g0 + lane < last, g0 + lane, v);
+                add_kept(v, min_weight, sum, equal);
+            }
+            sum = warp_sum(sum) * weight_of.factor;
+            equal = warp_sum(equal);
+            if (lane == 0) {
+                sh.mass[q] = sum;
+                sh.ties[q] = static_cast<unsigned int>(equal);
+            }
         }
         everyone();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int e = 2 * lane + h;
-            part_mass[h] = 0.0;
-            part_ties[h] = 0;
-            if (e < parts) {
-                SampleShared& from = block_at(e / SAMPLE_WARPS);
-                part_mass[h] = from.mass[e % SAMPLE_WARPS];
-                part_ties[h] = from.ties[e % SAMPLE_WARPS];
-            }
+            SampleShared& from = block_at(e / parts);
+            part_mass[h] = from.mass[e % parts];
+            part_ties[h] = from.ties[e % parts];
         }
     }
     __device__ __forceinline__ void draw(int64_t row, double min_weight)
@@ -972,14 +982,13 @@ template <typename T> struct SampleRow {
         const Whole pair_ties = __shfl_sync(FULL_WARP, ties_before, pair), even_ties = __shfl_sync(FULL_WARP, part_ties[0], pair);
         const bool second = !(even > 0.0 && before_pair + even > target) && odd > 0.0;
         const int part = 2 * pair + second;
-        if (some == 0 || part / SAMPLE_WARPS != rank) return;
+        if (some == 0 || part / parts != rank) return;
 
         // This block holds it: its threads share the part's groups, each a run of them in id order.
         const double rest = target - (before_pair + (second ? even : 0.0));
-        const int part_first = min(first_group + (part % SAMPLE_WARPS) * per_warp, last_group);
-        const int part_last = min(part_first + per_warp, last_group);
-        const int per_thread = (part_last - part_first + SAMPLE_THREADS - 1) / SAMPLE_THREADS;
-        const int mine_first = min(part_first + t * per_thread, part_last), mine_last = min(mine_first + per_thread, part_last);
+        const int from = part_first(part % parts), to = part_first(part % parts + 1);
+        const int per_thread = (to - from + SAMPLE_THREADS - 1) / SAMPLE_THREADS;
+        const int mine_first = min(from + t * per_thread, to), mine_last = min(mine_first + per_thread, to);
         double sum = 0.0;
         Whole equal = 0;
         for (int i = 0; i < per_thread; ++i) { // the same count for every lane: weights are worked out together
@@ -1041,18 +1050,13 @@ template <typename T> struct SampleRow {
         else stream<false, false>();
         {
             const uint32_t key = __reduce_max_sync(FULL_WARP, score_key(warp_top));
-            const double sum = warp_sum(warp_mass);
-            if (lane == 0) {
-                sh.best[warp] = key;
-                sh.mass[warp] = reference > LONE ? sum * weight_of.factor : 0.0;
-                sh.reference[warp] = reference;
-            }
+            if (lane == 0) sh.best[warp] = key;
         }
         everyone();
 
         // Every warp of every block works out the row's totals for itself.
         top_key = 0;
-        for (int e = lane; e < parts; e += 32) top_key = max(top_key, block_at(e / SAMPLE_WARPS).best[e % SAMPLE_WARPS]);
+        for (int e = lane; e < blocks * SAMPLE_WARPS; e += 32) top_key = max(top_key, block_at(e / SAMPLE_WARPS).best[e % SAMPLE_WARPS]);
         top_key = __reduce_max_sync(FULL_WARP, top_key);
         top = key_score(top_key);
         const unsigned int listed = cluster_listed();
@@ -1062,11 +1066,9 @@ template <typename T> struct SampleRow {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int e = 2 * lane + h;
-                if (e < parts) {
-                    SampleShared& from = block_at(e / SAMPLE_WARPS);
-                    const double m = from.mass[e % SAMPLE_WARPS];
-                    if (m > 0.0) part_mass[h] = m / score_weight(top, from.reference[e % SAMPLE_WARPS], inv);
-                }
+                SampleShared& from = block_at(e / parts);
+                const double m = from.mass[e % parts];
+                if (m > 0.0) part_mass[h] = m / score_weight(top, from.reference[e % parts], inv);
             }
             total = warp_sum(part_mass[0] + part_mass[1]);
         }
@@ -1092,7 +1094,7 @@ template <typename T> struct SampleRow {
 
         weight_of.refer(lone ? 0.0f : top, inv);
         const double min_weight = min_p / weight_of.factor; // in the units of weight_of
-        bool summed = !filtered && !lone; // part_mass and part_ties hold what each warp's ids keep
+        bool summed = !filtered && !lone; // part_mass and part_ties hold what each part's ids keep
         if (lone) {
             Whole c = 0;
             each([&](float, uint32_t k, uint32_t) { c += k == top_key; });
