@@ -106,7 +106,7 @@ struct WarpExp {
         double q = fma(r, poly[3], poly[2]);
         q = fma(r, q, poly[1]);
         q = fma(r, q, poly[0]);
-        const double at = __shfl_sync(FULL_WARP, step, n & 31);
+        const double at = __shfl_sync(FULL_WARP, step, n); // lane n modulo 32
         const double base = __hiloint2double(__double2hiint(at) + (n & ~31) * (1 << 15), __double2loint(at));
         return fma(base * r, q, base);
     }
@@ -422,13 +422,25 @@ template <typename T> struct SampleRow {
             const int full_first = max(from, x.lead > 0 ? 1 : 0);
             const int full_last = min(to, static_cast<int>((x.width + x.lead) / N));
             int g = full_first + lane;
+            uint4 next[UNROLL];
+            if (!MASS && g - lane + 32 * UNROLL <= full_last) {
+#pragma unroll
+                for (int i = 0; i < UNROLL; ++i) next[i] = __ldg(vectors + g + 32 * i);
+            }
             for (; g - lane + 32 * UNROLL <= full_last; g += 32 * UNROLL) {
-                uint4 raw[UNROLL];
                 float v[UNROLL][N];
+                if (MASS) {
 #pragma unroll
-                for (int i = 0; i < UNROLL; ++i) raw[i] = __ldg(vectors + g + 32 * i);
+                    for (int i = 0; i < UNROLL; ++i) next[i] = __ldg(vectors + g + 32 * i);
+                }
 #pragma unroll
-                for (int i = 0; i < UNROLL; ++i) x.unpack(raw[i], v[i]);
+                for (int i = 0; i < UNROLL; ++i) x.unpack(next[i], v[i]);
+                // Without sums a batch ahead is in flight (82 -> 77 us for top_k on 512 rows of 131072; with
+                // sums the registers that takes cost more than it gains).
+                if (!MASS && g - lane + 64 * UNROLL <= full_last) {
+#pragma unroll
+                    for (int i = 0; i < UNROLL; ++i) next[i] = __ldg(vectors + g + 32 * (UNROLL + i));
+                }
                 take<MASS, LIST, UNROLL>(v, g, limit, sums);
             }
             for (; g - lane < full_last; g += 32) {
@@ -635,17 +647,35 @@ template <typename T> struct SampleRow {
     }
 
     // --- Rows that are read again, all blocks together, each on its own groups.
+    // f(scores, group) for the groups first, first + step, ... below last, four in flight; the same number
+    // of calls for every `first` of a run of `step` lanes or threads, groups past `last` as -infinity.
+    template <typename F> __device__ __forceinline__ void groups_of(int first, int step, int last, int rounds, F f)
+    {
+        for (int i = 0; i < rounds; i += 4) {
+            float v[4][N];
+#pragma unroll
+            for (int m = 0; m < 4; ++m) x.load_if(i + m < rounds && first + (i + m) * step < last, first + (i + m) * step, v[m]);
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+                if (i + m < rounds) f(v[m], first + (i + m) * step);
+        }
+    }
     template <typename F> __device__ __forceinline__ void each(F f)
     {
-        for (int g = first_group + t; g < last_group; g += SAMPLE_THREADS) {
-            float v[N];
-            x.load(g, v);
+        const int rounds = (last_group - first_group + SAMPLE_THREADS - 1) / SAMPLE_THREADS;
+        groups_of(first_group + t, SAMPLE_THREADS, last_group, rounds, [&](float (&v)[N], int g) {
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 const uint32_t k = score_key(v[j]);
                 if (k != 0) f(v[j], k, static_cast<uint32_t>(x.id(g) + j));
             }
-        }
+        });
+    }
+    // f(scores, group) for a part's groups, the warp together.
+    template <typename F> __device__ __forceinline__ void each_of_part(int q, F f)
+    {
+        const int from = part_first(q), to = part_first(q + 1);
+        groups_of(from + lane, 32, to, (to - from + 31) / 32, f);
     }
     __device__ __forceinline__ void clear_bins()
     {
@@ -801,14 +831,13 @@ template <typename T> struct SampleRow {
         const float range = static_cast<float>(fmin(static_cast<double>(top) - static_cast<double>(key_score(sh.probe_low)), 45.0 / inv));
         const float per = range > 0.0f ? SAMPLE_BINS / range : 0.0f;
         clear_bins();
-        for (int g = first_group + t; g < last_group; g += SAMPLE_THREADS) {
-            float v[N];
-            x.load(g, v);
+        groups_of(first_group + t, SAMPLE_THREADS, last_group, (last_group - first_group + SAMPLE_THREADS - 1) / SAMPLE_THREADS,
+                  [&](float (&v)[N], int) {
 #pragma unroll
-            for (int j = 0; j < N; ++j)
-                if (v[j] < below && v[j] > -INFINITY)
-                    atomicAdd(&sh.counts[static_cast<int>(fminf((top - v[j]) * per, SAMPLE_BINS - 1))], 1u);
-        }
+                      for (int j = 0; j < N; ++j)
+                          if (v[j] < below && v[j] > -INFINITY)
+                              atomicAdd(&sh.counts[static_cast<int>(fminf((top - v[j]) * per, SAMPLE_BINS - 1))], 1u);
+                  });
         cluster_bins();
         for (int b = t; b < SAMPLE_BINS; b += SAMPLE_THREADS) sh.bins[b] = whole(exp(-(b + 0.5) / per * inv)) * sh.counts[b];
         __syncthreads();
@@ -826,11 +855,7 @@ template <typename T> struct SampleRow {
         __syncthreads();
         for (int q = warp * warp_parts; q < (warp + 1) * warp_parts; ++q) {
             double sum = 0.0;
-            const int last = part_first(q + 1);
-            for (int g0 = part_first(q); g0 < last; g0 += 32) {
-                const int g = g0 + lane;
-                float v[N];
-                x.load_if(g < last, g, v);
+            each_of_part(q, [&](float (&v)[N], int g) {
                 bool any = false;
                 const uint32_t id = static_cast<uint32_t>(x.id(g));
 #pragma unroll
@@ -853,7 +878,7 @@ template <typename T> struct SampleRow {
                         if (v[j] > -INFINITY) sum += w;
                     }
                 }
-            }
+            });
             sum = warp_sum(sum);
             if (lane == 0) sh.mass[q] = sum * weight_of.factor;
         }
@@ -941,12 +966,7 @@ template <typename T> struct SampleRow {
         for (int q = warp * warp_parts; q < (warp + 1) * warp_parts; ++q) {
             double sum = 0.0;
             Whole equal = 0;
-            const int last = part_first(q + 1);
-            for (int g0 = part_first(q); g0 < last; g0 += 32) {
-                float v[N];
-                x.load_if(g0 + lane < last, g0 + lane, v);
-                add_kept(v, min_weight, sum, equal);
-            }
+            each_of_part(q, [&](float (&v)[N], int) { add_kept(v, min_weight, sum, equal); });
             sum = warp_sum(sum) * weight_of.factor;
             equal = warp_sum(equal);
             if (lane == 0) {
@@ -991,11 +1011,7 @@ template <typename T> struct SampleRow {
         const int mine_first = min(from + t * per_thread, to), mine_last = min(mine_first + per_thread, to);
         double sum = 0.0;
         Whole equal = 0;
-        for (int i = 0; i < per_thread; ++i) { // the same count for every lane: weights are worked out together
-            float v[N];
-            x.load_if(mine_first + i < mine_last, mine_first + i, v);
-            add_kept(v, min_weight, sum, equal);
-        }
+        groups_of(mine_first, 1, mine_last, per_thread, [&](float (&v)[N], int) { add_kept(v, min_weight, sum, equal); });
         // Running sums over the block: of the ties, then of the weights with the ties that are kept.
         const Whole equal_upto = warp_inclusive(equal, lane);
         __syncthreads();
