@@ -83,13 +83,11 @@ __device__ __forceinline__ void warp_best(uint64_t& key, int& index)
     }
 }
 
-// One warp per row, EPL scores per lane (expert lane + 32 * m).
-template <typename T, int EPL>
-__global__ void __launch_bounds__(128) povs_route_kernel(const __grid_constant__ RouteParams p)
+// One row by one warp with every score in 64 bits, EPL scores per lane (expert lane + 32 * m): the
+// definition itself, for rows that 32 bits leave open.
+template <typename T, int EPL> __device__ __noinline__ void route_row_exactly(const RouteParams& p, int64_t row)
 {
     const int lane = threadIdx.x & 31;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    if (row >= p.rows) return;
     const T* x = static_cast<const T*>(p.logits) + row * p.row_stride;
     const int n = p.n_experts;
 
@@ -209,6 +207,251 @@ __global__ void __launch_bounds__(128) povs_route_kernel(const __grid_constant__
         if (p.renormalize) w = total == 0.0 ? 0.0 : w / total;
         p.experts[row * p.top_k + lane] = my_expert;
         p.weights[row * p.top_k + lane] = static_cast<float>(w);
+    }
+}
+
+__device__ __forceinline__ float warp_max(float v)
+{
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "r"(FULL_WARP));
+    return r;
+}
+__device__ __forceinline__ float exp2_fast(float v)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float reciprocal_fast(float v)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+constexpr float LOG2E = 1.44269504f;
+
+constexpr int ROUTE_WARPS = 4;
+
+// Choosing in 32 bits what the definition decides in 64.
+//
+// A choice score c, less the row's highest and plus 3.9998, is a float in [2, 4): its 23 mantissa bits
+// are steps of 2^-22, and above an index that counts down they make one whole number per expert whose
+// maximum is the next choice, ties by the lowest index (scores 2 and more below the highest all become
+// 2 + 2^-22).  Without a bias or groups the order of the scores is the logits', and c is a logit / 8, exact
+// but for one rounding of half a step.  Otherwise c is a score from 32-bit arithmetic plus its bias: the
+// exponential's argument is rounded by 2^-24 of its size z, z 2^-z <= 0.54, the exponential and the quotient
+// are good to 2^-22, a softmax's sum to (EPL + 5) 2^-24: in all below 2^-19 and 2^-24 for each of a lane's
+// scores, to which a bias adds 2^-24 of |c|.  Neighbours in the result no further apart than twice that
+// (`room` steps), and groups whose scores are as close, are told apart by
+// 64 bits (route_row_exactly), unless logit and bias are equal, a tie in either arithmetic.  Rows with
+// NaN, infinities or too few experts end there too, as they reach the lowest step.
+//
+// Bound by instructions: about 45 a lane's 8 experts for the scores, as many for the groups, 38 to sort a
+// lane's 8 numbers and 11 for each choice.
+template <typename T, int EPL, bool VECTOR>
+__global__ void __launch_bounds__(32 * ROUTE_WARPS, EPL <= 8 ? 8 : EPL <= 16 ? 5 : 3) povs_route_kernel(const __grid_constant__ RouteParams p)
+{
+    // Experts of a lane: V neighbours at a time (one load) where the rows' alignment allows.
+    constexpr int WIDEST = 16 / sizeof(T), V = !VECTOR ? 1 : EPL < WIDEST ? EPL : WIDEST;
+    constexpr int INDEX_BITS = EPL > 16 ? 10 : 9;
+    constexpr uint32_t INDEX_MASK = (1u << INDEX_BITS) - 1;
+    constexpr float TOP = 3.9998f, LOWEST = 2.0f + 1.0f / (1 << (31 - INDEX_BITS));
+    __shared__ float scores[ROUTE_WARPS][32 * EPL + 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int n = p.n_experts;
+    const bool grouped = p.top_groups < p.n_groups, by_logit = p.bias == nullptr && !grouped;
+    const int size = n / p.n_groups;
+    int lanes_per_group = 32;
+    while (lanes_per_group * p.n_groups > 32) lanes_per_group >>= 1;
+
+    auto expert = [&](int m) { return (m / V) * 32 * V + lane * V + m % V; };
+    int group[EPL];
+#pragma unroll
+    for (int m = 0; m < EPL; ++m) group[m] = grouped && expert(m) < n ? expert(m) / size : 0;
+
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * ROUTE_WARPS;
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROUTE_WARPS + warp; row < p.rows; row += stride) {
+        const T* x = static_cast<const T*>(p.logits) + row * p.row_stride;
+        float c[EPL];
+#pragma unroll
+        for (int i = 0; i < EPL / V; ++i) {
+            const int e = expert(i * V);
+            struct alignas(V * sizeof(T)) Few {
+                T v[V];
+            };
+            if (e < n) {
+                const Few few = *reinterpret_cast<const Few*>(x + e);
+#pragma unroll
+                for (int j = 0; j < V; ++j) c[i * V + j] = to_float(few.v[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) c[i * V + j] = -INFINITY;
+            }
+        }
+        // Scores.
+        float highest = -INFINITY, inv = 0.0f;
+        if (!p.sigmoid || by_logit) {
+#pragma unroll
+            for (int m = 0; m < EPL; ++m) highest = fmaxf(highest, c[m]);
+            highest = warp_max(highest);
+        }
+        const float top_logit = highest;
+        if (!p.sigmoid) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int m = 0; m < EPL; ++m) {
+                const float s = exp2_fast((c[m] - top_logit) * LOG2E);
+                sum += s;
+                if (!by_logit) c[m] = c[m] == -INFINITY ? -INFINITY : s;
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL_WARP, sum, o);
+            inv = 1.0f / sum;
+            if (!by_logit) {
+#pragma unroll
+                for (int m = 0; m < EPL; ++m) c[m] *= inv;
+            }
+        } else if (!by_logit) {
+#pragma unroll
+            for (int m = 0; m < EPL; ++m) c[m] = c[m] == -INFINITY ? -INFINITY : reciprocal_fast(1.0f + exp2_fast(c[m] * -LOG2E));
+        }
+        bool open = !p.sigmoid && !(inv <= 1.0001f && top_logit > -INFINITY); // NaN, infinities, nothing to choose
+        float room = 3.0f;
+        if (!by_logit) {
+            if (p.bias != nullptr) {
+#pragma unroll
+                for (int m = 0; m < EPL; ++m) c[m] += expert(m) < n ? __ldg(p.bias + expert(m)) : 0.0f;
+            }
+            if (grouped) {
+                // Rows of a group's scores, a few apart so that the groups' lanes hit different banks; each
+                // group's lanes take its two highest.
+                float* mine = scores[warp];
+#pragma unroll
+                for (int m = 0; m < EPL; ++m)
+                    if (expert(m) < n) mine[expert(m) + group[m] * lanes_per_group] = c[m];
+                __syncwarp();
+                const int g = lane / lanes_per_group;
+                float first = -INFINITY, second = -INFINITY;
+                if (g < p.n_groups)
+                    for (int i = lane % lanes_per_group; i < size; i += lanes_per_group) {
+                        const float v = mine[g * (size + lanes_per_group) + i];
+                        second = fmaxf(second, fminf(first, v));
+                        first = fmaxf(first, v);
+                        open |= v != v;
+                    }
+                __syncwarp();
+                for (int o = lanes_per_group / 2; o > 0; o >>= 1) {
+                    const float f = __shfl_xor_sync(FULL_WARP, first, o), s = __shfl_xor_sync(FULL_WARP, second, o);
+                    second = fmaxf(fminf(first, f), fmaxf(second, s));
+                    first = fmaxf(first, f);
+                }
+                const float score = p.group_max || size == 1 ? first : first + second;
+                // Groups surely before this one, and groups that may be.
+                const float slack = 8e-6f + 5e-7f * EPL + fabsf(score) * 1e-6f;
+                int sure = 0, maybe = 0;
+                for (int other = 0; other < p.n_groups; ++other) {
+                    const float v = __shfl_sync(FULL_WARP, score, other * lanes_per_group);
+                    sure += v > score + slack;
+                    maybe += other != g && !(v < score - slack);
+                }
+                const bool in = maybe < p.top_groups, real = g < p.n_groups;
+                open |= real && !in && sure < p.top_groups;
+                const unsigned kept = __ballot_sync(FULL_WARP, real && in);
+#pragma unroll
+                for (int m = 0; m < EPL; ++m)
+                    if (!((kept >> (group[m] * lanes_per_group)) & 1)) c[m] = -INFINITY;
+            }
+            highest = -INFINITY;
+#pragma unroll
+            for (int m = 0; m < EPL; ++m) highest = fmaxf(highest, c[m]);
+            highest = warp_max(highest);
+            room = 18.0f + EPL + fabsf(highest);
+        }
+        const float scale = by_logit ? 0.125f : 1.0f;
+        if (by_logit) highest *= 0.125f;
+        open |= !(fabsf(highest) < 1000.0f);
+        if (__any_sync(FULL_WARP, open)) {
+            route_row_exactly<T, EPL>(p, row);
+            continue;
+        }
+
+        // One whole number per expert, sorted within the lane, highest first.
+        const float offset = TOP - highest;
+        uint32_t key[EPL];
+#pragma unroll
+        for (int m = 0; m < EPL; ++m) {
+            const uint32_t bits = __float_as_uint(fmaxf(fmaf(c[m], scale, offset), LOWEST)) << 9;
+            key[m] = (bits & ~INDEX_MASK) | (INDEX_MASK - expert(m));
+        }
+#pragma unroll
+        for (int span = 2; span <= EPL; span *= 2)
+#pragma unroll
+            for (int step = span / 2; step > 0; step /= 2)
+#pragma unroll
+                for (int m = 0; m < EPL; ++m)
+                    if ((m & step) == 0) {
+                        const uint32_t a = key[m], b = key[m | step];
+                        const bool down = (m & span) == 0 || span == EPL;
+                        key[m] = down ? max(a, b) : min(a, b);
+                        key[m | step] = down ? min(a, b) : max(a, b);
+                    }
+        auto next = [&] {
+            const uint32_t best = __reduce_max_sync(FULL_WARP, key[0]);
+            if (key[0] == best) {
+#pragma unroll
+                for (int m = 0; m + 1 < EPL; ++m) key[m] = key[m + 1];
+                key[EPL - 1] = 0;
+            }
+            return best;
+        };
+        uint32_t chosen = 0; // lane j: the j-th choice
+        for (int j = 0; j < p.top_k; ++j) {
+            const uint32_t best = next();
+            if (lane == j) chosen = best;
+        }
+        const int e = static_cast<int>(INDEX_MASK - (chosen & INDEX_MASK));
+        const bool active = lane < p.top_k;
+        const float logit = active && e < n ? to_float(x[e]) : 0.0f;
+        const float bias = active && e < n && p.bias != nullptr ? __ldg(p.bias + e) : 0.0f;
+        // Told apart from the choice before?
+        constexpr int SHIFT = INDEX_BITS;
+        constexpr float STEP = INDEX_BITS > 9 ? 2.0f : 1.0f; // in units of 2^-22
+        const uint32_t before = __shfl_up_sync(FULL_WARP, chosen, 1);
+        const float logit_before = __shfl_up_sync(FULL_WARP, logit, 1), bias_before = __shfl_up_sync(FULL_WARP, bias, 1);
+        bool close = active && lane > 0 && static_cast<float>((before >> SHIFT) - (chosen >> SHIFT)) * STEP <= room &&
+                     !(logit == logit_before && bias == bias_before);
+        close |= active && ((chosen >> SHIFT) << (SHIFT - 9)) <= (1u << (INDEX_BITS - 9)); // the lowest step
+        // And the last from the rest: on past its ties.
+        const uint32_t last = __shfl_sync(FULL_WARP, chosen, p.top_k - 1);
+        const float logit_last = __shfl_sync(FULL_WARP, logit, p.top_k - 1), bias_last = __shfl_sync(FULL_WARP, bias, p.top_k - 1);
+        if (p.top_k < n)
+            for (;;) {
+                const uint32_t best = next();
+                if (static_cast<float>((last >> SHIFT) - (best >> SHIFT)) * STEP > room) break;
+                const int other = static_cast<int>(INDEX_MASK - (best & INDEX_MASK));
+                if (best == 0 || other >= n) break;
+                if (!(to_float(x[other]) == logit_last && (p.bias == nullptr || __ldg(p.bias + other) == bias_last))) {
+                    close = true;
+                    break;
+                }
+            }
+        if (__any_sync(FULL_WARP, close)) {
+            route_row_exactly<T, EPL>(p, row);
+            continue;
+        }
+        float s = 0.0f;
+        if (active) s = p.sigmoid ? 1.0f / (1.0f + exp2_fast(logit * -LOG2E)) : exp2_fast((logit - top_logit) * LOG2E) * inv;
+        float w = s * p.scale;
+        if (p.renormalize) {
+            float total = s;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(FULL_WARP, total, o);
+            w = total == 0.0f ? 0.0f : w / total;
+        }
+        if (active) {
+            p.experts[row * p.top_k + lane] = e;
+            p.weights[row * p.top_k + lane] = w;
+        }
     }
 }
 

@@ -101,16 +101,24 @@ int check_route(const povs::RouteParams& p, int32_t dtype, int32_t scoring, int3
     return POVS_OK;
 }
 
-template <typename T> void launch_route(const povs::RouteParams& p, cudaStream_t s)
+template <typename T, int EPL> void launch_route_of(const povs::RouteParams& p, int sms, cudaStream_t s)
 {
-    const unsigned grid = static_cast<unsigned>((p.rows + 3) / 4);
+    constexpr int V = EPL < 16 / static_cast<int>(sizeof(T)) ? EPL : 16 / static_cast<int>(sizeof(T));
+    const bool vector = p.n_experts % V == 0 && p.row_stride % V == 0 && address(p.logits) % (V * sizeof(T)) == 0;
+    const int grid = grid_for(p.rows, povs::ROUTE_WARPS, sms, 16);
+    if (vector) povs::povs_route_kernel<T, EPL, true><<<grid, 32 * povs::ROUTE_WARPS, 0, s>>>(p);
+    else povs::povs_route_kernel<T, EPL, false><<<grid, 32 * povs::ROUTE_WARPS, 0, s>>>(p);
+}
+
+template <typename T> void launch_route(const povs::RouteParams& p, int sms, cudaStream_t s)
+{
     const int epl = (p.n_experts + 31) / 32;
-    if (epl <= 1) povs::povs_route_kernel<T, 1><<<grid, 128, 0, s>>>(p);
-    else if (epl <= 2) povs::povs_route_kernel<T, 2><<<grid, 128, 0, s>>>(p);
-    else if (epl <= 4) povs::povs_route_kernel<T, 4><<<grid, 128, 0, s>>>(p);
-    else if (epl <= 8) povs::povs_route_kernel<T, 8><<<grid, 128, 0, s>>>(p);
-    else if (epl <= 16) povs::povs_route_kernel<T, 16><<<grid, 128, 0, s>>>(p);
-    else povs::povs_route_kernel<T, 32><<<grid, 128, 0, s>>>(p);
+    if (epl <= 1) launch_route_of<T, 1>(p, sms, s);
+    else if (epl <= 2) launch_route_of<T, 2>(p, sms, s);
+    else if (epl <= 4) launch_route_of<T, 4>(p, sms, s);
+    else if (epl <= 8) launch_route_of<T, 8>(p, sms, s);
+    else if (epl <= 16) launch_route_of<T, 16>(p, sms, s);
+    else launch_route_of<T, 32>(p, sms, s);
 }
 
 int check_rows(int64_t rows, int32_t top_k, int64_t n_slots)
@@ -275,9 +283,9 @@ extern "C" int povs_route_v1(const void* logits, int32_t dtype, int64_t rows, in
     r = enter(dg, device, &sms);
     if (r != POVS_OK) return r;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (dtype == POVS_FLOAT32) launch_route<float>(p, s);
-    else if (dtype == POVS_BFLOAT16) launch_route<__nv_bfloat16>(p, s);
-    else launch_route<__half>(p, s);
+    if (dtype == POVS_FLOAT32) launch_route<float>(p, sms, s);
+    else if (dtype == POVS_BFLOAT16) launch_route<__nv_bfloat16>(p, sms, s);
+    else launch_route<__half>(p, sms, s);
     return launched("route kernel");
 }
 
