@@ -246,8 +246,6 @@ constexpr int ROUTE_WARPS = 4;
 // 64 bits (route_row_exactly), unless logit and bias are equal, a tie in either arithmetic.  Rows with
 // NaN, infinities or too few experts end there too, as they reach the lowest step.
 //
-// Bound by instructions: about 45 a lane's 8 experts for the scores, as many for the groups, 38 to sort a
-// lane's 8 numbers and 11 for each choice.
 template <typename T, int EPL, bool VECTOR>
 __global__ void __launch_bounds__(32 * ROUTE_WARPS, EPL <= 8 ? 8 : EPL <= 16 ? 5 : 3) povs_route_kernel(const __grid_constant__ RouteParams p)
 {
@@ -261,13 +259,20 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, EPL <= 8 ? 8 : EPL <= 16 ? 5
     const int n = p.n_experts;
     const bool grouped = p.top_groups < p.n_groups, by_logit = p.bias == nullptr && !grouped;
     const int size = n / p.n_groups;
-    int lanes_per_group = 32;
-    while (lanes_per_group * p.n_groups > 32) lanes_per_group >>= 1;
-
     auto expert = [&](int m) { return (m / V) * 32 * V + lane * V + m % V; };
+    // Groups of whole loads, on a run of lanes whose number is a power of two, are scored in registers
+    // (`run` lanes), others through shared memory (`span` lanes each).
+    const int run = size % V == 0 && size / V <= 32 && (size / V & (size / V - 1)) == 0 ? size / V : 0;
+    int span_log2 = 5;
+    while ((p.n_groups << span_log2) > 32) --span_log2;
+    const int span = 1 << span_log2, my_group = lane >> span_log2, my_place = lane & (span - 1);
     int group[EPL];
 #pragma unroll
     for (int m = 0; m < EPL; ++m) group[m] = grouped && expert(m) < n ? expert(m) / size : 0;
+    constexpr bool KEEP_BIAS = EPL <= 8; // in registers, over the rows
+    float kept_bias[KEEP_BIAS ? EPL : 1];
+#pragma unroll
+    for (int m = 0; m < (KEEP_BIAS ? EPL : 0); ++m) kept_bias[m] = p.bias != nullptr && expert(m) < n ? p.bias[expert(m)] : 0.0f;
 
     const int64_t stride = static_cast<int64_t>(gridDim.x) * ROUTE_WARPS;
     for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROUTE_WARPS + warp; row < p.rows; row += stride) {
@@ -318,29 +323,76 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, EPL <= 8 ? 8 : EPL <= 16 ? 5
         bool open = !p.sigmoid && !(inv <= 1.0001f && top_logit > -INFINITY); // NaN, infinities, nothing to choose
         float room = 3.0f;
         if (!by_logit) {
-            if (p.bias != nullptr) {
+            if (KEEP_BIAS) {
+#pragma unroll
+                for (int m = 0; m < EPL; ++m) c[m] += kept_bias[KEEP_BIAS ? m : 0];
+            } else if (p.bias != nullptr) {
 #pragma unroll
                 for (int m = 0; m < EPL; ++m) c[m] += expert(m) < n ? __ldg(p.bias + expert(m)) : 0.0f;
             }
-            if (grouped) {
-                // Rows of a group's scores, a few apart so that the groups' lanes hit different banks; each
-                // group's lanes take its two highest.
+            if (grouped && run > 0) {
+                // Two highest of each load's V scores, then of the run's lanes.
+                float score[EPL / V];
+                unsigned taken = 0;
+#pragma unroll
+                for (int i = 0; i < EPL / V; ++i) {
+                    float first = c[i * V], second = -INFINITY;
+#pragma unroll
+                    for (int j = 1; j < V; ++j) {
+                        second = fmaxf(second, fminf(first, c[i * V + j]));
+                        first = fmaxf(first, c[i * V + j]);
+                    }
+                    for (int o = 1; o < run; o <<= 1) {
+                        const float f = __shfl_xor_sync(FULL_WARP, first, o), s = __shfl_xor_sync(FULL_WARP, second, o);
+                        second = fmaxf(fminf(first, f), fmaxf(second, s));
+                        first = fmaxf(first, f);
+                    }
+                    score[i] = p.group_max || size == 1 ? first : first + second;
+                    if (expert(i * V) >= n) score[i] = -INFINITY;
+                    open |= score[i] != score[i];
+                }
+                // The best group top_groups times, and once more for the distance to the rest.
+                float last = INFINITY;
+                for (int k = 0; k <= p.top_groups; ++k) {
+                    float best = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < EPL / V; ++i) best = fmaxf(best, (taken >> i) & 1 ? -INFINITY : score[i]);
+                    best = warp_max(best);
+                    if (k == p.top_groups) {
+                        open |= !(last - best > 8e-6f + 5e-7f * EPL + 1e-6f * fabsf(last));
+                        break;
+                    }
+                    int lanes = 0;
+#pragma unroll
+                    for (int i = 0; i < EPL / V; ++i) {
+                        const bool hit = score[i] == best && !((taken >> i) & 1);
+                        lanes += __popc(__ballot_sync(FULL_WARP, hit));
+                        if (hit) taken |= 1u << i;
+                    }
+                    open |= lanes != run;
+                    last = best;
+                }
+#pragma unroll
+                for (int m = 0; m < EPL; ++m)
+                    if (!((taken >> (m / V)) & 1)) c[m] = -INFINITY;
+            } else if (grouped) {
+                // Rows of a group's scores, `span` places apart so that the groups' lanes hit different banks;
+                // each group's lanes take its two highest.
                 float* mine = scores[warp];
 #pragma unroll
                 for (int m = 0; m < EPL; ++m)
-                    if (expert(m) < n) mine[expert(m) + group[m] * lanes_per_group] = c[m];
+                    if (expert(m) < n) mine[expert(m) + (group[m] << span_log2)] = c[m];
                 __syncwarp();
-                const int g = lane / lanes_per_group;
                 float first = -INFINITY, second = -INFINITY;
-                if (g < p.n_groups)
-                    for (int i = lane % lanes_per_group; i < size; i += lanes_per_group) {
-                        const float v = mine[g * (size + lanes_per_group) + i];
+                if (my_group < p.n_groups)
+                    for (int i = my_place; i < size; i += span) {
+                        const float v = mine[my_group * (size + span) + i];
                         second = fmaxf(second, fminf(first, v));
                         first = fmaxf(first, v);
                         open |= v != v;
                     }
                 __syncwarp();
-                for (int o = lanes_per_group / 2; o > 0; o >>= 1) {
+                for (int o = span / 2; o > 0; o >>= 1) {
                     const float f = __shfl_xor_sync(FULL_WARP, first, o), s = __shfl_xor_sync(FULL_WARP, second, o);
                     second = fmaxf(fminf(first, f), fmaxf(second, s));
                     first = fmaxf(first, f);
@@ -350,16 +402,16 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, EPL <= 8 ? 8 : EPL <= 16 ? 5
                 const float slack = 8e-6f + 5e-7f * EPL + fabsf(score) * 1e-6f;
                 int sure = 0, maybe = 0;
                 for (int other = 0; other < p.n_groups; ++other) {
-                    const float v = __shfl_sync(FULL_WARP, score, other * lanes_per_group);
+                    const float v = __shfl_sync(FULL_WARP, score, other << span_log2);
                     sure += v > score + slack;
-                    maybe += other != g && !(v < score - slack);
+                    maybe += other != my_group && !(v < score - slack);
                 }
-                const bool in = maybe < p.top_groups, real = g < p.n_groups;
+                const bool in = maybe < p.top_groups, real = my_group < p.n_groups;
                 open |= real && !in && sure < p.top_groups;
                 const unsigned kept = __ballot_sync(FULL_WARP, real && in);
 #pragma unroll
                 for (int m = 0; m < EPL; ++m)
-                    if (!((kept >> (group[m] * lanes_per_group)) & 1)) c[m] = -INFINITY;
+                    if (!((kept >> (group[m] << span_log2)) & 1)) c[m] = -INFINITY;
             }
             highest = -INFINITY;
 #pragma unroll
