@@ -172,7 +172,8 @@ def _i64_array(values) -> ctypes.Array:
 
 
 def current_stream_handle(device: torch.device) -> int:
-    return int(torch.cuda.current_stream(device).cuda_stream)
+    """The device's current cudaStream_t (the raw handle: 0.1 us, against 2.2 us for a Stream object)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def shuffle_device(
@@ -331,7 +332,7 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature, top_k, top
     """``povs_sample_v1``: one int64 id per row; the four settings are numbers or per-row tensors."""
     dev = logits.device
     rows, width = logits.shape
-    ids = torch.empty(rows, dtype=torch.int64, device=dev)
+    ids = logits.new_empty(rows, dtype=torch.int64)
     per_row = [v.data_ptr() if isinstance(v, torch.Tensor) else None for v in (temperature, top_k, top_p, min_p)]
     number = [0 if p is not None else v for p, v in zip(per_row, (temperature, top_k, top_p, min_p))]
     check(
@@ -350,8 +351,8 @@ def route(logits: torch.Tensor, bias: torch.Tensor | None, top_k: int, scoring: 
     """``povs_route_v1``: (experts int32, weights float32), both (rows, top_k)."""
     dev = logits.device
     rows, n = logits.shape
-    experts = torch.empty((rows, top_k), dtype=torch.int32, device=dev)
-    weights = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
+    experts = logits.new_empty((rows, top_k), dtype=torch.int32)
+    weights = logits.new_empty((rows, top_k), dtype=torch.float32)
     check(
         load().povs_route_v1(
             logits.data_ptr(), _SCORE_DTYPES[logits.dtype], rows, n, logits.stride(0),
@@ -368,7 +369,7 @@ def route_backward(logits: torch.Tensor, experts: torch.Tensor, grad_weights: to
     """``povs_route_backward_v1``: the gradient of the logits, contiguous."""
     dev = logits.device
     rows, n = logits.shape
-    grad = torch.empty((rows, n), dtype=logits.dtype, device=dev)
+    grad = logits.new_empty((rows, n))
     check(
         load().povs_route_backward_v1(
             logits.data_ptr(), _SCORE_DTYPES[logits.dtype], rows, n, logits.stride(0), experts.shape[1], scoring,
@@ -385,9 +386,9 @@ def plan_rows(experts: torch.Tensor, n_experts: int) -> tuple[torch.Tensor, torc
     lib = load()
     dev = experts.device
     n = experts.numel()
-    slots = torch.empty(experts.shape, dtype=torch.int32, device=dev)
-    sources = torch.empty(n, dtype=torch.int32, device=dev)
-    offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=dev)
+    slots = experts.new_empty(experts.shape, dtype=torch.int32)
+    sources = slots.new_empty(n)
+    offsets = slots.new_empty(n_experts + 1)
     need = lib.povs_plan_rows_workspace_v1(n, n_experts)
     check(need, "povs_plan_rows_workspace_v1")
     work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
@@ -406,7 +407,7 @@ def dispatch_rows(data: torch.Tensor, slots: torch.Tensor, offsets: torch.Tensor
     dev = data.device
     rows, k = slots.shape
     size = data.element_size()
-    out = torch.empty((rows * k, *data.shape[1:]), dtype=data.dtype, device=dev)
+    out = data.new_empty((rows * k, *data.shape[1:]))
     check(
         load().povs_dispatch_rows_v1(
             data.data_ptr(), rows, _row_elements(data) * size, data.stride(0) * size, slots.data_ptr(), k,
@@ -422,7 +423,7 @@ def combine_rows(data: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor 
     """``povs_combine_rows_v1``: weighted sums of each row's slots."""
     dev = data.device
     rows, k = slots.shape
-    out = torch.empty((rows, *data.shape[1:]), dtype=data.dtype, device=dev)
+    out = data.new_empty((rows, *data.shape[1:]))
     check(
         load().povs_combine_rows_v1(
             data.data_ptr(), _SCORE_DTYPES[data.dtype], data.shape[0], _row_elements(data), data.stride(0),
@@ -439,8 +440,8 @@ def combine_backward(grad: torch.Tensor, data: torch.Tensor, slots: torch.Tensor
     """``povs_combine_backward_v1``: the gradients of ``data`` and ``weights`` (None where not needed)."""
     dev = grad.device
     rows, k = slots.shape
-    grad_data = torch.empty(data.shape, dtype=data.dtype, device=dev) if need_data else None
-    grad_weights = torch.empty((rows, k), dtype=torch.float32, device=dev) if need_weights else None
+    grad_data = data.new_empty(data.shape) if need_data else None
+    grad_weights = data.new_empty((rows, k), dtype=torch.float32) if need_weights else None
     check(
         load().povs_combine_backward_v1(
             grad.data_ptr(), data.data_ptr(), _SCORE_DTYPES[data.dtype], data.shape[0], _row_elements(data),

@@ -12,7 +12,6 @@ import math
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native
 
@@ -105,8 +104,8 @@ class _Route(torch.autograd.Function):
         return experts, weights
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, _, grad_weights):
+        _first_order()
         logits, experts = ctx.saved_tensors
         top_k, scoring, _, _, _, renormalize, scale = ctx.spec
         return _native.route_backward(logits, experts, grad_weights.contiguous(), scoring, renormalize, scale), None, None
@@ -150,8 +149,8 @@ class _Dispatch(torch.autograd.Function):
         return _native.dispatch_rows(data, slots, offsets)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
+        _first_order()
         (slots,) = ctx.saved_tensors
         return _native.combine_rows(grad.contiguous(), slots, None), None, None
 
@@ -187,11 +186,18 @@ class _Combine(torch.autograd.Function):
         return _native.combine_rows(data, slots, weights)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
+        _first_order()
         data, weights, slots, offsets = ctx.saved_tensors
         return (*_native.combine_backward(grad.contiguous(), data, slots, weights, offsets, *ctx.needs_input_grad[:2]),
                 None, None)
+
+
+def _first_order() -> None:
+    """The gradients' kernels have no gradients: refuse ``create_graph=True``, under which a backward
+    pass runs with gradients enabled."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("povs gradients are once differentiable: call backward without create_graph=True")
 
 
 def _check_moved(data: torch.Tensor, plan: RowPlan, what: str) -> None:
@@ -199,9 +205,9 @@ def _check_moved(data: torch.Tensor, plan: RowPlan, what: str) -> None:
         raise TypeError(f"{what} takes a CUDA tensor of rows")
     assert data.dim() >= 1, f"data must have at least one dimension, but has {data.dim()}"
     assert data.is_contiguous() or data[:1].is_contiguous(), "rows of data must be contiguous"
-    for name, t in zip(("slots", "offsets"), (plan.slots, plan.offsets)):
-        if not isinstance(t, torch.Tensor) or t.device != data.device or t.dtype != torch.int32:
-            raise TypeError(f"plan.{name} must be an int32 tensor on the device of data ({data.device})")
-        assert t.is_contiguous(), f"plan.{name} must be contiguous"
-    assert plan.slots.dim() == 2 and plan.slots.shape[1] >= 1, f"plan.slots must have shape (rows, top_k), got {tuple(plan.slots.shape)}"
-    assert plan.offsets.dim() == 1 and plan.offsets.numel() >= 2, "plan.offsets must have shape (n_experts + 1,)"
+    slots, offsets = plan.slots, plan.offsets
+    if slots.device != data.device or offsets.device != data.device or slots.dtype != torch.int32 or offsets.dtype != torch.int32:
+        raise TypeError(f"plan.slots and plan.offsets must be int32 tensors on the device of data ({data.device})")
+    assert slots.is_contiguous() and offsets.is_contiguous(), "plan.slots and plan.offsets must be contiguous"
+    assert slots.dim() == 2 and slots.shape[1] >= 1, f"plan.slots must have shape (rows, top_k), got {tuple(slots.shape)}"
+    assert offsets.dim() == 1 and offsets.numel() >= 2, "plan.offsets must have shape (n_experts + 1,)"

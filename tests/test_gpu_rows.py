@@ -664,6 +664,17 @@ def test_calls_on_two_streams_at_once():
             assert all(torch.equal(a, b) for a, b in zip(outs, want[i]))
 
 
+def test_gradients_refuse_a_second_order():
+    plan = povs.plan_rows(_experts(8, 2, 4, seed=1), 4)
+    for make in (lambda t: povs.route(t, 2).weights, lambda t: povs.dispatch_rows(t, plan)):
+        x = torch.randn(8, 6, device=DEV).requires_grad_()
+        with pytest.raises(RuntimeError, match="once differentiable"):
+            torch.autograd.grad(make(x).sum(), x, create_graph=True)
+    y = torch.randn(16, 6, device=DEV).requires_grad_()
+    with pytest.raises(RuntimeError, match="once differentiable"):
+        torch.autograd.grad(povs.combine_rows(y, plan).sum(), y, create_graph=True)
+
+
 def test_same_inputs_same_bits():
     x, u = _scores(20, 100_000, torch.bfloat16, seed=1), _uniforms(20, seed=2)
     logits = _scores(5000, 128, torch.float32, seed=3)
