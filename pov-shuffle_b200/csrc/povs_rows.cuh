@@ -727,45 +727,52 @@ struct DispatchParams {
     int64_t row_stride; // bytes
     int64_t n_slots;
     int32_t top_k;
+    int32_t split_log2; // 2^split_log2 warps per row
 };
 
-// One warp per row and run of 32 * UNROLL pieces: read once, written to each of the row's slots.
+constexpr int MOVE_WARPS = 8; // warps per block of the moving kernels
+
+// A warp reads runs of 32 * UNROLL pieces of a row, all in flight, and writes each run to the row's
+// slots: every row is read once.  Bound by DRAM writes (each row leaves top_k times).
 template <int BYTES, int UNROLL>
-__global__ void __launch_bounds__(256) povs_dispatch_kernel(const __grid_constant__ DispatchParams p)
+__global__ void __launch_bounds__(32 * MOVE_WARPS) povs_dispatch_kernel(const __grid_constant__ DispatchParams p)
 {
     using V = typename Piece<BYTES>::type;
+    constexpr int RUN = 32 * UNROLL;
     const int lane = threadIdx.x & 31;
     const int64_t pieces = p.row_bytes / BYTES;
-    const int64_t runs = (pieces + 32 * UNROLL - 1) / (32 * UNROLL);
-    const int64_t warps = static_cast<int64_t>(gridDim.x) * 8;
-    const int64_t me = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    for (int64_t u = me; u < p.rows * runs; u += warps) {
-        const int64_t row = u / runs, c0 = (u % runs) * 32 * UNROLL + lane;
+    const int64_t warps = static_cast<int64_t>(gridDim.x) * MOVE_WARPS;
+    const int64_t me = static_cast<int64_t>(blockIdx.x) * MOVE_WARPS + (threadIdx.x >> 5);
+    const int64_t step = static_cast<int64_t>(RUN) << p.split_log2;
+    for (int64_t u = me; u < p.rows << p.split_log2; u += warps) {
+        const int64_t row = u >> p.split_log2;
         const V* src = reinterpret_cast<const V*>(p.data + row * p.row_stride);
-        V v[UNROLL];
+        const int32_t* slots = p.slots + row * p.top_k;
+        const int first = lane < p.top_k ? slots[lane] : -1;
+        for (int64_t c = (u & ((1 << p.split_log2) - 1)) * RUN + lane; c - lane < pieces; c += step) {
+            V v[UNROLL];
 #pragma unroll
-        for (int i = 0; i < UNROLL; ++i)
-            if (c0 + 32 * i < pieces) v[i] = src[c0 + 32 * i];
-        for (int j0 = 0; j0 < p.top_k; j0 += 32) {
-            const int k = min(32, p.top_k - j0);
-            const int mine = lane < k ? p.slots[row * p.top_k + j0 + lane] : -1;
-            for (int j = 0; j < k; ++j) {
-                const int slot = __shfl_sync(FULL_WARP, mine, j);
+            for (int i = 0; i < UNROLL; ++i)
+                if (c + 32 * i < pieces) v[i] = __ldg(src + c + 32 * i);
+            for (int j = 0; j < p.top_k; ++j) {
+                const int slot = j < 32 ? __shfl_sync(FULL_WARP, first, j) : slots[j];
                 if (slot < 0 || slot >= p.n_slots) continue;
-                V* dst = reinterpret_cast<V*>(p.out + slot * p.row_bytes);
+                V* dst = reinterpret_cast<V*>(p.out + slot * p.row_bytes) + c;
+                if (c - lane + RUN <= pieces) {
 #pragma unroll
-                for (int i = 0; i < UNROLL; ++i)
-                    if (c0 + 32 * i < pieces) dst[c0 + 32 * i] = v[i];
+                    for (int i = 0; i < UNROLL; ++i) dst[32 * i] = v[i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < UNROLL; ++i)
+                        if (c + 32 * i < pieces) dst[32 * i] = v[i];
+                }
             }
         }
     }
     const int64_t used = max(0, *p.used);
-    for (int64_t u = used * runs + me; u < p.n_slots * runs; u += warps) {
-        V* dst = reinterpret_cast<V*>(p.out + (u / runs) * p.row_bytes);
-        const int64_t c0 = (u % runs) * 32 * UNROLL + lane;
-#pragma unroll
-        for (int i = 0; i < UNROLL; ++i)
-            if (c0 + 32 * i < pieces) dst[c0 + 32 * i] = V{};
+    for (int64_t slot = used + me; slot < p.n_slots; slot += warps) {
+        V* dst = reinterpret_cast<V*>(p.out + slot * p.row_bytes);
+        for (int64_t c = lane; c < pieces; c += 32) dst[c] = V{};
     }
 }
 
@@ -783,6 +790,7 @@ struct CombineParams {
     int64_t data_stride;   // elements
     int64_t n_slots;
     int32_t top_k;
+    int32_t split_log2;    // 2^split_log2 warps per row
     // Backward only.
     const int32_t* used;
     const void* grad;      // rows, contiguous
@@ -794,99 +802,147 @@ template <typename T, int N> struct alignas(N * sizeof(T)) Lanes {
     T v[N];
 };
 
-// One warp per row and run of 32 * N elements; sums in 32 bits, rounded once.
-template <typename T, int N>
-__global__ void __launch_bounds__(256) povs_combine_kernel(const __grid_constant__ CombineParams p)
+// A warp sums runs of 32 * UNROLL pieces of N elements: the pieces of AT_ONCE slots are in flight
+// together, sums are taken in 32 bits in the order of the slots and rounded once.  Bound by DRAM reads.
+template <typename T, int N, int UNROLL>
+__global__ void __launch_bounds__(32 * MOVE_WARPS) povs_combine_kernel(const __grid_constant__ CombineParams p)
 {
     using V = Lanes<T, N>;
+    constexpr int RUN = 32 * UNROLL, AT_ONCE = 4;
     const int lane = threadIdx.x & 31;
     const int64_t pieces = p.width / N;
-    const int64_t runs = (pieces + 31) / 32;
-    const int64_t warps = static_cast<int64_t>(gridDim.x) * 8;
-    for (int64_t u = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); u < p.rows * runs; u += warps) {
-        const int64_t row = u / runs, c = (u % runs) * 32 + lane;
-        float sum[N];
+    const int64_t warps = static_cast<int64_t>(gridDim.x) * MOVE_WARPS;
+    const int64_t step = static_cast<int64_t>(RUN) << p.split_log2;
+    for (int64_t u = static_cast<int64_t>(blockIdx.x) * MOVE_WARPS + (threadIdx.x >> 5); u < p.rows << p.split_log2; u += warps) {
+        const int64_t row = u >> p.split_log2;
+        for (int64_t c = (u & ((1 << p.split_log2) - 1)) * RUN + lane; c - lane < pieces; c += step) {
+            float sum[UNROLL][N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) sum[i] = 0.0f;
-        for (int j0 = 0; j0 < p.top_k; j0 += 32) {
-            const int k = min(32, p.top_k - j0);
-            int mine = -1;
-            float weight = 1.0f;
-            if (lane < k) {
-                mine = p.slots[row * p.top_k + j0 + lane];
-                if (p.weights != nullptr) weight = p.weights[row * p.top_k + j0 + lane];
+            for (int i = 0; i < UNROLL; ++i)
+#pragma unroll
+                for (int e = 0; e < N; ++e) sum[i][e] = 0.0f;
+            for (int j0 = 0; j0 < p.top_k; j0 += 32) {
+                int slot = -1;
+                float weight = 0.0f;
+                if (j0 + lane < p.top_k) {
+                    slot = p.slots[row * p.top_k + j0 + lane];
+                    if (slot >= p.n_slots) slot = -1;
+                    weight = p.weights != nullptr ? p.weights[row * p.top_k + j0 + lane] : 1.0f;
+                }
+                for (int j = 0; j < min(32, p.top_k - j0); j += AT_ONCE) {
+                    V y[AT_ONCE][UNROLL];
+                    int at[AT_ONCE];
+#pragma unroll
+                    for (int a = 0; a < AT_ONCE; ++a) {
+                        at[a] = __shfl_sync(FULL_WARP, slot, j + a); // -1 behind the last
+                        const V* src = reinterpret_cast<const V*>(static_cast<const T*>(p.data) + max(at[a], 0) * p.data_stride) + c;
+#pragma unroll
+                        for (int i = 0; i < UNROLL; ++i)
+                            if (at[a] >= 0 && c + 32 * i < pieces) y[a][i] = src[32 * i];
+                    }
+#pragma unroll
+                    for (int a = 0; a < AT_ONCE; ++a) {
+                        const float w = __shfl_sync(FULL_WARP, weight, j + a);
+                        if (at[a] < 0) continue;
+#pragma unroll
+                        for (int i = 0; i < UNROLL; ++i)
+                            if (c + 32 * i < pieces) {
+#pragma unroll
+                                for (int e = 0; e < N; ++e) sum[i][e] = fmaf(w, to_float(y[a][i].v[e]), sum[i][e]);
+                            }
+                    }
+                }
             }
-#pragma unroll 4
-            for (int j = 0; j < k; ++j) {
-                const int slot = __shfl_sync(FULL_WARP, mine, j);
-                const float w = __shfl_sync(FULL_WARP, weight, j);
-                if (slot < 0 || slot >= p.n_slots || c >= pieces) continue;
-                const V y = reinterpret_cast<const V*>(static_cast<const T*>(p.data) + slot * p.data_stride)[c];
+            V* dst = reinterpret_cast<V*>(static_cast<T*>(p.out) + row * p.width) + c;
 #pragma unroll
-                for (int i = 0; i < N; ++i) sum[i] = fmaf(w, to_float(y.v[i]), sum[i]);
-            }
-        }
-        if (c < pieces) {
-            V o;
+            for (int i = 0; i < UNROLL; ++i)
+                if (c + 32 * i < pieces) {
+                    V o;
 #pragma unroll
-            for (int i = 0; i < N; ++i) o.v[i] = from_float<T>(sum[i]);
-            reinterpret_cast<V*>(static_cast<T*>(p.out) + row * p.width)[c] = o;
+                    for (int e = 0; e < N; ++e) o.v[e] = from_float<T>(sum[i][e]);
+                    dst[32 * i] = o;
+                }
         }
     }
 }
 
-constexpr int COMBINE_BACKWARD_THREADS = 128;
-
-// One block per row and slot column j: grad_data[slot] = w grad[row], grad_weights = <data[slot], grad[row]>.
-// Behind the rows' blocks come blocks that zero the unused slots of grad_data.
+// 2^split_log2 warps of a block share a row: for AT_ONCE slots at a time, grad_data[slot] = w grad[row] and
+// grad_weights = <data[slot], grad[row]> from one reading of each.  Afterwards the slots that no entry
+// uses are zeroed in grad_data.
 template <typename T, int N>
-__global__ void __launch_bounds__(COMBINE_BACKWARD_THREADS)
-    povs_combine_backward_kernel(const __grid_constant__ CombineParams p)
+__global__ void __launch_bounds__(32 * MOVE_WARPS) povs_combine_backward_kernel(const __grid_constant__ CombineParams p)
 {
     using V = Lanes<T, N>;
-    __shared__ float part[COMBINE_BACKWARD_THREADS / 32];
+    constexpr int AT_ONCE = 4;
+    __shared__ float part[MOVE_WARPS][AT_ONCE];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int split = 1 << p.split_log2, mine = warp & (split - 1), rows_at_once = MOVE_WARPS >> p.split_log2;
     const int64_t pieces = p.width / N;
-    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * rows_at_once; base < p.rows;
+         base += static_cast<int64_t>(gridDim.x) * rows_at_once) {
+        const int64_t row = base + (warp >> p.split_log2);
+        const bool there = row < p.rows;
         const V* g = reinterpret_cast<const V*>(static_cast<const T*>(p.grad) + row * p.width);
-        for (int j = 0; j < p.top_k; ++j) {
-            const int slot = p.slots[row * p.top_k + j];
-            const bool there = slot >= 0 && slot < p.n_slots;
-            const float w = p.weights != nullptr ? p.weights[row * p.top_k + j] : 1.0f;
-            float dot = 0.0f;
+        for (int j0 = 0; j0 < p.top_k; j0 += AT_ONCE) {
+            int at[AT_ONCE];
+            float w[AT_ONCE], dot[AT_ONCE];
+#pragma unroll
+            for (int a = 0; a < AT_ONCE; ++a) {
+                const bool is = there && j0 + a < p.top_k;
+                at[a] = is ? p.slots[row * p.top_k + j0 + a] : -1;
+                if (at[a] >= p.n_slots) at[a] = -1;
+                w[a] = is && p.weights != nullptr ? p.weights[row * p.top_k + j0 + a] : 1.0f;
+                dot[a] = 0.0f;
+            }
             if (there)
-                for (int64_t c = threadIdx.x; c < pieces; c += COMBINE_BACKWARD_THREADS) {
-                    const V a = g[c];
+                for (int64_t c = mine * 32 + lane; c < pieces; c += 32 * split) {
+                    const V d = g[c];
+                    V y[AT_ONCE];
                     if (p.grad_weights != nullptr) {
-                        const V y = reinterpret_cast<const V*>(static_cast<const T*>(p.data) + slot * p.data_stride)[c];
 #pragma unroll
-                        for (int i = 0; i < N; ++i) dot = fmaf(to_float(a.v[i]), to_float(y.v[i]), dot);
+                        for (int a = 0; a < AT_ONCE; ++a)
+                            if (at[a] >= 0) y[a] = reinterpret_cast<const V*>(static_cast<const T*>(p.data) + at[a] * p.data_stride)[c];
                     }
-                    if (p.grad_data != nullptr) {
-                        V o;
 #pragma unroll
-                        for (int i = 0; i < N; ++i) o.v[i] = from_float<T>(w * to_float(a.v[i]));
-                        reinterpret_cast<V*>(static_cast<T*>(p.grad_data) + slot * p.width)[c] = o;
+                    for (int a = 0; a < AT_ONCE; ++a) {
+                        if (at[a] < 0) continue;
+                        if (p.grad_weights != nullptr) {
+#pragma unroll
+                            for (int e = 0; e < N; ++e) dot[a] = fmaf(to_float(d.v[e]), to_float(y[a].v[e]), dot[a]);
+                        }
+                        if (p.grad_data != nullptr) {
+                            V o;
+#pragma unroll
+                            for (int e = 0; e < N; ++e) o.v[e] = from_float<T>(w[a] * to_float(d.v[e]));
+                            reinterpret_cast<V*>(static_cast<T*>(p.grad_data) + at[a] * p.width)[c] = o;
+                        }
                     }
                 }
             if (p.grad_weights != nullptr) {
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(FULL_WARP, dot, o);
-                if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = dot;
-                __syncthreads();
-                if (threadIdx.x == 0) {
-                    float total = 0.0f;
-                    for (int i = 0; i < COMBINE_BACKWARD_THREADS / 32; ++i) total += part[i];
-                    p.grad_weights[row * p.top_k + j] = total;
+                for (int a = 0; a < AT_ONCE; ++a) {
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) dot[a] += __shfl_xor_sync(FULL_WARP, dot[a], o);
+                    if (lane == 0) part[warp][a] = dot[a];
                 }
-                __syncthreads();
+                if (split > 1) __syncthreads();
+                else __syncwarp();
+                if (mine == 0 && lane < AT_ONCE && there && j0 + lane < p.top_k) {
+                    float total = 0.0f;
+                    for (int i = 0; i < split; ++i) total += part[warp + i][lane];
+                    p.grad_weights[row * p.top_k + j0 + lane] = total;
+                }
+                if (split > 1) __syncthreads();
+                else __syncwarp();
             }
         }
     }
     if (p.grad_data == nullptr) return;
     const int64_t used = max(0, *p.used);
-    for (int64_t s = used + blockIdx.x; s < p.n_slots; s += gridDim.x) {
-        V* dst = reinterpret_cast<V*>(static_cast<T*>(p.grad_data) + s * p.width);
-        for (int64_t c = threadIdx.x; c < pieces; c += COMBINE_BACKWARD_THREADS) dst[c] = V{};
+    for (int64_t slot = used + static_cast<int64_t>(blockIdx.x) * MOVE_WARPS + warp; slot < p.n_slots;
+         slot += static_cast<int64_t>(gridDim.x) * MOVE_WARPS) {
+        V* dst = reinterpret_cast<V*>(static_cast<T*>(p.grad_data) + slot * p.width);
+        for (int64_t c = lane; c < pieces; c += 32) dst[c] = V{};
     }
 }
 

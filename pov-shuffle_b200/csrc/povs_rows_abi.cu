@@ -130,29 +130,50 @@ int check_rows(int64_t rows, int32_t top_k, int64_t n_slots)
     return POVS_OK;
 }
 
-template <int BYTES> void launch_dispatch(const povs::DispatchParams& p, int sms, cudaStream_t s)
+// Warps per row of the moving kernels, as a power of two: one for each run of the row, as long as all
+// rows together have fewer than 64 per SM.
+int split_of(int64_t rows, int64_t runs, int sms, int most_log2)
 {
-    const int64_t runs = (p.row_bytes / BYTES + 127) / 128;
-    povs::povs_dispatch_kernel<BYTES, 4><<<grid_for(std::max(p.rows, p.n_slots) * runs, 8, sms, 8), 256, 0, s>>>(p);
+    int s = 0;
+    while (s < most_log2 && (int64_t{1} << s) < runs && (rows << s) < 64 * static_cast<int64_t>(sms)) ++s;
+    return s;
 }
 
-template <typename T, int N> void launch_combine(const povs::CombineParams& p, int sms, cudaStream_t s)
+template <int BYTES> void launch_dispatch(povs::DispatchParams& p, int sms, cudaStream_t s)
 {
-    const int64_t runs = (p.width / N + 31) / 32;
-    povs::povs_combine_kernel<T, N><<<grid_for(p.rows * runs, 8, sms, 8), 256, 0, s>>>(p);
+    constexpr int UNROLL = BYTES == 16 ? 4 : BYTES == 8 ? 8 : 16;
+    const int64_t runs = (p.row_bytes / BYTES + 32 * UNROLL - 1) / (32 * UNROLL);
+    p.split_log2 = split_of(p.rows, runs, sms, 10);
+    povs::povs_dispatch_kernel<BYTES, UNROLL>
+        <<<grid_for(std::max(p.rows << p.split_log2, int64_t{1}), povs::MOVE_WARPS, sms, 8), 32 * povs::MOVE_WARPS, 0, s>>>(p);
 }
 
-template <typename T, int N> void launch_combine_backward(const povs::CombineParams& p, int sms, cudaStream_t s)
+template <typename T, int N, int UNROLL> void launch_combine(povs::CombineParams& p, int sms, cudaStream_t s)
 {
+    const int64_t runs = (p.width / N + 32 * UNROLL - 1) / (32 * UNROLL);
+    p.split_log2 = split_of(p.rows, runs, sms, 10);
+    povs::povs_combine_kernel<T, N, UNROLL>
+        <<<grid_for(p.rows << p.split_log2, povs::MOVE_WARPS, sms, 8), 32 * povs::MOVE_WARPS, 0, s>>>(p);
+}
+
+template <typename T, int N> void launch_combine_backward(povs::CombineParams& p, int sms, cudaStream_t s)
+{
+    p.split_log2 = split_of(p.rows, (p.width / N + 31) / 32, sms, 3);
     povs::povs_combine_backward_kernel<T, N>
-        <<<grid_for(std::max(p.rows, p.n_slots), 1, sms, 16), povs::COMBINE_BACKWARD_THREADS, 0, s>>>(p);
+        <<<grid_for(std::max(p.rows << p.split_log2, int64_t{1}), povs::MOVE_WARPS, sms, 8), 32 * povs::MOVE_WARPS, 0, s>>>(p);
 }
 
-// Elements per load: 16 bytes where every row starts on a multiple of 16 bytes, else one element.
-template <typename T, typename F16, typename F1> void by_alignment(int align, F16 wide, F1 narrow)
+// 16 bytes per load where every row starts on a multiple of 16 bytes, else one element.
+template <typename T> void launch_combine_by(int align, povs::CombineParams& p, int sms, cudaStream_t s)
 {
-    if (align >= 16) wide();
-    else narrow();
+    if (align >= 16) launch_combine<T, 16 / sizeof(T), 1>(p, sms, s);
+    else launch_combine<T, 1, 4>(p, sms, s);
+}
+
+template <typename T> void launch_combine_backward_by(int align, povs::CombineParams& p, int sms, cudaStream_t s)
+{
+    if (align >= 16) launch_combine_backward<T, 16 / sizeof(T)>(p, sms, s);
+    else launch_combine_backward<T, 1>(p, sms, s);
 }
 
 int check_combine(const povs::CombineParams& p, int32_t dtype)
@@ -466,13 +487,9 @@ extern "C" int povs_combine_rows_v1(const void* data, int32_t dtype, int64_t n_s
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const uint64_t size = element_bytes(dtype);
     const int align = common_alignment({address(data), address(out), width * size, data_stride * size});
-    if (dtype == POVS_FLOAT32)
-        by_alignment<float>(align, [&] { launch_combine<float, 4>(p, sms, s); }, [&] { launch_combine<float, 1>(p, sms, s); });
-    else if (dtype == POVS_BFLOAT16)
-        by_alignment<__nv_bfloat16>(align, [&] { launch_combine<__nv_bfloat16, 8>(p, sms, s); },
-                                    [&] { launch_combine<__nv_bfloat16, 1>(p, sms, s); });
-    else
-        by_alignment<__half>(align, [&] { launch_combine<__half, 8>(p, sms, s); }, [&] { launch_combine<__half, 1>(p, sms, s); });
+    if (dtype == POVS_FLOAT32) launch_combine_by<float>(align, p, sms, s);
+    else if (dtype == POVS_BFLOAT16) launch_combine_by<__nv_bfloat16>(align, p, sms, s);
+    else launch_combine_by<__half>(align, p, sms, s);
     return launched("combine kernel");
 }
 
@@ -509,14 +526,8 @@ extern "C" int povs_combine_backward_v1(const void* grad, const void* data, int3
     const uint64_t size = element_bytes(dtype);
     const int align = common_alignment({address(grad), address(grad_weights != nullptr ? data : nullptr), address(p.grad_data),
                                         width * size, grad_weights != nullptr ? data_stride * size : 0});
-    if (dtype == POVS_FLOAT32)
-        by_alignment<float>(align, [&] { launch_combine_backward<float, 4>(p, sms, s); },
-                            [&] { launch_combine_backward<float, 1>(p, sms, s); });
-    else if (dtype == POVS_BFLOAT16)
-        by_alignment<__nv_bfloat16>(align, [&] { launch_combine_backward<__nv_bfloat16, 8>(p, sms, s); },
-                                    [&] { launch_combine_backward<__nv_bfloat16, 1>(p, sms, s); });
-    else
-        by_alignment<__half>(align, [&] { launch_combine_backward<__half, 8>(p, sms, s); },
-                             [&] { launch_combine_backward<__half, 1>(p, sms, s); });
+    if (dtype == POVS_FLOAT32) launch_combine_backward_by<float>(align, p, sms, s);
+    else if (dtype == POVS_BFLOAT16) launch_combine_backward_by<__nv_bfloat16>(align, p, sms, s);
+    else launch_combine_backward_by<__half>(align, p, sms, s);
     return launched("combine backward kernel");
 }
