@@ -7,6 +7,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <cstring>
 
 namespace povs {
 
@@ -760,11 +761,11 @@ __global__ void __launch_bounds__(32 * MOVE_WARPS) povs_dispatch_kernel(const __
                 V* dst = reinterpret_cast<V*>(p.out + slot * p.row_bytes) + c;
                 if (c - lane + RUN <= pieces) {
 #pragma unroll
-                    for (int i = 0; i < UNROLL; ++i) dst[32 * i] = v[i];
+                    for (int i = 0; i < UNROLL; ++i) __stcs(dst + 32 * i, v[i]);
                 } else {
 #pragma unroll
                     for (int i = 0; i < UNROLL; ++i)
-                        if (c + 32 * i < pieces) dst[32 * i] = v[i];
+                        if (c + 32 * i < pieces) __stcs(dst + 32 * i, v[i]);
                 }
             }
         }
@@ -798,17 +799,35 @@ struct CombineParams {
     float* grad_weights;   // rows * top_k, or NULL
 };
 
-template <typename T, int N> struct alignas(N * sizeof(T)) Lanes {
-    T v[N];
+// N elements as one load, and as floats.
+template <typename T, int N> struct Pack {
+    using Raw = typename Piece<N * sizeof(T)>::type;
+    static __device__ __forceinline__ void unpack(const Raw& raw, float (&v)[N])
+    {
+        T e[N];
+        memcpy(e, &raw, sizeof(raw));
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = to_float(e[i]);
+    }
+    static __device__ __forceinline__ Raw pack(const float (&v)[N])
+    {
+        T e[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) e[i] = from_float<T>(v[i]);
+        Raw raw;
+        memcpy(&raw, e, sizeof(raw));
+        return raw;
+    }
 };
 
 // A warp sums runs of 32 * UNROLL pieces of N elements: the pieces of AT_ONCE slots are in flight
 // together, sums are taken in 32 bits in the order of the slots and rounded once.  Bound by DRAM reads.
-template <typename T, int N, int UNROLL>
+template <typename T, int N, int UNROLL, int AT_ONCE>
 __global__ void __launch_bounds__(32 * MOVE_WARPS) povs_combine_kernel(const __grid_constant__ CombineParams p)
 {
-    using V = Lanes<T, N>;
-    constexpr int RUN = 32 * UNROLL, AT_ONCE = 4;
+    using P = Pack<T, N>;
+    using Raw = typename P::Raw;
+    constexpr int RUN = 32 * UNROLL;
     const int lane = threadIdx.x & 31;
     const int64_t pieces = p.width / N;
     const int64_t warps = static_cast<int64_t>(gridDim.x) * MOVE_WARPS;
@@ -816,6 +835,7 @@ __global__ void __launch_bounds__(32 * MOVE_WARPS) povs_combine_kernel(const __g
     for (int64_t u = static_cast<int64_t>(blockIdx.x) * MOVE_WARPS + (threadIdx.x >> 5); u < p.rows << p.split_log2; u += warps) {
         const int64_t row = u >> p.split_log2;
         for (int64_t c = (u & ((1 << p.split_log2) - 1)) * RUN + lane; c - lane < pieces; c += step) {
+            const bool full = c - lane + RUN <= pieces;
             float sum[UNROLL][N];
 #pragma unroll
             for (int i = 0; i < UNROLL; ++i)
@@ -823,45 +843,53 @@ __global__ void __launch_bounds__(32 * MOVE_WARPS) povs_combine_kernel(const __g
                 for (int e = 0; e < N; ++e) sum[i][e] = 0.0f;
             for (int j0 = 0; j0 < p.top_k; j0 += 32) {
                 int slot = -1;
-                float weight = 0.0f;
+                float weight = 0.0f; // of what is left out
                 if (j0 + lane < p.top_k) {
                     slot = p.slots[row * p.top_k + j0 + lane];
-                    if (slot >= p.n_slots) slot = -1;
-                    weight = p.weights != nullptr ? p.weights[row * p.top_k + j0 + lane] : 1.0f;
+                    if (slot < 0 || slot >= p.n_slots) slot = -1;
+                    else weight = p.weights != nullptr ? p.weights[row * p.top_k + j0 + lane] : 1.0f;
                 }
+                const unsigned valid = __ballot_sync(FULL_WARP, slot >= 0);
                 for (int j = 0; j < min(32, p.top_k - j0); j += AT_ONCE) {
-                    V y[AT_ONCE][UNROLL];
-                    int at[AT_ONCE];
+                    Raw y[AT_ONCE][UNROLL];
+                    constexpr unsigned EVERY = (1u << AT_ONCE) - 1;
+                    const Raw* src[AT_ONCE];
 #pragma unroll
                     for (int a = 0; a < AT_ONCE; ++a) {
-                        at[a] = __shfl_sync(FULL_WARP, slot, j + a); // -1 behind the last
-                        const V* src = reinterpret_cast<const V*>(static_cast<const T*>(p.data) + max(at[a], 0) * p.data_stride) + c;
+                        const int at = __shfl_sync(FULL_WARP, slot, j + a); // -1 behind the last
+                        src[a] = reinterpret_cast<const Raw*>(static_cast<const T*>(p.data) + max(at, 0) * p.data_stride) + c;
+                    }
+                    if (full && (valid >> j & EVERY) == EVERY) {
 #pragma unroll
-                        for (int i = 0; i < UNROLL; ++i)
-                            if (at[a] >= 0 && c + 32 * i < pieces) y[a][i] = src[32 * i];
+                        for (int a = 0; a < AT_ONCE; ++a)
+#pragma unroll
+                            for (int i = 0; i < UNROLL; ++i) y[a][i] = __ldg(src[a] + 32 * i);
+                    } else {
+#pragma unroll
+                        for (int a = 0; a < AT_ONCE; ++a)
+#pragma unroll
+                            for (int i = 0; i < UNROLL; ++i) {
+                                y[a][i] = Raw{};
+                                if ((valid >> (j + a) & 1) && c + 32 * i < pieces) y[a][i] = __ldg(src[a] + 32 * i);
+                            }
                     }
 #pragma unroll
                     for (int a = 0; a < AT_ONCE; ++a) {
                         const float w = __shfl_sync(FULL_WARP, weight, j + a);
-                        if (at[a] < 0) continue;
 #pragma unroll
-                        for (int i = 0; i < UNROLL; ++i)
-                            if (c + 32 * i < pieces) {
+                        for (int i = 0; i < UNROLL; ++i) {
+                            float v[N];
+                            P::unpack(y[a][i], v);
 #pragma unroll
-                                for (int e = 0; e < N; ++e) sum[i][e] = fmaf(w, to_float(y[a][i].v[e]), sum[i][e]);
-                            }
+                            for (int e = 0; e < N; ++e) sum[i][e] = fmaf(w, v[e], sum[i][e]);
+                        }
                     }
                 }
             }
-            V* dst = reinterpret_cast<V*>(static_cast<T*>(p.out) + row * p.width) + c;
+            Raw* dst = reinterpret_cast<Raw*>(static_cast<T*>(p.out) + row * p.width) + c;
 #pragma unroll
             for (int i = 0; i < UNROLL; ++i)
-                if (c + 32 * i < pieces) {
-                    V o;
-#pragma unroll
-                    for (int e = 0; e < N; ++e) o.v[e] = from_float<T>(sum[i][e]);
-                    dst[32 * i] = o;
-                }
+                if (c + 32 * i < pieces) dst[32 * i] = P::pack(sum[i]);
         }
     }
 }
@@ -869,11 +897,11 @@ __global__ void __launch_bounds__(32 * MOVE_WARPS) povs_combine_kernel(const __g
 // 2^split_log2 warps of a block share a row: for AT_ONCE slots at a time, grad_data[slot] = w grad[row] and
 // grad_weights = <data[slot], grad[row]> from one reading of each.  Afterwards the slots that no entry
 // uses are zeroed in grad_data.
-template <typename T, int N>
+template <typename T, int N, int UNROLL, int AT_ONCE>
 __global__ void __launch_bounds__(32 * MOVE_WARPS) povs_combine_backward_kernel(const __grid_constant__ CombineParams p)
 {
-    using V = Lanes<T, N>;
-    constexpr int AT_ONCE = 4;
+    using P = Pack<T, N>;
+    using Raw = typename P::Raw;
     __shared__ float part[MOVE_WARPS][AT_ONCE];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int split = 1 << p.split_log2, mine = warp & (split - 1), rows_at_once = MOVE_WARPS >> p.split_log2;
@@ -882,7 +910,7 @@ __global__ void __launch_bounds__(32 * MOVE_WARPS) povs_combine_backward_kernel(
          base += static_cast<int64_t>(gridDim.x) * rows_at_once) {
         const int64_t row = base + (warp >> p.split_log2);
         const bool there = row < p.rows;
-        const V* g = reinterpret_cast<const V*>(static_cast<const T*>(p.grad) + row * p.width);
+        const Raw* g = reinterpret_cast<const Raw*>(static_cast<const T*>(p.grad) + row * p.width);
         for (int j0 = 0; j0 < p.top_k; j0 += AT_ONCE) {
             int at[AT_ONCE];
             float w[AT_ONCE], dot[AT_ONCE];
@@ -895,26 +923,42 @@ __global__ void __launch_bounds__(32 * MOVE_WARPS) povs_combine_backward_kernel(
                 dot[a] = 0.0f;
             }
             if (there)
-                for (int64_t c = mine * 32 + lane; c < pieces; c += 32 * split) {
-                    const V d = g[c];
-                    V y[AT_ONCE];
+                for (int64_t c = mine * 32 * UNROLL + lane; c < pieces; c += 32 * UNROLL * split) {
+                    Raw up[UNROLL], y[AT_ONCE][UNROLL];
+#pragma unroll
+                    for (int i = 0; i < UNROLL; ++i) {
+                        up[i] = Raw{};
+                        if (c + 32 * i < pieces) up[i] = __ldg(g + c + 32 * i);
+                    }
                     if (p.grad_weights != nullptr) {
 #pragma unroll
-                        for (int a = 0; a < AT_ONCE; ++a)
-                            if (at[a] >= 0) y[a] = reinterpret_cast<const V*>(static_cast<const T*>(p.data) + at[a] * p.data_stride)[c];
+                        for (int a = 0; a < AT_ONCE; ++a) {
+                            const Raw* src = reinterpret_cast<const Raw*>(static_cast<const T*>(p.data) + max(at[a], 0) * p.data_stride);
+#pragma unroll
+                            for (int i = 0; i < UNROLL; ++i) {
+                                y[a][i] = Raw{};
+                                if (at[a] >= 0 && c + 32 * i < pieces) y[a][i] = __ldg(src + c + 32 * i);
+                            }
+                        }
                     }
 #pragma unroll
-                    for (int a = 0; a < AT_ONCE; ++a) {
-                        if (at[a] < 0) continue;
-                        if (p.grad_weights != nullptr) {
+                    for (int i = 0; i < UNROLL; ++i) {
+                        float d[N], v[N];
+                        P::unpack(up[i], d);
 #pragma unroll
-                            for (int e = 0; e < N; ++e) dot[a] = fmaf(to_float(d.v[e]), to_float(y[a].v[e]), dot[a]);
-                        }
-                        if (p.grad_data != nullptr) {
-                            V o;
+                        for (int a = 0; a < AT_ONCE; ++a) {
+                            if (p.grad_weights != nullptr) {
+                                P::unpack(y[a][i], v);
+                                if (at[a] >= 0) {
 #pragma unroll
-                            for (int e = 0; e < N; ++e) o.v[e] = from_float<T>(w[a] * to_float(d.v[e]));
-                            reinterpret_cast<V*>(static_cast<T*>(p.grad_data) + at[a] * p.width)[c] = o;
+                                    for (int e = 0; e < N; ++e) dot[a] = fmaf(d[e], v[e], dot[a]);
+                                }
+                            }
+                            if (p.grad_data != nullptr && at[a] >= 0 && c + 32 * i < pieces) {
+#pragma unroll
+                                for (int e = 0; e < N; ++e) v[e] = w[a] * d[e];
+                                __stcs(reinterpret_cast<Raw*>(static_cast<T*>(p.grad_data) + at[a] * p.width) + c + 32 * i, P::pack(v));
+                            }
                         }
                     }
                 }
@@ -941,8 +985,8 @@ __global__ void __launch_bounds__(32 * MOVE_WARPS) povs_combine_backward_kernel(
     const int64_t used = max(0, *p.used);
     for (int64_t slot = used + static_cast<int64_t>(blockIdx.x) * MOVE_WARPS + warp; slot < p.n_slots;
          slot += static_cast<int64_t>(gridDim.x) * MOVE_WARPS) {
-        V* dst = reinterpret_cast<V*>(static_cast<T*>(p.grad_data) + slot * p.width);
-        for (int64_t c = lane; c < pieces; c += 32) dst[c] = V{};
+        Raw* dst = reinterpret_cast<Raw*>(static_cast<T*>(p.grad_data) + slot * p.width);
+        for (int64_t c = lane; c < pieces; c += 32) dst[c] = Raw{};
     }
 }
 
