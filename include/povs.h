@@ -393,7 +393,8 @@ int povs_sample_v1(const void* logits, int32_t dtype, int64_t rows, int64_t widt
  * choice scores (POVS_GROUP_TOP2) or its highest (POVS_GROUP_MAX), and only the top_groups best
  * groups' experts can be chosen.  experts[r * top_k + j]: the j-th highest c, equal ones by the lowest
  * index; weights[r * top_k + j] = scale * s of it, divided by the sum of the row's chosen s with
- * renormalize.  Choices are made on scores computed in 64 bits.  An expert whose logit or choice
+ * renormalize.  Without bias and groups the order is the logits'; else choices are made on scores
+ * computed in 64 bits.  An expert whose logit or choice
  * score is -infinity is never chosen; a row with fewer than top_k others ends with experts -1 of
  * weight 0.  A NaN score ranks below every number.  No reference counterpart.
  */

@@ -92,13 +92,14 @@ template <typename T, int EPL> __device__ __noinline__ void route_row_exactly(co
     const T* x = static_cast<const T*>(p.logits) + row * p.row_stride;
     const int n = p.n_experts;
 
-    double s[EPL];
+    double s[EPL], logit[EPL];
     bool open[EPL]; // can be chosen
 #pragma unroll
     for (int m = 0; m < EPL; ++m) {
         const int e = lane + 32 * m;
         s[m] = e < n ? static_cast<double>(to_float(x[e])) : -INFINITY;
         open[m] = e < n && s[m] != -INFINITY;
+        logit[m] = s[m];
     }
     if (p.sigmoid) {
 #pragma unroll
@@ -123,11 +124,16 @@ template <typename T, int EPL> __device__ __noinline__ void route_row_exactly(co
         for (int m = 0; m < EPL; ++m) s[m] = open[m] ? s[m] * inv : 0.0;
     }
 
+    // Scores rise with the logits: where nothing is added and no groups are summed the logits' own order
+    // stands, also where scores of 64 bits fall together (a NaN score still comes last).
+    const bool by_logit = p.bias == nullptr && p.top_groups == p.n_groups;
     uint64_t key[EPL];
 #pragma unroll
     for (int m = 0; m < EPL; ++m) {
         const int e = lane + 32 * m;
-        const double c = p.bias != nullptr && e < n ? s[m] + static_cast<double>(p.bias[e]) : s[m];
+        const double c = by_logit && s[m] == s[m]         ? logit[m]
+                         : p.bias != nullptr && e < n ? s[m] + static_cast<double>(p.bias[e])
+                                                      : s[m];
         key[m] = open[m] && c != -INFINITY ? order_key(c) : 0;
     }
     if (p.top_groups < p.n_groups) {
@@ -505,6 +511,245 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, EPL <= 8 ? 8 : EPL <= 16 ? 5
             p.experts[row * p.top_k + lane] = e;
             p.weights[row * p.top_k + lane] = w;
         }
+    }
+}
+
+// The same choice with a lane per row, for batches large enough to fill the GPU with lanes.  A warp brings
+// 32 rows into shared memory (rows an odd number of 16-byte pieces apart, so that the lanes' loads hit
+// different banks); each lane walks its row, no lane waiting for another.  Eight scores at a time become
+// whole numbers as above, are sorted by a network of 19 exchanges and merged into the lane's eight best
+// (a bitonic half-cleaner and its 12 exchanges); the highest number that fell out is kept, as the ninth.
+// Where the order is the logits' and those have 16 bits, the numbers hold them whole and nothing is left open.
+constexpr int ROUTE_LIST = 8;
+
+__device__ __forceinline__ void exchange(uint32_t& a, uint32_t& b)
+{
+    const uint32_t high = max(a, b);
+    b = min(a, b);
+    a = high;
+}
+
+__device__ __forceinline__ void sort_down(uint32_t (&v)[ROUTE_LIST])
+{
+    exchange(v[0], v[1]); exchange(v[2], v[3]); exchange(v[4], v[5]); exchange(v[6], v[7]);
+    exchange(v[0], v[2]); exchange(v[1], v[3]); exchange(v[4], v[6]); exchange(v[5], v[7]);
+    exchange(v[1], v[2]); exchange(v[5], v[6]);
+    exchange(v[0], v[4]); exchange(v[1], v[5]); exchange(v[2], v[6]); exchange(v[3], v[7]);
+    exchange(v[2], v[4]); exchange(v[3], v[5]);
+    exchange(v[1], v[2]); exchange(v[3], v[4]); exchange(v[5], v[6]);
+}
+
+// Bytes between two rows of the tile: an odd number of 16-byte pieces.
+__host__ __device__ __forceinline__ int route_pitch(int row_bytes) { return (row_bytes / 16 | 1) * 16; }
+
+template <typename T, bool SIGMOID, bool BY_LOGIT, bool GROUPED>
+__global__ void __launch_bounds__(32) povs_route_lanes_kernel(const __grid_constant__ RouteParams p)
+{
+    constexpr bool WHOLE = BY_LOGIT && sizeof(T) == 2; // numbers that hold the logits whole
+    constexpr int V = 16 / sizeof(T), INDEX_BITS = WHOLE ? 16 : 9;
+    constexpr uint32_t INDEX_MASK = (1u << INDEX_BITS) - 1;
+    constexpr float TOP = 3.9998f, LOWEST = 2.0f + 1.0f / (1 << 22);
+    extern __shared__ __align__(16) uint8_t memory[];
+    const int lane = threadIdx.x, n = p.n_experts, row_bytes = n * static_cast<int>(sizeof(T)), pitch = route_pitch(row_bytes);
+    const int64_t first_row = static_cast<int64_t>(blockIdx.x) * 32, row = first_row + lane;
+    const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.rows - first_row));
+    float* bias = reinterpret_cast<float*>(memory + 32 * pitch); // n, for !BY_LOGIT
+    float* group_score = bias + n;                               // n_groups * 32, twice, for GROUPED
+    float* group_first = group_score + p.n_groups * 32;
+
+    {
+        const int pieces = row_bytes / 16;
+        const uint8_t* from = static_cast<const uint8_t*>(p.logits) + first_row * p.row_stride * static_cast<int64_t>(sizeof(T));
+        for (int r = 0, c = lane; r < rows;) {
+            if (c < pieces) {
+                const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(memory + r * pitch + c * 16));
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to),
+                             "l"(from + r * p.row_stride * static_cast<int64_t>(sizeof(T)) + c * 16) : "memory");
+                c += 32;
+            }
+            while (c >= pieces && r < rows) {
+                c -= pieces;
+                ++r;
+            }
+        }
+        if (!BY_LOGIT)
+            for (int e = lane; e < n; e += 32) bias[e] = p.bias != nullptr ? p.bias[e] : 0.0f;
+        asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
+        __syncwarp();
+    }
+    const bool active = lane < rows;
+    const uint8_t* mine = memory + (active ? lane : 0) * pitch;
+    auto read = [&](int e, float (&x)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; i += V) {
+            T v[V];
+            const uint4 raw = *reinterpret_cast<const uint4*>(mine + (e + i) * sizeof(T));
+            memcpy(v, &raw, sizeof(raw));
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[i + j] = to_float(v[j]);
+        }
+    };
+    float x[8];
+    float top = -INFINITY, inv = 0.0f;
+    if (!SIGMOID || (BY_LOGIT && !WHOLE)) {
+        for (int e = 0; e < n; e += 8) {
+            read(e, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, x[j]);
+        }
+    }
+    bool open = false;
+    if (!SIGMOID) {
+        float sums[2] = {0.0f, 0.0f};
+        for (int e = 0; e < n; e += 8) {
+            read(e, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sums[j & 1] += exp2_fast((x[j] - top) * LOG2E);
+        }
+        inv = reciprocal_fast(sums[0] + sums[1]);
+        open = !(inv <= 1.0001f && top > -INFINITY); // NaN, infinities, nothing to choose
+    }
+    // A choice score; masked experts stay at -infinity.
+    auto choice = [&](float logit, float b) {
+        const float s = SIGMOID ? reciprocal_fast(1.0f + exp2_fast(logit * -LOG2E)) : exp2_fast((logit - top) * LOG2E) * inv;
+        return logit == -INFINITY ? -INFINITY : s + b;
+    };
+    // The error that scores of 32 bits may have: as in the kernel above, with sums over n / 2 scores.
+    const float sum_error = SIGMOID ? 0.0f : 3e-8f * static_cast<float>(n);
+    float highest = BY_LOGIT ? top * 0.125f : -INFINITY;
+    unsigned kept = 0xffffffffu;
+    const int size = n / p.n_groups;
+    if (!BY_LOGIT) {
+        int g = 0, left = size;
+        float first = -INFINITY, second = -INFINITY;
+        for (int e = 0; e < n; e += 8) {
+            read(e, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float c = choice(x[j], bias[e + j]);
+                if (GROUPED) {
+                    second = fmaxf(second, fminf(first, c));
+                    open |= c != c;
+                }
+                first = fmaxf(first, c);
+            }
+            if (GROUPED && (left -= 8) == 0) {
+                group_score[g * 32 + lane] = p.group_max ? first : first + second;
+                group_first[g * 32 + lane] = first;
+                first = second = -INFINITY;
+                left = size;
+                ++g;
+            }
+        }
+        highest = first;
+    }
+    if (GROUPED) {
+        kept = 0;
+        highest = -INFINITY;
+        for (int g = 0; g < p.n_groups; ++g) {
+            const float score = group_score[g * 32 + lane];
+            const float slack = 8e-6f + 2.0f * sum_error + fabsf(score) * 1e-6f;
+            int sure = 0, maybe = 0; // groups surely before this one, and groups that may be
+            for (int other = 0; other < p.n_groups; ++other) {
+                const float v = group_score[other * 32 + lane];
+                sure += v > score + slack;
+                maybe += other != g && !(v < score - slack);
+            }
+            if (maybe < p.top_groups) {
+                kept |= 1u << g;
+                highest = fmaxf(highest, group_first[g * 32 + lane]);
+            } else {
+                open |= sure < p.top_groups;
+            }
+        }
+    }
+    const float room = BY_LOGIT ? 3.0f : 18.0f + fabsf(highest) + 8.4e6f * sum_error; // in steps of 2^-22
+    if (!WHOLE) open |= !(fabsf(highest) < 1000.0f);
+
+    uint32_t best[ROUTE_LIST], fell = 0;
+#pragma unroll
+    for (int i = 0; i < ROUTE_LIST; ++i) best[i] = 0;
+    const float offset = TOP - highest;
+    int g = 0, left = size;
+    for (int e = 0; e < n; e += 8) {
+        uint32_t key[ROUTE_LIST];
+        if constexpr (WHOLE) {
+            const uint4 raw = *reinterpret_cast<const uint4*>(mine + e * sizeof(T));
+            const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t high = j & 1 ? words[j / 2] & 0xffff0000u : words[j / 2] << 16; // the logit's bits, in order:
+                const uint32_t ordered = high == 0x80000000u ? 0x80000000u : high ^ (static_cast<uint32_t>(static_cast<int32_t>(high) >> 31) | 0x80000000u);
+                key[j] = (ordered & 0xffff0000u) | (INDEX_MASK - (e + j));
+            }
+        } else {
+            read(e, x);
+            const bool in = !GROUPED || (kept >> g & 1);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float c = BY_LOGIT ? x[j] * 0.125f : in ? choice(x[j], bias[e + j]) : -INFINITY;
+                key[j] = __float_as_uint(fmaxf(c + offset, LOWEST)) << 9 | (INDEX_MASK - (e + j));
+            }
+            if (GROUPED && (left -= 8) == 0) {
+                left = size;
+                ++g;
+            }
+        }
+        sort_down(key);
+#pragma unroll
+        for (int i = 0; i < ROUTE_LIST; ++i) {
+            fell = max(fell, min(best[i], key[ROUTE_LIST - 1 - i]));
+            best[i] = max(best[i], key[ROUTE_LIST - 1 - i]);
+        }
+#pragma unroll
+        for (int step = ROUTE_LIST / 2; step > 0; step /= 2)
+#pragma unroll
+            for (int i = 0; i < ROUTE_LIST; ++i)
+                if ((i & step) == 0) exchange(best[i], best[i | step]);
+    }
+
+    // The chosen, told apart from one another and from the rest.
+    float score[ROUTE_LIST], total = 0.0f, logit_before = 0.0f, bias_before = 0.0f;
+    int chosen[ROUTE_LIST];
+#pragma unroll
+    for (int j = 0; j < ROUTE_LIST; ++j) {
+        score[j] = 0.0f;
+        chosen[j] = 0;
+        const uint32_t next = j + 1 < ROUTE_LIST ? best[j + 1] : fell;
+        if (j < p.top_k) {
+            const int e = min(static_cast<int>(INDEX_MASK - (best[j] & INDEX_MASK)), n - 1);
+            const float logit = to_float(reinterpret_cast<const T*>(mine)[e]), b = BY_LOGIT ? 0.0f : bias[e];
+            if (WHOLE) {
+                open |= !(logit > -INFINITY);
+            } else {
+                open |= best[j] >> 9 <= 1;
+                if (j > 0)
+                    open |= static_cast<float>((best[j - 1] >> 9) - (best[j] >> 9)) <= room && !(logit == logit_before && b == bias_before);
+                if (j == p.top_k - 1 && p.top_k < n) open |= static_cast<float>((best[j] >> 9) - (next >> 9)) <= room;
+            }
+            logit_before = logit;
+            bias_before = b;
+            score[j] = SIGMOID ? reciprocal_fast(1.0f + exp2_fast(logit * -LOG2E)) : exp2_fast((logit - top) * LOG2E) * inv;
+            total += score[j];
+            chosen[j] = e;
+        }
+    }
+    float factor = p.scale;
+    if (p.renormalize) factor = total == 0.0f ? 0.0f : factor / total;
+    if (active && !open) {
+        int32_t* experts = p.experts + row * p.top_k;
+        float* weights = p.weights + row * p.top_k;
+#pragma unroll
+        for (int j = 0; j < ROUTE_LIST; ++j)
+            if (j < p.top_k) {
+                experts[j] = chosen[j];
+                weights[j] = score[j] * factor;
+            }
+    }
+    for (unsigned rest = __ballot_sync(FULL_WARP, active && open); rest != 0; rest &= rest - 1) {
+        const int64_t r = first_row + __ffs(rest) - 1;
+        if (n <= 256) route_row_exactly<T, 8>(p, r);
+        else route_row_exactly<T, 16>(p, r);
     }
 }
 

@@ -54,7 +54,8 @@ def route(
     """Choose ``top_k`` experts for every row.
 
     With ``s`` the softmax or sigmoid of a row's logits, the experts with the highest ``s + bias`` are
-    chosen (equal ones by the lowest index; scores are compared in 64 bits), and their weights are
+    chosen (equal ones by the lowest index; scores are compared in 64 bits, or by their logits where
+    there is neither bias nor group), and their weights are
     ``scale * s``, divided by the sum of the chosen ``s`` with ``renormalize``.  The weights have a gradient
     with respect to ``logits``; ``bias`` moves the choice alone and gets none.  An expert whose logit or
     biased score is -inf is never chosen; a row with fewer than ``top_k`` others ends with experts -1

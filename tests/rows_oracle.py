@@ -56,6 +56,8 @@ def route_row(x, top_k, scoring="softmax", bias=None, n_groups=1, top_groups=Non
     s = scores(x, scoring)
     with np.errstate(all="ignore"):
         c = s if bias is None else s + bias.astype(np.float64)
+        if bias is None and (top_groups is None or top_groups == n_groups):
+            c = np.where(np.isnan(s), np.nan, x)  # scores rise with the logits
         c = np.where(x == -np.inf, -np.inf, c)
         if top_groups is not None and top_groups < n_groups:
             parts = c.reshape(n_groups, -1)

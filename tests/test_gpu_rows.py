@@ -279,6 +279,47 @@ def test_route_rows_with_masks_and_ties(dtype, kw):
     np.testing.assert_allclose(_host(got.weights), weights, rtol=64 * U32 + 32 * U32, atol=1e-37)
 
 
+@pytest.mark.parametrize("n,k,kw", [
+    (8, 8, {}),
+    (64, 6, {"renormalize": True}),
+    (128, 8, {"scoring": "sigmoid"}),
+    (128, 1, {"bias": True}),
+    (256, 8, {"scoring": "sigmoid", "bias": True, "n_groups": 8, "top_groups": 4, "renormalize": True, "scale": 2.5}),
+    (160, 6, {"n_groups": 4, "top_groups": 2, "group_score": "max"}),
+    (512, 4, {"scoring": "sigmoid", "n_groups": 32, "top_groups": 9}),
+    (384, 7, {"bias": True, "renormalize": True}),
+], ids=str)
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_route_of_many_rows(dtype, n, k, kw):
+    """Batches that fill the GPU with one lane per row, the last warp in part, among them masked, tied and
+    close rows."""
+    rows = 9503
+    kw = _route_settings(n, kw, seed=n)
+    x = _scores(rows, n, dtype, seed=n, sharp=1.5)
+    inf = float("inf")
+    x[5] = -inf
+    x[40, 1:] = -inf
+    x[41, ::2] = -inf
+    x[77] = 0.5
+    x[78] = x[78, 0]
+    x[78, n - 1] += 1
+    x[100] = torch.finfo(dtype).min
+    x[101, 3] = inf
+    x[102, 2] = float("nan")
+    x[9502, 0] = torch.finfo(dtype).max
+    x[200:260] = (x[200:260] * 4).round() / 4
+    x[300] = torch.linspace(-1e-6, 1e-6, n, device=DEV).to(dtype)
+    got = povs.route(x, k, **kw)
+    host = {**kw, "bias": _host(kw["bias"])} if "bias" in kw else kw
+    experts, weights = oracle.route(_host(x), k, **host)
+    np.testing.assert_array_equal(_host(got.experts), experts)
+    plain = np.ones(rows, bool)
+    plain[[5, 40, 41, 100, 101, 102, 9502]] = False
+    # As _weight_bound, with a softmax's sum over all n scores by one lane.
+    bound = _weight_bound(_host(x)[plain], n) + n * U32
+    np.testing.assert_allclose(_host(got.weights), weights, rtol=bound, atol=1e-37)
+
+
 def test_route_masked_by_bias_and_row_strides():
     n, k = 40, 4
     x = _scores(33, 2 * n, torch.float16, seed=1)[:, 3:3 + n]
