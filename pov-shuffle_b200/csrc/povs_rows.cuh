@@ -514,12 +514,14 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, EPL <= 8 ? 8 : EPL <= 16 ? 5
     }
 }
 
-// The same choice with a lane per row, for batches large enough to fill the GPU with lanes.  A warp brings
-// 32 rows into shared memory (rows an odd number of 16-byte pieces apart, so that the lanes' loads hit
-// different banks); each lane walks its row, no lane waiting for another.  Eight scores at a time become
-// whole numbers as above, are sorted by a network of 19 exchanges and merged into the lane's eight best
-// (a bitonic half-cleaner and its 12 exchanges); the highest number that fell out is kept, as the ninth.
-// Where the order is the logits' and those have 16 bits, the numbers hold them whole and nothing is left open.
+// The same choice with L lanes per row, for batches large enough to fill the GPU with lanes.  A warp brings
+// 32 / L rows into shared memory (rows an odd number of 16-byte pieces apart, so that the lanes' loads hit
+// different banks); each lane walks its share of a row, no lane waiting for another.  Eight scores at a
+// time become whole numbers as above, are sorted by a network of 19 exchanges and merged into the lane's
+// eight best (a bitonic half-cleaner and its 12 exchanges), and so are the L lanes' lists at the end; the
+// highest number that fell out is kept, as the ninth.  L is what keeps a warp's rows below 9 KB, and so about
+// 24 warps on an SM.  Where the order is the logits' and those have 16 bits, the numbers hold them whole and
+// nothing is left open.
 constexpr int ROUTE_LIST = 8;
 
 __device__ __forceinline__ void exchange(uint32_t& a, uint32_t& b)
@@ -539,10 +541,25 @@ __device__ __forceinline__ void sort_down(uint32_t (&v)[ROUTE_LIST])
     exchange(v[1], v[2]); exchange(v[3], v[4]); exchange(v[5], v[6]);
 }
 
+// The eight highest of two falling lists, and the highest number that falls out.
+__device__ __forceinline__ void merge_down(uint32_t (&best)[ROUTE_LIST], const uint32_t (&other)[ROUTE_LIST], uint32_t& fell)
+{
+#pragma unroll
+    for (int i = 0; i < ROUTE_LIST; ++i) {
+        fell = max(fell, min(best[i], other[ROUTE_LIST - 1 - i]));
+        best[i] = max(best[i], other[ROUTE_LIST - 1 - i]);
+    }
+#pragma unroll
+    for (int step = ROUTE_LIST / 2; step > 0; step /= 2)
+#pragma unroll
+        for (int i = 0; i < ROUTE_LIST; ++i)
+            if ((i & step) == 0) exchange(best[i], best[i | step]);
+}
+
 // Bytes between two rows of the tile: an odd number of 16-byte pieces.
 __host__ __device__ __forceinline__ int route_pitch(int row_bytes) { return (row_bytes / 16 | 1) * 16; }
 
-template <typename T, bool SIGMOID, bool BY_LOGIT, bool GROUPED>
+template <typename T, int L, bool SIGMOID, bool BY_LOGIT, bool GROUPED>
 __global__ void __launch_bounds__(32) povs_route_lanes_kernel(const __grid_constant__ RouteParams p)
 {
     constexpr bool WHOLE = BY_LOGIT && sizeof(T) == 2; // numbers that hold the logits whole
@@ -551,11 +568,22 @@ __global__ void __launch_bounds__(32) povs_route_lanes_kernel(const __grid_const
     constexpr float TOP = 3.9998f, LOWEST = 2.0f + 1.0f / (1 << 22);
     extern __shared__ __align__(16) uint8_t memory[];
     const int lane = threadIdx.x, n = p.n_experts, row_bytes = n * static_cast<int>(sizeof(T)), pitch = route_pitch(row_bytes);
-    const int64_t first_row = static_cast<int64_t>(blockIdx.x) * 32, row = first_row + lane;
-    const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.rows - first_row));
-    float* bias = reinterpret_cast<float*>(memory + 32 * pitch); // n, for !BY_LOGIT
-    float* group_score = bias + n;                               // n_groups * 32, twice, for GROUPED
-    float* group_first = group_score + p.n_groups * 32;
+    constexpr int ROWS = 32 / L;
+    const int place = lane % ROWS, share = lane / ROWS; // this lane's row and which part of it
+    const int64_t first_row = static_cast<int64_t>(blockIdx.x) * ROWS, row = first_row + place;
+    const int rows = static_cast<int>(min(static_cast<int64_t>(ROWS), p.rows - first_row));
+    const int from_e = n / L * share, to_e = from_e + n / L;
+    float* bias = reinterpret_cast<float*>(memory + ROWS * pitch); // n, for !BY_LOGIT
+    float* group_score = bias + n;                                 // n_groups * ROWS, twice, for GROUPED
+    float* group_first = group_score + p.n_groups * ROWS;
+    auto over_shares = [&](float v, bool highest) {
+#pragma unroll
+        for (int o = ROWS; o < 32; o *= 2) {
+            const float other = __shfl_xor_sync(FULL_WARP, v, o);
+            v = highest ? fmaxf(v, other) : v + other;
+        }
+        return v;
+    };
 
     {
         const int pieces = row_bytes / 16;
@@ -577,8 +605,8 @@ __global__ void __launch_bounds__(32) povs_route_lanes_kernel(const __grid_const
         asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
         __syncwarp();
     }
-    const bool active = lane < rows;
-    const uint8_t* mine = memory + (active ? lane : 0) * pitch;
+    const bool active = place < rows;
+    const uint8_t* mine = memory + (active ? place : 0) * pitch;
     auto read = [&](int e, float (&x)[8]) {
 #pragma unroll
         for (int i = 0; i < 8; i += V) {
@@ -592,21 +620,22 @@ __global__ void __launch_bounds__(32) povs_route_lanes_kernel(const __grid_const
     float x[8];
     float top = -INFINITY, inv = 0.0f;
     if (!SIGMOID || (BY_LOGIT && !WHOLE)) {
-        for (int e = 0; e < n; e += 8) {
+        for (int e = from_e; e < to_e; e += 8) {
             read(e, x);
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = fmaxf(top, x[j]);
         }
+        top = over_shares(top, true);
     }
     bool open = false;
     if (!SIGMOID) {
         float sums[2] = {0.0f, 0.0f};
-        for (int e = 0; e < n; e += 8) {
+        for (int e = from_e; e < to_e; e += 8) {
             read(e, x);
 #pragma unroll
             for (int j = 0; j < 8; ++j) sums[j & 1] += exp2_fast((x[j] - top) * LOG2E);
         }
-        inv = reciprocal_fast(sums[0] + sums[1]);
+        inv = reciprocal_fast(over_shares(sums[0] + sums[1], false));
         open = !(inv <= 1.0001f && top > -INFINITY); // NaN, infinities, nothing to choose
     }
     // A choice score; masked experts stay at -infinity.
@@ -620,9 +649,9 @@ __global__ void __launch_bounds__(32) povs_route_lanes_kernel(const __grid_const
     unsigned kept = 0xffffffffu;
     const int size = n / p.n_groups;
     if (!BY_LOGIT) {
-        int g = 0, left = size;
+        int g = p.n_groups / L * share, left = size;
         float first = -INFINITY, second = -INFINITY;
-        for (int e = 0; e < n; e += 8) {
+        for (int e = from_e; e < to_e; e += 8) {
             read(e, x);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -634,34 +663,36 @@ __global__ void __launch_bounds__(32) povs_route_lanes_kernel(const __grid_const
                 first = fmaxf(first, c);
             }
             if (GROUPED && (left -= 8) == 0) {
-                group_score[g * 32 + lane] = p.group_max ? first : first + second;
-                group_first[g * 32 + lane] = first;
+                group_score[g * ROWS + place] = p.group_max ? first : first + second;
+                group_first[g * ROWS + place] = first;
                 first = second = -INFINITY;
                 left = size;
                 ++g;
             }
         }
-        highest = first;
+        if (!GROUPED) highest = over_shares(first, true);
     }
     if (GROUPED) {
         kept = 0;
         highest = -INFINITY;
-        for (int g = 0; g < p.n_groups; ++g) {
-            const float score = group_score[g * 32 + lane];
+        __syncwarp();
+        for (int g = p.n_groups / L * share; g < p.n_groups / L * (share + 1); ++g) {
+            const float score = group_score[g * ROWS + place];
             const float slack = 8e-6f + 2.0f * sum_error + fabsf(score) * 1e-6f;
             int sure = 0, maybe = 0; // groups surely before this one, and groups that may be
             for (int other = 0; other < p.n_groups; ++other) {
-                const float v = group_score[other * 32 + lane];
+                const float v = group_score[other * ROWS + place];
                 sure += v > score + slack;
                 maybe += other != g && !(v < score - slack);
             }
             if (maybe < p.top_groups) {
                 kept |= 1u << g;
-                highest = fmaxf(highest, group_first[g * 32 + lane]);
+                highest = fmaxf(highest, group_first[g * ROWS + place]);
             } else {
                 open |= sure < p.top_groups;
             }
         }
+        highest = over_shares(highest, true);
     }
     const float room = BY_LOGIT ? 3.0f : 18.0f + fabsf(highest) + 8.4e6f * sum_error; // in steps of 2^-22
     if (!WHOLE) open |= !(fabsf(highest) < 1000.0f);
@@ -670,8 +701,8 @@ __global__ void __launch_bounds__(32) povs_route_lanes_kernel(const __grid_const
 #pragma unroll
     for (int i = 0; i < ROUTE_LIST; ++i) best[i] = 0;
     const float offset = TOP - highest;
-    int g = 0, left = size;
-    for (int e = 0; e < n; e += 8) {
+    int g = p.n_groups / L * share, left = size;
+    for (int e = from_e; e < to_e; e += 8) {
         uint32_t key[ROUTE_LIST];
         if constexpr (WHOLE) {
             const uint4 raw = *reinterpret_cast<const uint4*>(mine + e * sizeof(T));
@@ -696,16 +727,16 @@ __global__ void __launch_bounds__(32) povs_route_lanes_kernel(const __grid_const
             }
         }
         sort_down(key);
+        merge_down(best, key, fell);
+    }
 #pragma unroll
-        for (int i = 0; i < ROUTE_LIST; ++i) {
-            fell = max(fell, min(best[i], key[ROUTE_LIST - 1 - i]));
-            best[i] = max(best[i], key[ROUTE_LIST - 1 - i]);
-        }
+    for (int o = ROWS; o < 32; o *= 2) {
+        uint32_t other[ROUTE_LIST];
 #pragma unroll
-        for (int step = ROUTE_LIST / 2; step > 0; step /= 2)
-#pragma unroll
-            for (int i = 0; i < ROUTE_LIST; ++i)
-                if ((i & step) == 0) exchange(best[i], best[i | step]);
+        for (int i = 0; i < ROUTE_LIST; ++i) other[i] = __shfl_xor_sync(FULL_WARP, best[i], o);
+        fell = max(fell, __shfl_xor_sync(FULL_WARP, fell, o));
+        merge_down(best, other, fell);
+        open |= __shfl_xor_sync(FULL_WARP, static_cast<int>(open), o) != 0;
     }
 
     // The chosen, told apart from one another and from the rest.
@@ -736,7 +767,7 @@ __global__ void __launch_bounds__(32) povs_route_lanes_kernel(const __grid_const
     }
     float factor = p.scale;
     if (p.renormalize) factor = total == 0.0f ? 0.0f : factor / total;
-    if (active && !open) {
+    if (active && !open && share == 0) {
         int32_t* experts = p.experts + row * p.top_k;
         float* weights = p.weights + row * p.top_k;
 #pragma unroll
@@ -746,7 +777,7 @@ __global__ void __launch_bounds__(32) povs_route_lanes_kernel(const __grid_const
                 weights[j] = score[j] * factor;
             }
     }
-    for (unsigned rest = __ballot_sync(FULL_WARP, active && open); rest != 0; rest &= rest - 1) {
+    for (unsigned rest = __ballot_sync(FULL_WARP, active && open && share == 0); rest != 0; rest &= rest - 1) {
         const int64_t r = first_row + __ffs(rest) - 1;
         if (n <= 256) route_row_exactly<T, 8>(p, r);
         else route_row_exactly<T, 16>(p, r);

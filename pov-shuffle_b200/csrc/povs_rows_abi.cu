@@ -110,21 +110,41 @@ template <typename T, int EPL> void launch_route_of(const povs::RouteParams& p, 
     else povs::povs_route_kernel<T, EPL, false><<<grid, 32 * povs::ROUTE_WARPS, 0, s>>>(p);
 }
 
-template <typename T, bool SIGMOID, bool BY_LOGIT, bool GROUPED> int launch_route_lanes(const povs::RouteParams& p, cudaStream_t s)
+template <typename T, int L, bool SIGMOID, bool BY_LOGIT, bool GROUPED> int launch_route_lanes(const povs::RouteParams& p, cudaStream_t s)
 {
-    const int floats = (BY_LOGIT ? 0 : p.n_experts) + (GROUPED ? 2 * 32 * p.n_groups : 0);
-    const int smem = 32 * povs::route_pitch(p.n_experts * static_cast<int>(sizeof(T))) + 4 * floats;
-    auto* kernel = povs::povs_route_lanes_kernel<T, SIGMOID, BY_LOGIT, GROUPED>;
+    constexpr int ROWS = 32 / L;
+    const int floats = (BY_LOGIT ? 0 : p.n_experts) + (GROUPED ? 2 * ROWS * p.n_groups : 0);
+    const int smem = ROWS * povs::route_pitch(p.n_experts * static_cast<int>(sizeof(T))) + 4 * floats;
+    auto* kernel = povs::povs_route_lanes_kernel<T, L, SIGMOID, BY_LOGIT, GROUPED>;
     if (smem > 48 * 1024) POVS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    kernel<<<static_cast<unsigned>((p.rows + 31) / 32), 32, smem, s>>>(p);
+    kernel<<<static_cast<unsigned>((p.rows + ROWS - 1) / ROWS), 32, smem, s>>>(p);
     return POVS_OK;
 }
 
-// A lane per row where rows fill the GPU with lanes, eight choices or fewer are asked, and rows and
-// groups come in whole pieces; else a warp per row.
+template <typename T, int L> int launch_route_lanes_of(const povs::RouteParams& p, cudaStream_t s)
+{
+    const bool grouped = p.top_groups < p.n_groups, by_logit = p.bias == nullptr && !grouped;
+    if (by_logit) return p.sigmoid ? launch_route_lanes<T, L, true, true, false>(p, s) : launch_route_lanes<T, L, false, true, false>(p, s);
+    if (grouped) return p.sigmoid ? launch_route_lanes<T, L, true, false, true>(p, s) : launch_route_lanes<T, L, false, false, true>(p, s);
+    return p.sigmoid ? launch_route_lanes<T, L, true, false, false>(p, s) : launch_route_lanes<T, L, false, false, false>(p, s);
+}
+
+// Lanes per row: as many (1, 2, 4 or 8) as bring a warp's rows below 9 KB, in whole pieces of experts and groups.
+int route_lanes(const povs::RouteParams& p, int element)
+{
+    int lanes = 1;
+    while (lanes < 8 && 32 / lanes * p.n_experts * element > 9 * 1024 && p.n_experts / (2 * lanes) % 8 == 0 &&
+           p.n_experts % (2 * lanes) == 0 && (p.top_groups == p.n_groups || p.n_groups % (2 * lanes) == 0))
+        lanes *= 2;
+    return lanes;
+}
+
+// Lanes where rows fill the GPU with them, eight choices or fewer are asked, and rows and groups come in
+// whole pieces; else a warp per row.  B200, float32, top 8: 65536 x 256 with groups 63 us against 94 by warps,
+// 16384 x 256 13 against 20, but 8192 x 256 20 against 14 and 16384 x 512 58 against 36.
 bool route_by_lanes(const povs::RouteParams& p, int element, int sms)
 {
-    return p.rows >= 64 * static_cast<int64_t>(sms) && p.top_k <= povs::ROUTE_LIST && p.n_experts <= 512 && p.n_experts % 8 == 0 &&
+    return p.rows >= 64 * static_cast<int64_t>(sms) && p.top_k <= povs::ROUTE_LIST && p.n_experts <= 256 && p.n_experts % 8 == 0 &&
            (p.top_groups == p.n_groups || p.n_experts / p.n_groups % 8 == 0) && p.n_experts * element % 16 == 0 &&
            p.row_stride * element % 16 == 0 && address(p.logits) % 16 == 0;
 }
@@ -132,10 +152,12 @@ bool route_by_lanes(const povs::RouteParams& p, int element, int sms)
 template <typename T> int launch_route(const povs::RouteParams& p, int sms, cudaStream_t s)
 {
     if (route_by_lanes(p, sizeof(T), sms)) {
-        const bool grouped = p.top_groups < p.n_groups, by_logit = p.bias == nullptr && !grouped;
-        if (by_logit) return p.sigmoid ? launch_route_lanes<T, true, true, false>(p, s) : launch_route_lanes<T, false, true, false>(p, s);
-        if (grouped) return p.sigmoid ? launch_route_lanes<T, true, false, true>(p, s) : launch_route_lanes<T, false, false, true>(p, s);
-        return p.sigmoid ? launch_route_lanes<T, true, false, false>(p, s) : launch_route_lanes<T, false, false, false>(p, s);
+        switch (route_lanes(p, sizeof(T))) {
+        case 8: return launch_route_lanes_of<T, 8>(p, s);
+        case 4: return launch_route_lanes_of<T, 4>(p, s);
+        case 2: return launch_route_lanes_of<T, 2>(p, s);
+        default: return launch_route_lanes_of<T, 1>(p, s);
+        }
     }
     const int epl = (p.n_experts + 31) / 32;
     if (epl <= 1) launch_route_of<T, 1>(p, sms, s);
