@@ -248,10 +248,12 @@ int check_combine(const povs::CombineParams& p, int32_t dtype)
     return POVS_OK;
 }
 
-// Blocks per row: as many as the GPU holds at once for these rows (four per SM), of 2048 ids or more.
-int sample_cluster(int64_t rows, int64_t width, int sms)
+// Blocks per row: as many as the GPU holds at once for these rows (four per SM), of 2048 ids or more;
+// two where a nucleus may be wide, which is read again (512 rows of 131072, top-p 0.9: 288 us against 384,
+// but 90 against 75 for top-k 50).
+int sample_cluster(int64_t rows, int64_t width, bool nucleus, int sms)
 {
-    int c = 1;
+    int c = nucleus && rows < (1 << 29) && width >= 8192 ? 2 : 1;
     while (2 * c <= povs::SAMPLE_MAX_CLUSTER && rows * 2 * c <= 4 * static_cast<int64_t>(sms) && width / (2 * c) >= 2048) c *= 2;
     return c;
 }
@@ -326,7 +328,7 @@ extern "C" int povs_sample_v1(const void* logits, int32_t dtype, int64_t rows, i
     p.poly[2] = ln2 * ln2 * ln2 / 6 + 1.25 * h2 * fifth;
     p.poly[3] = ln2 * ln2 * ln2 * ln2 / 24;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    p.cluster = sample_cluster(rows, width, sms);
+    p.cluster = sample_cluster(rows, width, top_ps != nullptr || (top_p < 1.0 && top_ks == nullptr && top_k == 0), sms);
     cudaError_t e;
     if (dtype == POVS_FLOAT32) e = launch_sample<float>(p, s);
     else if (dtype == POVS_BFLOAT16) e = launch_sample<__nv_bfloat16>(p, s);

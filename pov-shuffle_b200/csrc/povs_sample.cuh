@@ -848,9 +848,20 @@ template <typename T> struct SampleRow {
             __syncthreads();
             return false;
         }
-        const float place = static_cast<float>(found) + static_cast<float>(static_cast<double>(sh.left) / static_cast<double>(sh.bins[found]));
-        const float half = fminf(1.0f, 700.0f / static_cast<float>(sh.counts[found]));
-        const float from = place - half, to = place + half;
+        // The window [from, to) in bins: the border's bin with its neighbours, as far as the list holds them;
+        // of a bin too full for it, the part around the border's place.
+        constexpr unsigned int ROOM = SAMPLE_LIST - 200;
+        const int bin = static_cast<int>(found);
+        const unsigned int here = sh.counts[bin], above = bin > 0 ? sh.counts[bin - 1] : 0, under = bin + 1 < SAMPLE_BINS ? sh.counts[bin + 1] : 0;
+        const float place = static_cast<float>(static_cast<double>(sh.left) / static_cast<double>(sh.bins[bin]));
+        float from = static_cast<float>(bin), to = from + 1.0f;
+        if (here > ROOM) {
+            from += place - 700.0f / static_cast<float>(here);
+            to = from + 1400.0f / static_cast<float>(here);
+        } else {
+            if (here + above <= ROOM && (place < 0.5f || here + above + under <= ROOM)) from -= 1.0f;
+            if (here + under <= ROOM && (place >= 0.5f || here + above + under <= ROOM)) to += 1.0f;
+        }
         if (t == 0) sh.listed = 0;
         __syncthreads();
         for (int q = warp * warp_parts; q < (warp + 1) * warp_parts; ++q) {
@@ -864,7 +875,7 @@ template <typename T> struct SampleRow {
                     if (y < from) {
                         any = true;
                     } else {
-                        if (y <= to && v[j] > -INFINITY) {
+                        if (y < to && v[j] > -INFINITY) {
                             const unsigned int at = atomicAdd(&sh.listed, 1u);
                             if (at < SAMPLE_LIST) sh.list[at] = (static_cast<Entry>(score_key(v[j])) << 32) | ~(id + j);
                         }
