@@ -194,11 +194,13 @@ struct SampleShared {
     unsigned long long cut_ties;
     // This block's own.
     unsigned long long part[SAMPLE_WARPS];
+    unsigned long long part_high[SAMPLE_WARPS];
+    unsigned int listed_of[SAMPLE_MAX_CLUSTER];
     double part_mass[SAMPLE_WARPS];
     double listed_mass;
+    uint32_t most[SAMPLE_THREADS];
     unsigned int probe_counts[16];
     uint32_t probe_low;
-    uint32_t lowest;
     int few;
     int few_at[32];
     unsigned long long found;
@@ -316,7 +318,7 @@ template <typename T> struct SampleRow {
     }
 
     // --- The probe: scores spread evenly over the row.  Its rank that corresponds to the ids wanted,
-    // with four standard deviations to spare where top_k must be met, gives the list's threshold (its
+    // with about three standard deviations to spare where top_k must be met, gives the list's threshold (its
     // upper 16 bits, found bit by bit).  Every block of the row finds the same one.
     __device__ __forceinline__ void probe()
     {
@@ -344,19 +346,39 @@ template <typename T> struct SampleRow {
             if (top_k > 0) {
                 want = static_cast<double>(top_k) * share;
                 if (want > room) listing = false;
-                want = fmin(want + 4.0 * sqrt(want) + 6.0, room);
+                want = fmin(want + 2.6 * sqrt(want) + 3.6, room);
             }
             const unsigned int rank_wanted = static_cast<unsigned int>(fmax(want, 1.0));
-            uint32_t found = 0;
-            for (int bit = 31; bit >= 16; --bit) {
-                const uint32_t candidate = found | (1u << bit);
-                unsigned int c = 0;
+            // Few wanted: that rank among the threads' highest is a little lower, and each warp finds it alone.
+            const bool few = rank_wanted <= SAMPLE_THREADS / 4;
+            uint32_t most = 0;
 #pragma unroll
-                for (int m = 0; m < PER; ++m) c += k[m] >= candidate;
-                c = __reduce_add_sync(FULL_WARP, c);
-                if (lane == 0) atomicAdd(&sh.probe_counts[bit - 16], c);
-                __syncthreads();
-                if (sh.probe_counts[bit - 16] >= rank_wanted) found = candidate;
+            for (int m = 0; m < PER; ++m) most = max(most, k[m]);
+            sh.most[t] = most;
+            __syncthreads();
+            uint32_t found = 0;
+            if (few) {
+                uint32_t of_lane[SAMPLE_WARPS];
+#pragma unroll
+                for (int m = 0; m < SAMPLE_WARPS; ++m) of_lane[m] = sh.most[m * 32 + lane];
+                for (int bit = 31; bit >= 16; --bit) {
+                    const uint32_t candidate = found | (1u << bit);
+                    unsigned int c = 0;
+#pragma unroll
+                    for (int m = 0; m < SAMPLE_WARPS; ++m) c += of_lane[m] >= candidate;
+                    if (__reduce_add_sync(FULL_WARP, c) >= rank_wanted) found = candidate;
+                }
+            } else {
+                for (int bit = 31; bit >= 16; --bit) {
+                    const uint32_t candidate = found | (1u << bit);
+                    unsigned int c = 0;
+#pragma unroll
+                    for (int m = 0; m < PER; ++m) c += k[m] >= candidate;
+                    c = __reduce_add_sync(FULL_WARP, c);
+                    if (lane == 0) atomicAdd(&sh.probe_counts[bit - 16], c);
+                    __syncthreads();
+                    if (sh.probe_counts[bit - 16] >= rank_wanted) found = candidate;
+                }
             }
             threshold = max(found, LOWEST_KEY);
         }
@@ -491,102 +513,174 @@ template <typename T> struct SampleRow {
         }
         __syncthreads();
     }
-    // From the highest entry down, the one at which the running sum of `amount` reaches `want`, digit by
-    // digit; 0 where the whole sum stays below.  BY_ID looks at the lower half (~id) alone: ids in
-    // ascending order.
-    template <bool BY_ID, typename Amount> __device__ __forceinline__ Entry select(int n, Whole want, Amount amount)
+    // Lowest and highest of a block's numbers (nothing to give: ~0 and 0).
+    __device__ __forceinline__ void block_range(Entry& low, Entry& high)
     {
-        Entry prefix = 0;
-        for (int shift = BY_ID ? 24 : 56; shift >= 0; shift -= 8) {
-            if (shift < 32 && shift >= id_bits) { // ~id has ones there
-                prefix = (prefix << 8) | 255;
-                continue;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            low = min(low, __shfl_xor_sync(FULL_WARP, low, o));
+            high = max(high, __shfl_xor_sync(FULL_WARP, high, o));
+        }
+        __syncthreads();
+        if (lane == 0) {
+            sh.part[warp] = low;
+            sh.part_high[warp] = high;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < SAMPLE_WARPS; ++w) {
+            low = min(low, sh.part[w]);
+            high = max(high, sh.part_high[w]);
+        }
+    }
+    // Of the list's first n entries, in descending order, the one at which the running sum of `amount` reaches
+    // `want`; 0 where the whole sum stays below.  BY_ID orders by the lower half (~id) alone: ids ascend.
+    // A round sums into bins between the highest and the lowest entry, by score or, where those are
+    // equal, by id, and goes on with the entries of the bin that holds the border, until a warp can hold
+    // them.  Evenly spread entries end in one round, those of 16-bit scores, many equal, in two.
+    template <bool BY_ID, typename Amount> __device__ __forceinline__ Entry border_of(int n, Whole want, Amount amount)
+    {
+        auto order = [&](int i) { return BY_ID ? sh.list[i] & 0xffffffffull : sh.list[i]; };
+        Entry low = ~0ull, high = 0; // the entries still in question
+        for (int i = t; i < n; i += SAMPLE_THREADS)
+            if (amount(i) != 0) {
+                low = min(low, order(i));
+                high = max(high, order(i));
             }
-            sh.bins[t] = 0;
+        block_range(low, high);
+        if (low > high) return 0;
+        for (;;) {
+            for (int b = t; b < SAMPLE_BINS; b += SAMPLE_THREADS) sh.bins[b] = 0;
+            if (t == 0) sh.few = 0;
             __syncthreads();
+            const uint32_t id_high = static_cast<uint32_t>(high), id_range = id_high - static_cast<uint32_t>(low);
+            const bool by_id = (low >> 32) == (high >> 32);
+            const double score_high = score_of(high), spread = score_high - score_of(low);
+            const double per_score = spread > 0.0 ? SAMPLE_BINS / spread : 0.0, per_id = SAMPLE_BINS / (id_range + 1.0);
+            auto bin_of = [&](Entry c) {
+                const double b = by_id ? (id_high - static_cast<uint32_t>(c)) * per_id : (score_high - score_of(c)) * per_score;
+                return b < SAMPLE_BINS - 1 ? static_cast<int>(b) : SAMPLE_BINS - 1;
+            };
             for (int i = t; i < n; i += SAMPLE_THREADS) {
-                const Entry c = BY_ID ? sh.list[i] & 0xffffffffull : sh.list[i];
-                if (shift < 56 && (c >> (shift + 8)) != prefix) continue;
+                const Entry c = order(i);
+                if (c < low || c > high) continue;
                 const Whole a = amount(i);
-                if (a != 0) atomicAdd(&sh.bins[255 - ((c >> shift) & 255)], a);
+                if (a != 0) atomicAdd(&sh.bins[bin_of(c)], a);
             }
             __syncthreads();
-            crossing<256>(want);
+            crossing<SAMPLE_BINS>(want);
             const Whole found = sh.found;
             want = sh.left;
-            __syncthreads();
-            if (found == ~0ull) return 0;
-            prefix = (prefix << 8) | (255 - found);
-        }
-        return prefix;
-    }
-    // The same by bins of a number that does not fall along the order (bin_of: an entry's bin): one
-    // round of sums, then the few entries of the bin that holds the border.  Where those are more than
-    // a warp has lanes, digit by digit.
-    template <bool BY_ID, typename BinOf, typename Amount>
-    __device__ __forceinline__ Entry border_of(int n, Whole want, BinOf bin_of, Amount amount)
-    {
-        for (int b = t; b < SAMPLE_BINS; b += SAMPLE_THREADS) sh.bins[b] = 0;
-        if (t == 0) sh.few = 0;
-        __syncthreads();
-        for (int i = t; i < n; i += SAMPLE_THREADS) {
-            const Whole a = amount(i);
-            if (a != 0) atomicAdd(&sh.bins[bin_of(sh.list[i])], a);
-        }
-        __syncthreads();
-        crossing<SAMPLE_BINS>(want);
-        const Whole found = sh.found, left = sh.left;
-        if (found == ~0ull) {
-            __syncthreads();
-            return 0;
-        }
-        const int bin = static_cast<int>(found);
-        for (int i = t; i < n; i += SAMPLE_THREADS)
-            if (bin_of(sh.list[i]) == bin && amount(i) != 0) {
+            if (found == ~0ull) {
+                __syncthreads();
+                return 0;
+            }
+            const int bin = static_cast<int>(found);
+            Entry next_low = ~0ull, next_high = 0;
+            for (int i = t; i < n; i += SAMPLE_THREADS) {
+                const Entry c = order(i);
+                if (c < low || c > high || bin_of(c) != bin || amount(i) == 0) continue;
+                next_low = min(next_low, c);
+                next_high = max(next_high, c);
                 const int at = atomicAdd(&sh.few, 1);
                 if (at < 32) sh.few_at[at] = i;
             }
-        __syncthreads();
-        const int few = sh.few;
-        if (few > 32) return select<BY_ID>(n, left, [&](int i) { return bin_of(sh.list[i]) == bin ? amount(i) : Whole{0}; });
-        if (warp == 0) {
-            const int i = lane < few ? sh.few_at[lane] : 0;
-            const Entry c = BY_ID ? sh.list[i] & 0xffffffffull : sh.list[i];
-            const Whole a = lane < few ? amount(i) : Whole{0};
-            Whole before = 0;
-            for (int o = 0; o < few; ++o) {
-                const Entry other = __shfl_sync(FULL_WARP, c, o);
-                const Whole b = __shfl_sync(FULL_WARP, a, o);
-                if (other > c) before += b;
+            __syncthreads();
+            const int few = sh.few;
+            if (few <= 32) {
+                if (warp == 0) {
+                    const int i = lane < few ? sh.few_at[lane] : 0;
+                    const Entry c = order(i);
+                    const Whole a = lane < few ? amount(i) : Whole{0};
+                    Whole before = 0;
+                    for (int o = 0; o < few; ++o) {
+                        const Entry other = __shfl_sync(FULL_WARP, c, o);
+                        const Whole b = __shfl_sync(FULL_WARP, a, o);
+                        if (other > c) before += b;
+                    }
+                    if (lane < few && before < want && before + a >= want) sh.found = c;
+                }
+                __syncthreads();
+                const Entry entry = sh.found;
+                __syncthreads();
+                return entry;
             }
-            if (lane < few && before < left && before + a >= left) sh.found = c;
+            block_range(next_low, next_high);
+            low = next_low;
+            high = next_high;
         }
-        __syncthreads();
-        const Entry entry = sh.found;
-        __syncthreads();
-        return entry;
     }
     // The other blocks' listed entries, appended to rank 0's, and all their weights.
     __device__ __forceinline__ void gather(int n)
     {
-        unsigned int at = min(sh.listed, static_cast<unsigned int>(SAMPLE_LIST));
-        for (int r = 1; r < blocks; ++r) {
-            SampleShared& from = block_at(r);
-            const unsigned int c = from.listed;
-            for (unsigned int i = t; i < c && at + i < SAMPLE_LIST; i += SAMPLE_THREADS) sh.list[at + i] = from.list[i];
-            at += c;
+        if (blocks > 1) {
+            // Where each block's entries go; every thread then fetches its own, all on their way at once.
+            if (t < blocks) sh.listed_of[t] = block_at(t).listed;
+            __syncthreads();
+            for (int i = static_cast<int>(sh.listed_of[0]) + t; i < n; i += SAMPLE_THREADS) {
+                unsigned int at = i, r = 0;
+                while (at >= sh.listed_of[r]) at -= sh.listed_of[r++];
+                sh.list[i] = block_at(r).list[at];
+            }
+            __syncthreads();
         }
-        if (t == 0) sh.lowest = 0xffffffffu;
+        for (int i = t; i < n; i += SAMPLE_THREADS)
+            sh.weight[i] = score_weight(key_score(static_cast<uint32_t>(sh.list[i] >> 32)), top, inv);
         __syncthreads();
-        uint32_t lowest = 0xffffffffu;
-        for (int i = t; i < n; i += SAMPLE_THREADS) {
-            const uint32_t k = static_cast<uint32_t>(sh.list[i] >> 32);
-            lowest = min(lowest, k);
-            sh.weight[i] = score_weight(key_score(k), top, inv);
+    }
+    // A short list, an entry per thread: each sums what stands before it in the order of the scores, and
+    // then in that of the ids, over all others.
+    __device__ __forceinline__ bool draw_from_short_list(int n, double total, int64_t row, bool complete)
+    {
+        const Entry mine = t < n ? sh.list[t] : 0;
+        const double w = t < n ? sh.weight[t] : 0.0;
+        const Whole units = t < n ? whole(w) : 0;
+        sh.bins[t] = units;
+        __syncthreads();
+        int rank_of_mine = 0;
+        Whole before = 0;
+#pragma unroll 4
+        for (int i = 0; i < n; ++i)
+            if (sh.list[i] > mine) {
+                ++rank_of_mine;
+                before += sh.bins[i];
+            }
+        bool keep = t < n && (top_k == 0 || rank_of_mine < top_k), resolved = top_k == 0 || n >= top_k || complete;
+        if (resolved && nucleus) {
+            const Whole mass = block_total(keep ? units : 0);
+            const double want = ceil(top_p * (top_k > 0 ? static_cast<double>(mass) : total * unit));
+            const Whole least = want > 1.0 ? static_cast<Whole>(want) : Whole{1};
+            keep &= before < least;
+            if (top_k == 0) resolved = complete || mass >= least;
         }
-        lowest = __reduce_min_sync(FULL_WARP, lowest);
-        if (lane == 0) atomicMin(&sh.lowest, lowest);
+        if (!ends_inside(resolved, complete, n)) return false;
+        keep &= w >= min_p || static_cast<uint32_t>(mine >> 32) == top_key;
+        const Whole kept = keep ? units : 0;
+        const Whole m = block_total(kept);
+        sh.bins[t] = kept;
         __syncthreads();
+        Whole upto = 0;
+        const uint32_t order = static_cast<uint32_t>(mine); // ~id
+#pragma unroll 4
+        for (int i = 0; i < n; ++i)
+            if (static_cast<uint32_t>(sh.list[i]) >= order) upto += sh.bins[i];
+        const double target = u * static_cast<double>(m);
+        const Whole want = target < static_cast<double>(m) ? min(static_cast<Whole>(target) + 1, m) : m;
+        if (kept != 0 && upto >= want && upto - kept < want) p.ids[row] = static_cast<int64_t>(~order);
+        return true;
+    }
+    // Whether the filters' borders lie inside the list; else its weight is left in sh.listed_mass.  min_p ends
+    // inside where the threshold's own weight is below it.
+    __device__ __forceinline__ bool ends_inside(bool resolved, bool complete, int n)
+    {
+        if (floor_p && top_k == 0 && (!resolved || !nucleus))
+            resolved = complete || score_weight(key_score(threshold), top, inv) < min_p;
+        if (resolved) return true;
+        Whole m = 0;
+        for (int i = t; i < n; i += SAMPLE_THREADS) m += whole(sh.weight[i]);
+        m = block_total(m);
+        if (t == 0) sh.listed_mass = static_cast<double>(m) / unit;
+        return false;
     }
     // Rank 0: the filters and the draw on the list, which holds every score from the threshold up; false
     // where they reach below it.
@@ -594,43 +688,26 @@ template <typename T> struct SampleRow {
     {
         const bool complete = threshold == LOWEST_KEY;
         gather(n);
-        const float spread = top - key_score(sh.lowest);
-        const float per_score = spread > 0.0f ? SAMPLE_BINS / spread : 0.0f;
-        const float per_id = static_cast<float>(SAMPLE_BINS) / static_cast<float>(p.width);
-        auto score_bin = [&](Entry c) { return static_cast<int>(fminf((top - score_of(c)) * per_score, SAMPLE_BINS - 1)); };
-        auto id_bin = [&](Entry c) {
-            return static_cast<int>(fminf(static_cast<float>(~static_cast<uint32_t>(c)) * per_id, SAMPLE_BINS - 1));
-        };
+        if (n <= SAMPLE_THREADS) return draw_from_short_list(n, total, row, complete);
         bool resolved = true;
         Entry border = 0; // kept are the entries from here up
         if (top_k > 0) {
-            if (n >= top_k) border = border_of<false>(n, static_cast<Whole>(top_k), score_bin, [](int) { return Whole{1}; });
+            if (n >= top_k) border = border_of<false>(n, static_cast<Whole>(top_k), [](int) { return Whole{1}; });
             else resolved = complete;
         }
         if (resolved && nucleus) {
-            double mass = total * unit;
-            if (top_k > 0) {
-                Whole m = 0;
-                for (int i = t; i < n; i += SAMPLE_THREADS) m += sh.list[i] >= border ? whole(sh.weight[i]) : Whole{0};
-                mass = static_cast<double>(block_total(m));
-            }
-            const double want = ceil(top_p * mass);
             const Entry from = border;
-            const Entry at = border_of<false>(n, want > 1.0 ? static_cast<Whole>(want) : Whole{1}, score_bin,
-                                              [&](int i) { return sh.list[i] >= from ? whole(sh.weight[i]) : Whole{0}; });
-            if (at != 0) border = at;
-            else if (top_k == 0) resolved = complete; // every listed id is in the nucleus, and more may be
-        }
-        // min_p ends inside the list where the threshold's own weight is below it.
-        if (floor_p && top_k == 0 && (!resolved || !nucleus))
-            resolved = complete || score_weight(key_score(threshold), top, inv) < min_p;
-        if (!resolved) {
             Whole m = 0;
-            for (int i = t; i < n; i += SAMPLE_THREADS) m += whole(sh.weight[i]);
+            for (int i = t; i < n; i += SAMPLE_THREADS) m += sh.list[i] >= from ? whole(sh.weight[i]) : Whole{0};
             m = block_total(m);
-            if (t == 0) sh.listed_mass = static_cast<double>(m) / unit;
-            return false;
+            const double want = ceil(top_p * (top_k > 0 ? static_cast<double>(m) : total * unit));
+            const Whole least = want > 1.0 ? static_cast<Whole>(want) : Whole{1};
+            if (m >= least)
+                border = max(from, border_of<false>(n, least, [&](int i) { return sh.list[i] >= from ? whole(sh.weight[i]) : Whole{0}; }));
+            else if (top_k == 0)
+                resolved = complete; // every listed id is in the nucleus, and more may be
         }
+        if (!ends_inside(resolved, complete, n)) return false;
         const Entry from = border;
         auto kept = [&](int i) {
             const double w = sh.weight[i];
@@ -641,7 +718,7 @@ template <typename T> struct SampleRow {
         m = block_total(m);
         const double target = u * static_cast<double>(m);
         const Whole want = target < static_cast<double>(m) ? min(static_cast<Whole>(target) + 1, m) : m;
-        const Entry at = border_of<true>(n, want, id_bin, kept);
+        const Entry at = border_of<true>(n, want, kept);
         if (t == 0) p.ids[row] = static_cast<int64_t>(~static_cast<uint32_t>(at));
         return true;
     }
@@ -698,8 +775,12 @@ template <typename T> struct SampleRow {
         for (int m = 0; m < PER; ++m) {
             b[m] = 0;
             c[m] = 0;
-            for (int r = 0; r < blocks; ++r) {
-                SampleShared& from = block_at(r);
+        }
+#pragma unroll 2
+        for (int r = 0; r < blocks; ++r) {
+            SampleShared& from = block_at(r);
+#pragma unroll
+            for (int m = 0; m < PER; ++m) {
                 b[m] += from.bins[m * SAMPLE_THREADS + t];
                 c[m] += from.counts[m * SAMPLE_THREADS + t];
             }
@@ -770,7 +851,7 @@ template <typename T> struct SampleRow {
                 if (rank == 0) {
                     const int n = static_cast<int>(in_bin);
                     gather(n);
-                    const Entry border = select<false>(n, left, [&](int i) { return BY_MASS ? whole(sh.weight[i]) : Whole{1}; });
+                    const Entry border = border_of<false>(n, left, [&](int i) { return BY_MASS ? whole(sh.weight[i]) : Whole{1}; });
                     Whole equal = 0;
                     for (int i = t; i < n; i += SAMPLE_THREADS) equal += sh.list[i] >= border && (sh.list[i] >> 32) == (border >> 32);
                     equal = block_total(equal);
@@ -905,12 +986,7 @@ template <typename T> struct SampleRow {
         if (inside && rank == 0) {
             const int n = static_cast<int>(listed);
             gather(n);
-            const float finer = SAMPLE_BINS / (to - from);
-            auto bin_of = [&](Entry c) {
-                const float y = (top - score_of(c)) * per;
-                return static_cast<int>(fminf(fmaxf(y - from, 0.0f) * finer, SAMPLE_BINS - 1));
-            };
-            const Entry border = border_of<false>(n, static_cast<Whole>(ceil(rest)), bin_of, [&](int i) { return whole(sh.weight[i]); });
+            const Entry border = border_of<false>(n, static_cast<Whole>(ceil(rest)), [&](int i) { return whole(sh.weight[i]); });
             clear_bins();
             if (t == 0) sh.few = 0;
             __syncthreads();
