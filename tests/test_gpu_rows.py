@@ -705,6 +705,48 @@ def test_calls_on_two_streams_at_once():
             assert all(torch.equal(a, b) for a, b in zip(outs, want[i]))
 
 
+def test_refusals():
+    x, u = torch.zeros(4, 8, device=DEV), torch.zeros(4, device=DEV)
+    plan = povs.plan_rows(torch.zeros(4, 2, dtype=torch.int32, device=DEV), 3)
+    rows = torch.zeros(8, 5, device=DEV)
+    for call in (
+        lambda: povs.sample(x.double(), u), lambda: povs.sample(x, u.half()), lambda: povs.sample(x, u.cpu()),
+        lambda: povs.sample(x, u, temperature=u.double()), lambda: povs.sample(x, u, top_k=u),
+        lambda: povs.route(x.double(), 2), lambda: povs.route(x, 2, bias=torch.zeros(8, device=DEV).half()),
+        lambda: povs.route(x, 2, bias=torch.zeros(8)), lambda: povs.plan_rows(x, 3),
+        lambda: povs.dispatch_rows(x.cpu(), plan), lambda: povs.dispatch_rows(x, plan._replace(slots=plan.slots.long())),
+        lambda: povs.combine_rows(rows.double(), plan), lambda: povs.combine_rows(rows, plan, torch.zeros(4, 2, device=DEV).half()),
+        lambda: povs.dispatch_rows(x.double().requires_grad_(), plan),
+    ):
+        with pytest.raises(TypeError):
+            call()
+    for call in (
+        lambda: povs.sample(x.t(), u), lambda: povs.sample(x[0], u), lambda: povs.sample(x, u[:3]),
+        lambda: povs.sample(x, u, temperature=-1.0), lambda: povs.sample(x, u, temperature=float("nan")),
+        lambda: povs.sample(x, u, top_k=-1), lambda: povs.sample(x, u, top_p=1.5), lambda: povs.sample(x, u, min_p=-0.5),
+        lambda: povs.sample(x, u, top_p=u[:2]), lambda: povs.sample(x[:, :0], u),
+        lambda: povs.route(x.t(), 2), lambda: povs.route(x, 0), lambda: povs.route(x, 9), lambda: povs.route(x, 2, scoring="relu"),
+        lambda: povs.route(x, 2, n_groups=3), lambda: povs.route(x, 2, n_groups=4, top_groups=5),
+        lambda: povs.route(x, 3, n_groups=4, top_groups=1), lambda: povs.route(x, 2, group_score="mean"),
+        lambda: povs.route(x, 2, scale=float("inf")), lambda: povs.route(x, 2, bias=torch.zeros(7, device=DEV)),
+        lambda: povs.route(torch.zeros(2, 1025, device=DEV), 2), lambda: povs.plan_rows(plan.slots.t(), 3),
+        lambda: povs.plan_rows(plan.slots, 0), lambda: povs.plan_rows(plan.slots, 4097), lambda: povs.plan_rows(plan.slots[0], 3),
+        lambda: povs.dispatch_rows(x[:3], plan), lambda: povs.dispatch_rows(x.t()[:4], plan),
+        lambda: povs.combine_rows(rows[:7], plan), lambda: povs.combine_rows(rows, plan, torch.zeros(4, 3, device=DEV)),
+        lambda: povs.combine_rows(rows, plan, torch.zeros(2, 4, device=DEV).t()),
+    ):
+        with pytest.raises(AssertionError):
+            call()
+
+
+def test_row_operators_take_numpy_numbers_and_huge_top_k():
+    x, u = _scores(4, 50, torch.float32, seed=1), _uniforms(4, seed=2)
+    kw = dict(temperature=np.float32(0.5), top_k=np.int64(7), top_p=np.float32(0.5), min_p=np.float64(0.25))
+    np.testing.assert_array_equal(_host(povs.sample(x, u, **kw)), _sample_wanted(x, u, **{k: float(v) if k != "top_k" else 7 for k, v in kw.items()}))
+    assert torch.equal(povs.sample(x, u, top_k=2**70), povs.sample(x, u))
+    assert torch.equal(povs.route(x, np.int32(3), scale=np.float32(2)).weights, povs.route(x, 3, scale=2.0).weights)
+
+
 def test_gradients_refuse_a_second_order():
     plan = povs.plan_rows(_experts(8, 2, 4, seed=1), 4)
     for make in (lambda t: povs.route(t, 2).weights, lambda t: povs.dispatch_rows(t, plan)):
