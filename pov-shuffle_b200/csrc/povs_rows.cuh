@@ -525,8 +525,9 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, EPL <= 8 ? 8 : EPL <= 16 ? 5
 // 24 warps on an SM.  Where the order is the logits' and those have 16 bits, the numbers hold them whole and
 // nothing is left open.
 //
-// B200, top 8: 65536 x 256 float32 in 63 us with groups and bias (1.1 TB/s; a warp per row: 94), 35 us by the
-// logits alone; 32749 x 128 bfloat16 in 11 us (a warp per row: 17).  Bound by instructions.
+// B200, top 8: 65536 x 256 float32 in 57 us with groups and bias (1.25 TB/s; a warp per row: 94; without the
+// bound of 80 registers that lets 24 warps in, 63), 32 us by the logits alone; 32749 x 128 bfloat16 in 11 us (a
+// warp per row: 17).  Bound by instructions (530 a row with groups).
 constexpr int ROUTE_LIST = 8;
 
 __device__ __forceinline__ void exchange(uint32_t& a, uint32_t& b)
@@ -565,7 +566,7 @@ __device__ __forceinline__ void merge_down(uint32_t (&best)[ROUTE_LIST], const u
 __host__ __device__ __forceinline__ int route_pitch(int row_bytes) { return (row_bytes / 16 | 1) * 16; }
 
 template <typename T, int L, bool SIGMOID, bool BY_LOGIT, bool GROUPED>
-__global__ void __launch_bounds__(32) povs_route_lanes_kernel(const __grid_constant__ RouteParams p)
+__global__ void __launch_bounds__(32, 24) povs_route_lanes_kernel(const __grid_constant__ RouteParams p)
 {
     constexpr bool WHOLE = BY_LOGIT && sizeof(T) == 2; // numbers that hold the logits whole
     constexpr int V = 16 / sizeof(T), INDEX_BITS = WHOLE ? 16 : 9;

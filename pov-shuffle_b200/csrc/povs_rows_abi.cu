@@ -140,7 +140,7 @@ int route_lanes(const povs::RouteParams& p, int element)
 }
 
 // Lanes where rows fill the GPU with them, eight choices or fewer are asked, and rows and groups come in
-// whole pieces; else a warp per row.  B200, float32, top 8: 65536 x 256 with groups 63 us against 94 by warps,
+// whole pieces; else a warp per row.  B200, float32, top 8: 65536 x 256 with groups 57 us against 94 by warps,
 // 16384 x 256 13 against 20, but 8192 x 256 20 against 14 and 16384 x 512 58 against 36.
 bool route_by_lanes(const povs::RouteParams& p, int element, int sms)
 {
