@@ -102,6 +102,7 @@ class _Route(torch.autograd.Function):
     def forward(ctx, logits, bias, spec):
         experts, weights = _native.route(logits, bias, *spec)
         ctx.mark_non_differentiable(experts)
+        ctx.set_materialize_grads(False)  # or every backward pass would fill a gradient of experts
         ctx.save_for_backward(logits, experts)
         ctx.spec = spec
         return experts, weights
@@ -109,6 +110,8 @@ class _Route(torch.autograd.Function):
     @staticmethod
     def backward(ctx, _, grad_weights):
         _first_order()
+        if grad_weights is None:
+            return None, None, None
         logits, experts = ctx.saved_tensors
         top_k, scoring, _, _, _, renormalize, scale = ctx.spec
         return _native.route_backward(logits, experts, grad_weights.contiguous(), scoring, renormalize, scale), None, None
