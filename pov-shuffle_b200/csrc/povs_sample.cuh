@@ -909,25 +909,39 @@ template <typename T> struct SampleRow {
             range = static_cast<double>(hi) - static_cast<double>(lo);
         }
     }
-    // A nucleus whose border lies below the list (scores from `below` up weigh listed_mass).  Counts of
-    // the scores below it by bins of their distance from the top, each taken at its bin's middle, place
-    // the border to a small part of a bin; the next reading sums the weights above a window around
-    // that place and lists the window, and the border is found inside, with each part's kept weight.  False where it lies outside.
+    // A nucleus whose border lies below the list (scores from `below` up weigh listed_mass).  Counts of the
+    // scores below it by bins of their distance from the top, each taken at its bin's middle or mean, place
+    // the border to a small part of a bin; the next reading sums the weights above a window around that
+    // place and lists the window, and the border is found inside, with each part's kept weight.  False
+    // where it lies outside (none of 256 rows of 131072 normal scores at three temperatures and shares).
     __device__ __forceinline__ bool border_in_window(double need, double listed_mass, float below)
     {
         const float range = static_cast<float>(fmin(static_cast<double>(top) - static_cast<double>(key_score(sh.probe_low)), 45.0 / inv));
         const float per = range > 0.0f ? SAMPLE_BINS / range : 0.0f;
+        // Scores of 16 bits sit unevenly in a bin: the sum of their places in it, in steps of 1/256, gives the mean.
+        constexpr bool UNEVEN = sizeof(T) == 2;
+        unsigned int* places = reinterpret_cast<unsigned int*>(sh.weight); // the list's weights are done with
+        if (UNEVEN)
+            for (int b = t; b < SAMPLE_BINS; b += SAMPLE_THREADS) places[b] = 0;
         clear_bins();
         groups_of(first_group + t, SAMPLE_THREADS, last_group, (last_group - first_group + SAMPLE_THREADS - 1) / SAMPLE_THREADS,
                   [&](float (&v)[N], int) {
 #pragma unroll
                       for (int j = 0; j < N; ++j)
-                          if (v[j] < below && v[j] > -INFINITY)
-                              atomicAdd(&sh.counts[static_cast<int>(fminf((top - v[j]) * per, SAMPLE_BINS - 1))], 1u);
+                          if (v[j] < below && v[j] > -INFINITY) {
+                              const float y = (top - v[j]) * per;
+                              const int bin = static_cast<int>(fminf(y, SAMPLE_BINS - 1));
+                              atomicAdd(&sh.counts[bin], 1u);
+                              if (UNEVEN) atomicAdd(&places[bin], static_cast<unsigned int>(fminf((y - bin) * 256.0f, 255.0f)));
+                          }
                   });
-        cluster_bins();
-        for (int b = t; b < SAMPLE_BINS; b += SAMPLE_THREADS) sh.bins[b] = whole(exp(-(b + 0.5) / per * inv)) * sh.counts[b];
         __syncthreads();
+        for (int b = t; b < SAMPLE_BINS; b += SAMPLE_THREADS) {
+            const unsigned int c = sh.counts[b];
+            const double mean = UNEVEN && c != 0 ? (places[b] / static_cast<double>(c) + 0.5) / 256 : 0.5;
+            sh.bins[b] = whole(exp(-(b + mean) / per * inv)) * c;
+        }
+        cluster_bins();
         const double wanted = (need - listed_mass) * unit;
         crossing<SAMPLE_BINS>(wanted > 1.0 ? static_cast<Whole>(wanted) : Whole{1});
         const Whole found = sh.found;
@@ -935,19 +949,28 @@ template <typename T> struct SampleRow {
             __syncthreads();
             return false;
         }
-        // The window [from, to) in bins: the border's bin with its neighbours, as far as the list holds them;
-        // of a bin too full for it, the part around the border's place.
+        // The window [from, to) in bins: the border's bin and up to three on either side (scores of 16 bits sit
+        // unevenly in their bins), or one, as far as the list holds them; of a bin too full for it, the part
+        // around the border's place.
         constexpr unsigned int ROOM = SAMPLE_LIST - 200;
         const int bin = static_cast<int>(found);
-        const unsigned int here = sh.counts[bin], above = bin > 0 ? sh.counts[bin - 1] : 0, under = bin + 1 < SAMPLE_BINS ? sh.counts[bin + 1] : 0;
         const float place = static_cast<float>(static_cast<double>(sh.left) / static_cast<double>(sh.bins[bin]));
+        auto count_of = [&](int b) { return b >= 0 && b < SAMPLE_BINS ? sh.counts[b] : 0u; };
+        unsigned int inside_window = sh.counts[bin];
         float from = static_cast<float>(bin), to = from + 1.0f;
-        if (here > ROOM) {
-            from += place - 700.0f / static_cast<float>(here);
-            to = from + 1400.0f / static_cast<float>(here);
+        if (inside_window > ROOM) {
+            from += place - 700.0f / static_cast<float>(inside_window);
+            to = from + 1400.0f / static_cast<float>(inside_window);
+        } else if (inside_window + count_of(bin - 1) + count_of(bin + 1) > ROOM) {
+            if (place < 0.5f && inside_window + count_of(bin - 1) <= ROOM) from -= 1.0f;
+            if (place >= 0.5f && inside_window + count_of(bin + 1) <= ROOM) to += 1.0f;
         } else {
-            if (here + above <= ROOM && (place < 0.5f || here + above + under <= ROOM)) from -= 1.0f;
-            if (here + under <= ROOM && (place >= 0.5f || here + above + under <= ROOM)) to += 1.0f;
+            for (int around = 1; around <= 3; ++around) {
+                inside_window += count_of(bin - around) + count_of(bin + around);
+                if (around > 1 && inside_window > ROOM / 2) break;
+                from -= 1.0f;
+                to += 1.0f;
+            }
         }
         if (t == 0) sh.listed = 0;
         __syncthreads();
