@@ -357,7 +357,8 @@ int povs_ngram_count_v1(const void* ids, int32_t id_bytes, int64_t n_episodes, i
                         uint64_t* overflow, int64_t overflow_cap, int32_t device, void* stream);
 
 /*
- * Row operators whose order follows from scores.  Element types of scores and rows: */
+ * Row operators whose order follows from scores.  Every pointer is a multiple of its elements' size
+ * (others are refused).  Element types of scores and rows: */
 #define POVS_FLOAT32 0
 #define POVS_BFLOAT16 1
 #define POVS_FLOAT16 2

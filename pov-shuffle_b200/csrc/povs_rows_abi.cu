@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <initializer_list>
 
 #include "povs_host.h"
 #include "povs_rows.cuh"
@@ -63,6 +64,20 @@ int common_alignment(std::initializer_list<uint64_t> numbers)
 }
 
 uint64_t address(const void* p) { return reinterpret_cast<uint64_t>(p); }
+
+// The kernels load whole elements: one that is not on a multiple of its size would be a fault on the GPU.
+struct Elements {
+    const char* name;
+    const void* p;
+    int64_t size;
+};
+int check_aligned(std::initializer_list<Elements> all)
+{
+    for (const Elements& e : all)
+        if (address(e.p) % e.size != 0)
+            return fail(POVS_ERR_INVALID_ARGUMENT, "%s is not aligned to its elements of %lld bytes", e.name, static_cast<long long>(e.size));
+    return POVS_OK;
+}
 
 // Blocks of a grid-stride kernel: one per `per_block` units, at most `waves` per SM.
 int grid_for(int64_t units, int64_t per_block, int sms, int waves)
@@ -296,6 +311,9 @@ extern "C" int povs_sample_v1(const void* logits, int32_t dtype, int64_t rows, i
     if (top_ks == nullptr && top_k < 0) return fail(POVS_ERR_INVALID_ARGUMENT, "top_k must not be negative");
     if (top_ps == nullptr && !(top_p >= 0.0 && top_p <= 1.0)) return fail(POVS_ERR_INVALID_ARGUMENT, "top_p must be in [0, 1]");
     if (min_ps == nullptr && !(min_p >= 0.0 && min_p <= 1.0)) return fail(POVS_ERR_INVALID_ARGUMENT, "min_p must be in [0, 1]");
+    r = check_aligned({{"logits", logits, element_bytes(dtype)}, {"uniforms", uniforms, uniform_bytes}, {"temperatures", temperatures, 4},
+                       {"top_ks", top_ks, 4}, {"top_ps", top_ps, 4}, {"min_ps", min_ps, 4}, {"ids", ids, 8}});
+    if (r != POVS_OK) return r;
     if (rows == 0) return POVS_OK;
     DeviceGuard dg;
     int sms = 0;
@@ -362,6 +380,8 @@ extern "C" int povs_route_v1(const void* logits, int32_t dtype, int64_t rows, in
     if (rows == 0) return POVS_OK;
     if (experts == nullptr || weights == nullptr)
         return fail(POVS_ERR_INVALID_ARGUMENT, "experts and weights must not be NULL");
+    r = check_aligned({{"logits", logits, element_bytes(dtype)}, {"bias", bias, 4}, {"experts", experts, 4}, {"weights", weights, 4}});
+    if (r != POVS_OK) return r;
     DeviceGuard dg;
     int sms = 0;
     r = enter(dg, device, &sms);
@@ -397,6 +417,9 @@ extern "C" int povs_route_backward_v1(const void* logits, int32_t dtype, int64_t
     if (rows == 0) return POVS_OK;
     if (experts == nullptr || grad_weights == nullptr || grad_logits == nullptr)
         return fail(POVS_ERR_INVALID_ARGUMENT, "experts, grad_weights and grad_logits must not be NULL");
+    r = check_aligned({{"logits", logits, element_bytes(dtype)}, {"grad_logits", grad_logits, element_bytes(dtype)},
+                       {"experts", experts, 4}, {"grad_weights", grad_weights, 4}});
+    if (r != POVS_OK) return r;
     DeviceGuard dg;
     int sms = 0;
     r = enter(dg, device, &sms);
@@ -461,6 +484,9 @@ extern "C" int povs_plan_rows_v1(const void* experts, int32_t id_bytes, int64_t 
         if (workspace == nullptr || workspace_bytes < need)
             return fail(POVS_ERR_INVALID_ARGUMENT, "the workspace must hold %lld bytes", static_cast<long long>(need));
     }
+    r = check_aligned({{"experts", experts, id_bytes}, {"slots", slots, 4}, {"sources", sources, 4}, {"offsets", offsets, 4},
+                       {"workspace", blocks > 1 ? workspace : nullptr, 4}});
+    if (r != POVS_OK) return r;
     DeviceGuard dg;
     int sms = 0;
     r = enter(dg, device, &sms);
@@ -498,6 +524,8 @@ extern "C" int povs_dispatch_rows_v1(const void* data, int64_t rows, int64_t row
     if (row_bytes == 0 || n_slots == 0) return POVS_OK;
     if (out == nullptr || used == nullptr || (rows > 0 && (data == nullptr || slots == nullptr)))
         return fail(POVS_ERR_INVALID_ARGUMENT, "data, slots, used and out must not be NULL");
+    r = check_aligned({{"slots", slots, 4}, {"used", used, 4}});
+    if (r != POVS_OK) return r;
     DeviceGuard dg;
     int sms = 0;
     r = enter(dg, device, &sms);
@@ -543,13 +571,15 @@ extern "C" int povs_combine_rows_v1(const void* data, int32_t dtype, int64_t n_s
     if (rows == 0 || width == 0) return POVS_OK;
     if (out == nullptr || (n_slots > 0 && data == nullptr))
         return fail(POVS_ERR_INVALID_ARGUMENT, "data and out must not be NULL");
+    const int64_t size = element_bytes(dtype);
+    r = check_aligned({{"data", data, size}, {"slots", slots, 4}, {"weights", weights, 4}, {"out", out, size}});
+    if (r != POVS_OK) return r;
     DeviceGuard dg;
     int sms = 0;
     r = enter(dg, device, &sms);
     if (r != POVS_OK) return r;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const uint64_t size = element_bytes(dtype);
-    const int align = common_alignment({address(data), address(out), width * size, data_stride * size});
+    const int align = common_alignment({address(data), address(out), static_cast<uint64_t>(width * size), static_cast<uint64_t>(data_stride * size)});
     if (dtype == POVS_FLOAT32) launch_combine_by<float>(align, p, sms, s);
     else if (dtype == POVS_BFLOAT16) launch_combine_by<__nv_bfloat16>(align, p, sms, s);
     else launch_combine_by<__half>(align, p, sms, s);
@@ -581,14 +611,17 @@ extern "C" int povs_combine_backward_v1(const void* grad, const void* data, int3
     if (p.grad_data == nullptr && (grad_weights == nullptr || rows == 0)) return POVS_OK;
     if ((rows > 0 && width > 0 && grad == nullptr) || (grad_weights != nullptr && n_slots > 0 && width > 0 && data == nullptr))
         return fail(POVS_ERR_INVALID_ARGUMENT, "grad and data must not be NULL");
+    const int64_t size = element_bytes(dtype);
+    r = check_aligned({{"grad", grad, size}, {"data", data, size}, {"slots", slots, 4}, {"weights", weights, 4}, {"used", used, 4},
+                       {"grad_data", grad_data, size}, {"grad_weights", grad_weights, 4}});
+    if (r != POVS_OK) return r;
     DeviceGuard dg;
     int sms = 0;
     r = enter(dg, device, &sms);
     if (r != POVS_OK) return r;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const uint64_t size = element_bytes(dtype);
     const int align = common_alignment({address(grad), address(grad_weights != nullptr ? data : nullptr), address(p.grad_data),
-                                        width * size, grad_weights != nullptr ? data_stride * size : 0});
+                                        static_cast<uint64_t>(width * size), static_cast<uint64_t>(grad_weights != nullptr ? data_stride * size : 0)});
     if (dtype == POVS_FLOAT32) launch_combine_backward_by<float>(align, p, sms, s);
     else if (dtype == POVS_BFLOAT16) launch_combine_backward_by<__nv_bfloat16>(align, p, sms, s);
     else launch_combine_backward_by<__half>(align, p, sms, s);
