@@ -1113,7 +1113,10 @@ template <typename T> struct SampleRow {
         // The pair that holds the target; where rounding leaves none, the last one with a weight.
         const unsigned above = __ballot_sync(FULL_WARP, upto > target && two > 0.0), some = __ballot_sync(FULL_WARP, two > 0.0);
         const int pair = above != 0 ? __ffs(above) - 1 : 31 - __clz(some);
-        const double before_pair = __shfl_sync(FULL_WARP, upto - two, pair);
+        // What lies before it: the sum that was compared with the target there, not one rebuilt by a
+        // subtraction, which may round to above the target.
+        const double before_lane = __shfl_up_sync(FULL_WARP, upto, 1);
+        const double before_pair = __shfl_sync(FULL_WARP, lane == 0 ? 0.0 : before_lane, pair);
         const double even = __shfl_sync(FULL_WARP, part_mass[0], pair), odd = __shfl_sync(FULL_WARP, part_mass[1], pair);
         const Whole pair_ties = __shfl_sync(FULL_WARP, ties_before, pair), even_ties = __shfl_sync(FULL_WARP, part_ties[0], pair);
         const bool second = !(even > 0.0 && before_pair + even > target) && odd > 0.0;
@@ -1121,7 +1124,7 @@ template <typename T> struct SampleRow {
         if (some == 0 || part / parts != rank) return;
 
         // This block holds it: its threads share the part's groups, each a run of them in id order.
-        const double rest = target - (before_pair + (second ? even : 0.0));
+        const double rest = fmax(target - (before_pair + (second ? even : 0.0)), 0.0);
         const int from = part_first(part % parts), to = part_first(part % parts + 1);
         const int per_thread = (to - from + SAMPLE_THREADS - 1) / SAMPLE_THREADS;
         const int mine_first = min(from + t * per_thread, to), mine_last = min(mine_first + per_thread, to);
@@ -1136,7 +1139,7 @@ template <typename T> struct SampleRow {
         Whole seen = pair_ties + (second ? even_ties : 0) + equal_upto - equal;
         for (int w = 0; w < warp; ++w) seen += sh.part[w];
         const double mine = sum * weight_of.factor + tied(seen, equal, cut_weight);
-        const double mine_upto = warp_inclusive(mine, lane);
+        const double mine_upto = warp_inclusive(mine, lane), up = __shfl_up_sync(FULL_WARP, mine_upto, 1);
         if (lane == 31) sh.part_mass[warp] = mine_upto;
         if (t == 0) sh.found = ~0ull;
         __syncthreads();
@@ -1147,8 +1150,9 @@ template <typename T> struct SampleRow {
         if (mine > 0.0) atomicMin(&sh.found, ticket);
         __syncthreads();
         if (!(mine > 0.0) || sh.found != ticket) return;
-        double running = before + mine_upto - mine;
-        int64_t id = -1;
+        double running = lane == 0 ? before : before + up;
+        bool done = false;
+        int64_t id = -1; // the thread's first kept id whatever the sums say, then the next ones
         for (int g = mine_first; g < mine_last; ++g) {
             float v[N];
             x.load(g, v);
@@ -1158,11 +1162,12 @@ template <typename T> struct SampleRow {
                 if (k == 0 || k < cut) continue;
                 if (cut != 0 && k == cut && seen++ >= ties) continue;
                 const double w = score_weight(v[j], top, inv);
-                if (!(w >= min_p || k == top_key) || w == 0.0 || running > rest) continue;
+                if (!(w >= min_p || k == top_key) || w == 0.0 || done) continue;
                 id = x.id(g) + j;
                 running += w;
+                done = running > rest;
             }
-            if (running > rest) break;
+            if (done) break;
         }
         p.ids[row] = id;
     }
