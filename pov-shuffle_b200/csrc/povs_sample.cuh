@@ -243,8 +243,9 @@ template <typename T> struct SampleRow {
     // What the stream leaves.
     float top, warp_top, reference;
     uint32_t top_key;
-    // Kept are the keys above `cut` and, in id order, the first `ties` of those equal to it (0: all).
-    uint32_t cut = 0;
+    // Kept are the keys above `cut` and, in id order, the first `ties` of those equal to it (0: all), of these the
+    // ones from `lowest` up.
+    uint32_t cut = 0, lowest = LOWEST_KEY;
     Whole ties = 0;
     int parity = 0;
     // Parts 2 lane and 2 lane + 1 of the row.
@@ -1053,6 +1054,14 @@ template <typename T> struct SampleRow {
     }
 
     // --- The draw in id order, with `cut` and `ties` settled.
+    // The lowest key that sums and draw count, the same for both.  Scores whose weight is below 2^-400 (masks of a
+    // finite value) are left out: WarpExp gives them 2^-500 and more, where in 64 bits they weigh nothing that a
+    // random number could tell.
+    __device__ __forceinline__ uint32_t lowest_counted() const
+    {
+        const float v = __double2float_ru(static_cast<double>(top) - 400.0 * 0.69314718055994530942 / inv);
+        return min(max(score_key(v), LOWEST_KEY), top_key);
+    }
     // Weight of `have` ids equal to the cut, `before` of them before.
     __device__ __forceinline__ double tied(Whole before, Whole have, double cut_weight) const
     {
@@ -1065,9 +1074,10 @@ template <typename T> struct SampleRow {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const uint32_t k = score_key(v[j]);
+            const bool in = k > cut && k >= lowest;
             equal += cut != 0 && k == cut;
-            if (k <= cut) v[j] = -INFINITY;
-            any |= k > cut;
+            if (!in) v[j] = -INFINITY;
+            any |= in;
         }
         if (__any_sync(FULL_WARP, any)) {
 #pragma unroll
@@ -1102,11 +1112,15 @@ template <typename T> struct SampleRow {
     __device__ __forceinline__ void draw(int64_t row, double min_weight)
     {
         const double w_cut = cut != 0 ? score_weight(key_score(cut), top, inv) : 0.0;
-        const double cut_weight = cut == top_key || w_cut >= min_p ? w_cut : 0.0;
+        const double cut_weight = cut >= lowest && (cut == top_key || w_cut >= min_p) ? w_cut : 0.0;
         const Whole two_ties = part_ties[0] + part_ties[1];
         const Whole ties_before = warp_inclusive(two_ties, lane) - two_ties;
         part_mass[0] += tied(ties_before, part_ties[0], cut_weight);
         part_mass[1] += tied(ties_before + part_ties[0], part_ties[1], cut_weight);
+        // A part of nothing but scores left out would be one without an id to draw.
+        const double least = warp_sum(part_mass[0] + part_mass[1]) * 0x1p-200;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) part_mass[h] = part_mass[h] > least ? part_mass[h] : 0.0;
         const double two = part_mass[0] + part_mass[1];
         const double upto = warp_inclusive(two, lane);
         const double target = u * __shfl_sync(FULL_WARP, upto, 31);
@@ -1159,10 +1173,10 @@ template <typename T> struct SampleRow {
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 const uint32_t k = score_key(v[j]);
-                if (k == 0 || k < cut) continue;
+                if (k < lowest || k < cut) continue;
                 if (cut != 0 && k == cut && seen++ >= ties) continue;
                 const double w = score_weight(v[j], top, inv);
-                if (!(w >= min_p || k == top_key) || w == 0.0 || done) continue;
+                if (!(w >= min_p || k == top_key) || done) continue;
                 id = x.id(g) + j;
                 running += w;
                 done = running > rest;
@@ -1230,6 +1244,7 @@ template <typename T> struct SampleRow {
         }
 
         weight_of.refer(lone ? 0.0f : top, inv);
+        lowest = lowest_counted();
         const double min_weight = min_p / weight_of.factor; // in the units of weight_of
         bool summed = !filtered && !lone; // part_mass and part_ties hold what each part's ids keep
         if (lone) {

@@ -49,3 +49,27 @@ def test_sample_constant_rows_at_even_random_numbers(dtype, width, score):
     want = torch.floor(u * width).long()
     assert (ids >= 0).all() and (ids < width).all()
     assert ((ids - want).abs() <= 1).all()
+
+
+ENDS = [0.0, 2.0**-60, 0.5, 1.0 - 2.0**-24, 1.0 - 2.0**-53, 1.0, 7.5, -1.0, float("nan")]
+
+
+@pytest.mark.parametrize("kw", [{}, {"temperature": 0.05}, {"top_p": 0.999}, {"top_k": 3000}, {"min_p": 1e-7},
+                                {"top_k": 3000, "min_p": 1e-3}], ids=str)
+@pytest.mark.parametrize("dtype,mask", [(torch.float32, -1e4), (torch.float32, "lowest"), (torch.float16, "lowest")], ids=str)
+@pytest.mark.parametrize("width", [301, 40_009])
+def test_sample_masks_of_finite_value_are_never_drawn(width, dtype, mask, kw):
+    """Ids masked with a finite score weigh 0 in 64 bits.  Between masked runs at both ends, random numbers at
+    and beyond the ends of [0, 1) draw the first or the last id that has a weight."""
+    first, last = width // 3, width - width // 4
+    x = torch.full((len(ENDS), width), torch.finfo(dtype).min if mask == "lowest" else mask, dtype=dtype)
+    x[:, first:last] = torch.linspace(0.0, 1.0, last - first).to(dtype) * 0.01
+    x = x.to(DEV)
+    for u in (torch.tensor(ENDS, dtype=torch.float64, device=DEV), torch.tensor(ENDS, device=DEV)):
+        got = _host(povs.sample(x, u, **kw))
+        want = [oracle.sample_row(_host(x[r]), 0.0 if np.isnan(v) else v, **kw) for r, v in enumerate(_host(u))]
+        low, high = want[0], want[5]
+        assert first <= low <= high < last
+        exact = [0, 5, 6, 7, 8]
+        assert [got[i] for i in exact] == [want[i] for i in exact]
+        assert (got >= low).all() and (got <= high).all()
