@@ -1062,13 +1062,28 @@ template <typename T> struct SampleRow {
         const float v = __double2float_ru(static_cast<double>(top) - 400.0 * 0.69314718055994530942 / inv);
         return min(max(score_key(v), LOWEST_KEY), top_key);
     }
+    // The lowest key whose weight is min_p or more (the highest score's always is): a warp's 32 lanes cut the
+    // range of keys 33-fold a round, with the weights that the list is filtered by.
+    __device__ __forceinline__ uint32_t lowest_of_min_p() const
+    {
+        uint32_t below = LOWEST_KEY - 1, kept = top_key;
+        while (kept - below > 1) {
+            const uint32_t at = below + static_cast<uint32_t>(static_cast<uint64_t>(kept - below) * (lane + 1) / 33);
+            const unsigned in = __ballot_sync(FULL_WARP, at > below && score_weight(key_score(at), top, inv) >= min_p);
+            const uint32_t last_out = __shfl_sync(FULL_WARP, at, in == 0 ? 31 : max(__ffs(in) - 2, 0));
+            const uint32_t first_in = __shfl_sync(FULL_WARP, at, in == 0 ? 0 : __ffs(in) - 1);
+            if (!(in & 1)) below = last_out;
+            if (in != 0) kept = first_in;
+        }
+        return kept;
+    }
     // Weight of `have` ids equal to the cut, `before` of them before.
     __device__ __forceinline__ double tied(Whole before, Whole have, double cut_weight) const
     {
         return before >= ties ? 0.0 : static_cast<double>(min(have, ties - before)) * cut_weight;
     }
     // Adds a group's kept weights, ties apart, in units of weight_of.  The whole warp takes part.
-    __device__ __forceinline__ void add_kept(float (&v)[N], double min_weight, double& sum, Whole& equal)
+    __device__ __forceinline__ void add_kept(float (&v)[N], double& sum, Whole& equal)
     {
         bool any = false;
 #pragma unroll
@@ -1083,16 +1098,16 @@ template <typename T> struct SampleRow {
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 const double w = weight_of(v[j], p.poly);
-                if (v[j] > -INFINITY && (w >= min_weight || v[j] == top)) sum += w;
+                if (v[j] > -INFINITY) sum += w;
             }
         }
     }
-    __device__ __forceinline__ void sum_parts(double min_weight)
+    __device__ __forceinline__ void sum_parts()
     {
         for (int q = warp * warp_parts; q < (warp + 1) * warp_parts; ++q) {
             double sum = 0.0;
             Whole equal = 0;
-            each_of_part(q, [&](float (&v)[N], int) { add_kept(v, min_weight, sum, equal); });
+            each_of_part(q, [&](float (&v)[N], int) { add_kept(v, sum, equal); });
             sum = warp_sum(sum) * weight_of.factor;
             equal = warp_sum(equal);
             if (lane == 0) {
@@ -1109,10 +1124,10 @@ template <typename T> struct SampleRow {
             part_ties[h] = from.ties[e % parts];
         }
     }
-    __device__ __forceinline__ void draw(int64_t row, double min_weight)
+    __device__ __forceinline__ void draw(int64_t row)
     {
         const double w_cut = cut != 0 ? score_weight(key_score(cut), top, inv) : 0.0;
-        const double cut_weight = cut >= lowest && (cut == top_key || w_cut >= min_p) ? w_cut : 0.0;
+        const double cut_weight = cut >= lowest ? w_cut : 0.0;
         const Whole two_ties = part_ties[0] + part_ties[1];
         const Whole ties_before = warp_inclusive(two_ties, lane) - two_ties;
         part_mass[0] += tied(ties_before, part_ties[0], cut_weight);
@@ -1144,7 +1159,7 @@ template <typename T> struct SampleRow {
         const int mine_first = min(from + t * per_thread, to), mine_last = min(mine_first + per_thread, to);
         double sum = 0.0;
         Whole equal = 0;
-        groups_of(mine_first, 1, mine_last, per_thread, [&](float (&v)[N], int) { add_kept(v, min_weight, sum, equal); });
+        groups_of(mine_first, 1, mine_last, per_thread, [&](float (&v)[N], int) { add_kept(v, sum, equal); });
         // Running sums over the block: of the ties, then of the weights with the ties that are kept.
         const Whole equal_upto = warp_inclusive(equal, lane);
         __syncthreads();
@@ -1175,10 +1190,9 @@ template <typename T> struct SampleRow {
                 const uint32_t k = score_key(v[j]);
                 if (k < lowest || k < cut) continue;
                 if (cut != 0 && k == cut && seen++ >= ties) continue;
-                const double w = score_weight(v[j], top, inv);
-                if (!(w >= min_p || k == top_key) || done) continue;
+                if (done) continue;
                 id = x.id(g) + j;
-                running += w;
+                running += score_weight(v[j], top, inv);
                 done = running > rest;
             }
             if (done) break;
@@ -1245,7 +1259,7 @@ template <typename T> struct SampleRow {
 
         weight_of.refer(lone ? 0.0f : top, inv);
         lowest = lowest_counted();
-        const double min_weight = min_p / weight_of.factor; // in the units of weight_of
+        if (floor_p && !lone) lowest = max(lowest, lowest_of_min_p());
         bool summed = !filtered && !lone; // part_mass and part_ties hold what each part's ids keep
         if (lone) {
             Whole c = 0;
@@ -1274,9 +1288,9 @@ template <typename T> struct SampleRow {
                 narrow<true>(want > 1.0 ? static_cast<Whole>(want) : Whole{1});
             }
         }
-        if (!summed) sum_parts(min_weight);
+        if (!summed) sum_parts();
         everyone(); // the last look at the other blocks
-        draw(row, min_weight);
+        draw(row);
     }
 };
 

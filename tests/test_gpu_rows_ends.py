@@ -73,3 +73,15 @@ def test_sample_masks_of_finite_value_are_never_drawn(width, dtype, mask, kw):
         exact = [0, 5, 6, 7, 8]
         assert [got[i] for i in exact] == [want[i] for i in exact]
         assert (got >= low).all() and (got <= high).all()
+
+
+@pytest.mark.parametrize("kw", [{}, {"top_p": 0.9999}, {"top_k": 30_000}], ids=str)
+@pytest.mark.parametrize("width", [500, 40_009])
+def test_sample_min_p_at_a_weight(width, kw):
+    """A lowest weight 2^-46 above or below that of thousands of equal scores keeps all of them or none."""
+    x = torch.where(torch.arange(width) % 3 == 0, 0.0, -2.0).to(torch.float32).expand(40, -1).to(DEV)
+    u = ((torch.arange(40, dtype=torch.float64) + 0.5) / 40).to(DEV)
+    for min_p in (math.exp(-2.0) * (1 - 2.0**-46), math.exp(-2.0) * (1 + 2.0**-46)):
+        got = _host(povs.sample(x, u, min_p=min_p, **kw))
+        want = [oracle.sample_row(_host(x[r]), v, min_p=min_p, **kw) for r, v in enumerate(_host(u))]
+        np.testing.assert_array_equal(got, want)
