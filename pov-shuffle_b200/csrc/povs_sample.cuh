@@ -235,7 +235,6 @@ template <typename T> struct SampleRow {
     double top_p, min_p, inv, u;
     bool nucleus, floor_p, filtered, need_mass;
     double unit;
-    int id_bits;
     // The list's threshold (`list_from` +infinity: no list).
     uint32_t threshold;
     float list_from;
@@ -287,8 +286,6 @@ template <typename T> struct SampleRow {
         u = p.uniform_bytes == 4 ? static_cast<const float*>(p.uniforms)[row] : static_cast<const double*>(p.uniforms)[row];
         u = u > 0.0 ? u : 0.0;
         unit = static_cast<double>(1ull << p.weight_bits);
-        id_bits = 0;
-        while (id_bits < 32 && (p.width - 1) >> id_bits) ++id_bits;
     }
 
     __device__ __forceinline__ void everyone()
@@ -662,6 +659,12 @@ template <typename T> struct SampleRow {
         }
         if (!ends_inside(resolved, complete, n)) return false;
         keep &= w >= min_p || static_cast<uint32_t>(mine >> 32) == top_key;
+        if (u == 0.0) {
+            Entry first = keep && w > 0.0 ? static_cast<Entry>(static_cast<uint32_t>(~mine)) : ~0ull, unused = 0;
+            block_range(first, unused);
+            if (t == 0) p.ids[row] = static_cast<int64_t>(first);
+            return true;
+        }
         const Whole kept = keep ? units : 0;
         const Whole m = block_total(kept);
         sh.bins[t] = kept;
@@ -720,6 +723,15 @@ template <typename T> struct SampleRow {
             const double w = sh.weight[i];
             return sh.list[i] >= from && (w >= min_p || static_cast<uint32_t>(sh.list[i] >> 32) == top_key) ? whole(w) : Whole{0};
         };
+        if (u == 0.0) { // the lowest id kept, however small its weight
+            Entry first = ~0ull, unused = 0;
+            for (int i = t; i < n; i += SAMPLE_THREADS)
+                if (sh.list[i] >= from && sh.weight[i] > 0.0 && (sh.weight[i] >= min_p || static_cast<uint32_t>(sh.list[i] >> 32) == top_key))
+                    first = min(first, static_cast<Entry>(static_cast<uint32_t>(~sh.list[i])));
+            block_range(first, unused);
+            if (t == 0) p.ids[row] = static_cast<int64_t>(first);
+            return true;
+        }
         Whole m = 0;
         for (int i = t; i < n; i += SAMPLE_THREADS) m += kept(i);
         m = block_total(m);
@@ -1062,14 +1074,14 @@ template <typename T> struct SampleRow {
         const float v = __double2float_ru(static_cast<double>(top) - 400.0 * 0.69314718055994530942 / inv);
         return min(max(score_key(v), LOWEST_KEY), top_key);
     }
-    // The lowest key whose weight is min_p or more (the highest score's always is): a warp's 32 lanes cut the
+    // The lowest key whose weight is `least` or more (the highest score's always is): a warp's 32 lanes cut the
     // range of keys 33-fold a round, with the weights that the list is filtered by.
-    __device__ __forceinline__ uint32_t lowest_of_min_p() const
+    __device__ __forceinline__ uint32_t lowest_of(double least) const
     {
         uint32_t below = LOWEST_KEY - 1, kept = top_key;
         while (kept - below > 1) {
             const uint32_t at = below + static_cast<uint32_t>(static_cast<uint64_t>(kept - below) * (lane + 1) / 33);
-            const unsigned in = __ballot_sync(FULL_WARP, at > below && score_weight(key_score(at), top, inv) >= min_p);
+            const unsigned in = __ballot_sync(FULL_WARP, at > below && score_weight(key_score(at), top, inv) >= least);
             const uint32_t last_out = __shfl_sync(FULL_WARP, at, in == 0 ? 31 : max(__ffs(in) - 2, 0));
             const uint32_t first_in = __shfl_sync(FULL_WARP, at, in == 0 ? 0 : __ffs(in) - 1);
             if (!(in & 1)) below = last_out;
@@ -1200,6 +1212,23 @@ template <typename T> struct SampleRow {
         p.ids[row] = id;
     }
 
+    // The draw at 0: the lowest id kept, however small its weight.
+    __device__ __forceinline__ void draw_first(int64_t row)
+    {
+        Entry first = ~0ull, unused = 0;
+        each([&](float, uint32_t k, uint32_t id) {
+            if (k >= lowest && k >= cut) first = min(first, static_cast<Entry>(id));
+        });
+        block_range(first, unused);
+        if (blocks > 1) {
+            if (t == 0) sh.exchange[parity] = first;
+            cluster.sync();
+            for (int r = 0; r < blocks; ++r) first = min(first, block_at(r).exchange[parity]);
+            cluster.sync(); // the last look at the other blocks
+        }
+        if (rank == 0 && t == 0) p.ids[row] = static_cast<int64_t>(first);
+    }
+
     __device__ __forceinline__ void run(int64_t row)
     {
         if (t == 0) {
@@ -1259,7 +1288,8 @@ template <typename T> struct SampleRow {
 
         weight_of.refer(lone ? 0.0f : top, inv);
         lowest = lowest_counted();
-        if (floor_p && !lone) lowest = max(lowest, lowest_of_min_p());
+        if (u == 0.0 && !lone) lowest = lowest_of(fmax(min_p, 4.9406564584124654e-324));
+        else if (floor_p && !lone) lowest = max(lowest, lowest_of(min_p));
         bool summed = !filtered && !lone; // part_mass and part_ties hold what each part's ids keep
         if (lone) {
             Whole c = 0;
@@ -1287,6 +1317,10 @@ template <typename T> struct SampleRow {
                 const double want = ceil(need * unit);
                 narrow<true>(want > 1.0 ? static_cast<Whole>(want) : Whole{1});
             }
+        }
+        if (u == 0.0) {
+            draw_first(row);
+            return;
         }
         if (!summed) sum_parts();
         everyone(); // the last look at the other blocks

@@ -85,3 +85,22 @@ def test_sample_min_p_at_a_weight(width, kw):
         got = _host(povs.sample(x, u, min_p=min_p, **kw))
         want = [oracle.sample_row(_host(x[r]), v, min_p=min_p, **kw) for r, v in enumerate(_host(u))]
         np.testing.assert_array_equal(got, want)
+
+
+@pytest.mark.parametrize("kw", [{}, {"top_k": 200}, {"top_k": 2000}, {"top_k": 9000}, {"top_p": 1 - 1e-15}, {"min_p": 1e-200}], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("width", [257, 5000, 40_009])
+def test_sample_zero_draws_the_first_weight(width, dtype, kw):
+    """At 0 the running sum has to exceed 0: the lowest id with any weight that 64 bits hold."""
+    rows = 8
+    g = torch.Generator().manual_seed(width)
+    x = -torch.rand(rows, width, generator=g) * 0.2
+    heavy = torch.randint(width // 2, width, (rows, 1), generator=g)
+    x.scatter_(1, heavy, 0.0)
+    for temperature, level in ((1.0, 60.0), (0.1, 9.0), (0.01, 6.5)):
+        y = (x * 0.1 - level).scatter_(1, heavy, 0.0)
+        y[0::2, :3] = -800.0  # weighs nothing at any of the temperatures
+        y = y.to(dtype).to(DEV)
+        got = _host(povs.sample(y, torch.zeros(rows, device=DEV), temperature=temperature, **kw))
+        want = [oracle.sample_row(_host(r), 0.0, temperature=temperature, **kw) for r in y]
+        np.testing.assert_array_equal(got, want)
