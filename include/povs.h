@@ -377,8 +377,11 @@ int povs_ngram_count_v1(const void* ids, int32_t id_bytes, int64_t n_episodes, i
  * whole sum.  temperature 0 (in the array: any value not above 0, or NaN): the lowest id of the
  * highest score.  Where some scores are +infinity, they alone have a weight, each the same.  A row without a
  * number above -infinity gets -1.  temperatures, top_ks, top_ps and min_ps are NULL or hold one value
- * per row in place of the value beside them; temperatures above 1e28 count as 1e28.  Weights and sums
- * have 64 bits and are good to 2^-40 of the row's sum; the id is the same on every run.
+ * per row in place of the value beside them; temperatures above 1e28 count as 1e28, those below 1e-36 as
+ * 1e-36.  Weights and sums have 64 bits, good to 2^-40 of the row's sum.  Where top_p keeps, or top_k with top_p
+ * reaches, more ids than fit a list of 2048, top_p's border may be found from weights rounded to whole numbers
+ * that keep a row's sum below 2^63: with n = ceil(log2(width)) good to 2^(2n - 63) of the sum at worst (2^-29 for
+ * 131072 ids).  uniforms 0 draws the first id with any weight.  The id is the same on every run.
  * No reference counterpart: numpy.random.Generator.choice beside its Generator.shuffle baseline.
  */
 int povs_sample_v1(const void* logits, int32_t dtype, int64_t rows, int64_t width, int64_t row_stride,

@@ -34,7 +34,7 @@ struct SampleParams {
     int64_t row_stride; // elements
     const void* uniforms;
     int32_t uniform_bytes; // 4 or 8
-    int32_t weight_bits;   // in sums of whole numbers a weight of 1 is 2^weight_bits; a row's sum stays below 2^63
+    int32_t weight_bits;   // in sums of whole numbers over a row a weight of 1 is 2^weight_bits; they stay below 2^63
     int32_t cluster;       // blocks per row
     // One value per row, or NULL for the value beside it.
     const float* temperatures;
@@ -53,6 +53,7 @@ constexpr int SAMPLE_THREADS = 256;
 constexpr int SAMPLE_WARPS = SAMPLE_THREADS / 32;
 constexpr int SAMPLE_MAX_CLUSTER = 8;
 constexpr int SAMPLE_LIST = 2048;   // listed scores per block, and per row
+constexpr double LIST_UNIT = 0x1p51; // a weight of 1 in sums over a list: those stay at or below 2^62
 constexpr int SAMPLE_TARGET = 1024; // listed scores aimed at where no top_k says how many
 constexpr int SAMPLE_PROBE = 4096;  // scores probed
 constexpr int SAMPLE_BINS = 1024;
@@ -219,7 +220,7 @@ template <typename T> struct SampleRow {
     using Groups = RowGroups<T>;
     static constexpr int N = Groups::N;
     using Entry = unsigned long long; // an entry of the list
-    using Whole = unsigned long long; // a weight in units of 2^-weight_bits, or a count
+    using Whole = unsigned long long; // a weight in units, or a count
 
     const SampleParams& p;
     SampleShared& sh;
@@ -295,7 +296,12 @@ template <typename T> struct SampleRow {
     }
     __device__ __forceinline__ SampleShared& block_at(int r) { return blocks > 1 ? *cluster.map_shared_rank(&sh, r) : sh; }
     __device__ __forceinline__ int part_first(int q) const { return min(first_group + q * per_part, last_group); }
+    // Weights as whole numbers, whose sums no order of adding changes: in a row's units for sums over all of it,
+    // in the list's own (good to 2^-41 in all) for sums over a list.
     __device__ __forceinline__ Whole whole(double w) const { return static_cast<Whole>(llrint(w * unit)); }
+    __device__ __forceinline__ static Whole list_units(double w) { return static_cast<Whole>(llrint(w * LIST_UNIT)); }
+    // The least whole number not below `want`, at least 1; beyond a list's whole sum any number is the same.
+    __device__ __forceinline__ static Whole least_of(double want) { return want > 1.0 ? static_cast<Whole>(ceil(fmin(want, 0x1p63))) : Whole{1}; }
     __device__ __forceinline__ static float score_of(Entry c) { return key_score(static_cast<uint32_t>(c >> 32)); }
 
     __device__ __forceinline__ Whole block_total(Whole v)
@@ -638,7 +644,7 @@ template <typename T> struct SampleRow {
     {
         const Entry mine = t < n ? sh.list[t] : 0;
         const double w = t < n ? sh.weight[t] : 0.0;
-        const Whole units = t < n ? whole(w) : 0;
+        const Whole units = t < n ? list_units(w) : 0;
         sh.bins[t] = units;
         __syncthreads();
         int rank_of_mine = 0;
@@ -652,8 +658,7 @@ template <typename T> struct SampleRow {
         bool keep = t < n && (top_k == 0 || rank_of_mine < top_k), resolved = top_k == 0 || n >= top_k || complete;
         if (resolved && nucleus) {
             const Whole mass = block_total(keep ? units : 0);
-            const double want = ceil(top_p * (top_k > 0 ? static_cast<double>(mass) : total * unit));
-            const Whole least = want > 1.0 ? static_cast<Whole>(want) : Whole{1};
+            const Whole least = least_of(top_p * (top_k > 0 ? static_cast<double>(mass) : total * LIST_UNIT));
             keep &= before < least;
             if (top_k == 0) resolved = complete || mass >= least;
         }
@@ -687,9 +692,9 @@ template <typename T> struct SampleRow {
             resolved = complete || score_weight(key_score(threshold), top, inv) < min_p;
         if (resolved) return true;
         Whole m = 0;
-        for (int i = t; i < n; i += SAMPLE_THREADS) m += whole(sh.weight[i]);
+        for (int i = t; i < n; i += SAMPLE_THREADS) m += list_units(sh.weight[i]);
         m = block_total(m);
-        if (t == 0) sh.listed_mass = static_cast<double>(m) / unit;
+        if (t == 0) sh.listed_mass = static_cast<double>(m) / LIST_UNIT;
         return false;
     }
     // Rank 0: the filters and the draw on the list, which holds every score from the threshold up; false
@@ -708,12 +713,11 @@ template <typename T> struct SampleRow {
         if (resolved && nucleus) {
             const Entry from = border;
             Whole m = 0;
-            for (int i = t; i < n; i += SAMPLE_THREADS) m += sh.list[i] >= from ? whole(sh.weight[i]) : Whole{0};
+            for (int i = t; i < n; i += SAMPLE_THREADS) m += sh.list[i] >= from ? list_units(sh.weight[i]) : Whole{0};
             m = block_total(m);
-            const double want = ceil(top_p * (top_k > 0 ? static_cast<double>(m) : total * unit));
-            const Whole least = want > 1.0 ? static_cast<Whole>(want) : Whole{1};
+            const Whole least = least_of(top_p * (top_k > 0 ? static_cast<double>(m) : total * LIST_UNIT));
             if (m >= least)
-                border = max(from, border_of<false>(n, least, [&](int i) { return sh.list[i] >= from ? whole(sh.weight[i]) : Whole{0}; }));
+                border = max(from, border_of<false>(n, least, [&](int i) { return sh.list[i] >= from ? list_units(sh.weight[i]) : Whole{0}; }));
             else if (top_k == 0)
                 resolved = complete; // every listed id is in the nucleus, and more may be
         }
@@ -721,7 +725,7 @@ template <typename T> struct SampleRow {
         const Entry from = border;
         auto kept = [&](int i) {
             const double w = sh.weight[i];
-            return sh.list[i] >= from && (w >= min_p || static_cast<uint32_t>(sh.list[i] >> 32) == top_key) ? whole(w) : Whole{0};
+            return sh.list[i] >= from && (w >= min_p || static_cast<uint32_t>(sh.list[i] >> 32) == top_key) ? list_units(w) : Whole{0};
         };
         if (u == 0.0) { // the lowest id kept, however small its weight
             Entry first = ~0ull, unused = 0;
@@ -1023,12 +1027,12 @@ template <typename T> struct SampleRow {
             const int e = 2 * lane + h;
             part_mass[h] = block_at(e / parts).mass[e % parts];
         }
-        const double rest = (need - warp_sum(part_mass[0] + part_mass[1])) * unit;
+        const double rest = (need - warp_sum(part_mass[0] + part_mass[1])) * LIST_UNIT;
         const bool inside = listed <= SAMPLE_LIST && rest >= 1.0;
         if (inside && rank == 0) {
             const int n = static_cast<int>(listed);
             gather(n);
-            const Entry border = border_of<false>(n, static_cast<Whole>(ceil(rest)), [&](int i) { return whole(sh.weight[i]); });
+            const Entry border = border_of<false>(n, least_of(rest), [&](int i) { return list_units(sh.weight[i]); });
             clear_bins();
             if (t == 0) sh.few = 0;
             __syncthreads();
@@ -1040,7 +1044,7 @@ template <typename T> struct SampleRow {
                 // The part that holds it.
                 const int g = static_cast<int>((static_cast<int64_t>(~static_cast<uint32_t>(c)) + x.lead) / N);
                 const int e = g / per_block * parts + g % per_block / per_part;
-                if (k > key) atomicAdd(&sh.bins[e], whole(sh.weight[i]));
+                if (k > key) atomicAdd(&sh.bins[e], list_units(sh.weight[i]));
                 else atomicAdd(&sh.counts[e], 1u);
                 if (c >= border && k == key) atomicAdd(&sh.few, 1);
             }
@@ -1057,7 +1061,7 @@ template <typename T> struct SampleRow {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int e = 2 * lane + h;
-                part_mass[h] += static_cast<double>(block_at(0).bins[e]) / unit;
+                part_mass[h] += static_cast<double>(block_at(0).bins[e]) / LIST_UNIT;
                 part_ties[h] = block_at(0).counts[e];
             }
         }

@@ -31,7 +31,9 @@ def sample(
     always stays).  The result is the lowest id at which the kept weights, summed in id order, exceed
     the row's uniform number times their sum.  NaN and -inf scores are never drawn; where scores are
     +inf, one of them is; a row without any number above -inf gives -1.  Weights and sums have 64
-    bits; the same inputs give the same ids on every run.  Temperatures above 1e28 count as 1e28.
+    bits and are good to 2^-40 of the row's sum (``top_p``'s border, where it keeps thousands of ids of a row of
+    ``2**n``, to ``2**(2 * n - 63)`` at worst); the same inputs give the same ids on every run.  Temperatures
+    above 1e28 count as 1e28, those below 1e-36 as 1e-36.
 
     :param logits: CUDA tensor (rows, width) of float32, bfloat16 or float16; ids contiguous, any row stride.
     :param uniforms: (rows,) float32 or float64 in [0, 1), contiguous, on the same device.

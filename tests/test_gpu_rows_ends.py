@@ -104,3 +104,21 @@ def test_sample_zero_draws_the_first_weight(width, dtype, kw):
         got = _host(povs.sample(y, torch.zeros(rows, device=DEV), temperature=temperature, **kw))
         want = [oracle.sample_row(_host(r), 0.0, temperature=temperature, **kw) for r in y]
         np.testing.assert_array_equal(got, want)
+
+
+@pytest.mark.parametrize("width", [100_003, 1_500_001])
+def test_sample_small_weights_of_a_wide_row(width):
+    """One id of weight 1 before 1499 of weight e^-25, among scores far below: random numbers in the middle of
+    each of the small ones draw it.  Rounded to 2^-51 of the highest, 1499 of them are off by 2^-41 in all, a
+    twentieth of one."""
+    k = 1500
+    g = torch.Generator().manual_seed(1)
+    row = -100.0 - 100.0 * torch.rand(width, generator=g)
+    at = torch.sort(torch.randperm(width - 1, generator=g)[: k - 1] + 1).values
+    row[0], row[at] = 0.0, -25.0
+    picks = torch.arange(0, k - 1, 37)
+    w = math.exp(-25.0)
+    u = (1.0 + (picks.double() + 0.5) * w) / (1.0 + (k - 1) * w)
+    for kw in ({"top_k": k}, {"min_p": 1e-12}):
+        got = povs.sample(row.to(DEV).expand(len(picks), -1), u.to(DEV), **kw).cpu()
+        assert torch.equal(got, at[picks])
