@@ -147,12 +147,13 @@ template <typename T, int EPL> __device__ __noinline__ void route_row_exactly(co
             for (int m = 0; m < EPL; ++m) {
                 const int e = lane + 32 * m;
                 if (e >= g * size && e < (g + 1) * size) {
-                    if (key[m] > first || at == n) {
+                    const uint64_t k = key[m] != 0 ? key[m] : order_key(-INFINITY);
+                    if (k > first || at == n) {
                         second = first;
-                        first = key[m];
+                        first = k;
                         at = e;
-                    } else if (key[m] > second) {
-                        second = key[m];
+                    } else if (k > second) {
+                        second = k;
                     }
                 }
             }
@@ -346,8 +347,10 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, EPL <= 8 ? 8 : EPL <= 16 ? 5
 #pragma unroll
                 for (int i = 0; i < EPL / V; ++i) {
                     float first = c[i * V], second = -INFINITY;
+                    open |= first != first; // minima and maxima would drop a NaN
 #pragma unroll
                     for (int j = 1; j < V; ++j) {
+                        open |= c[i * V + j] != c[i * V + j];
                         second = fmaxf(second, fminf(first, c[i * V + j]));
                         first = fmaxf(first, c[i * V + j]);
                     }
@@ -358,7 +361,6 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, EPL <= 8 ? 8 : EPL <= 16 ? 5
                     }
                     score[i] = p.group_max || size == 1 ? first : first + second;
                     if (expert(i * V) >= n) score[i] = -INFINITY;
-                    open |= score[i] != score[i];
                 }
                 // The best group top_groups times, and once more for the distance to the rest.
                 float last = INFINITY;

@@ -37,6 +37,36 @@ def _same_route(x: torch.Tensor, k: int, **kw) -> None:
     np.testing.assert_array_equal(_host(povs.route(x, k, **kw).experts), experts)
 
 
+# Rows for a warp each, and enough to fill the GPU with lanes.
+FEW_AND_MANY = [300, 9600]
+
+
+@pytest.mark.parametrize("n,groups,top_groups,k,rows", [(64, 8, 4, 6, 300), (96, 32, 9, 4, 300), (512, 16, 3, 10, 300),
+                                                        (64, 8, 4, 12, 9600), (256, 8, 4, 8, 9600)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_route_groups_with_nan_scores(dtype, n, groups, top_groups, k, rows):
+    """A NaN logit ranks below every number of its group, wherever in the group it stands."""
+    x = _randn(rows, n, seed=n, sharp=0.5, dtype=dtype)
+    at = torch.randint(0, n, (rows, 2), generator=torch.Generator().manual_seed(1)).to(DEV)
+    x.scatter_(1, at, float("nan"))
+    _same_route(x, k, scoring="sigmoid", n_groups=groups, top_groups=top_groups)
+
+
+def test_route_groups_with_nan_biases_and_masks():
+    """NaN biases, and groups that masks leave one number or none: those of a number and NaN count no
+    more and no less than those of a number and a masked expert."""
+    n, groups = 64, 16
+    x = _randn(200, n, seed=4, sharp=0.5)
+    bias = torch.zeros(n, device=DEV)
+    bias[::9] = float("nan")
+    _same_route(x, 6, scoring="sigmoid", bias=bias, n_groups=groups, top_groups=5)
+    x[:100, :40] = -float("inf")
+    x[:50, 3::4] = 0.25
+    x[:100, 1::4] = float("nan")
+    _same_route(x, 4, scoring="sigmoid", n_groups=groups, top_groups=10)
+    _same_route(x, 4, scoring="sigmoid", bias=bias, n_groups=groups, top_groups=12, group_score="max")
+
+
 @pytest.mark.parametrize("score", [0.0, 0.3, 0.235038429])
 @pytest.mark.parametrize("width", [131072, 16384])
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
