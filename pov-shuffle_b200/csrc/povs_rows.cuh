@@ -238,6 +238,10 @@ __device__ __forceinline__ float reciprocal_fast(float v)
 }
 constexpr float LOG2E = 1.44269504f;
 
+// Two highest scores of a group that cancel: their errors grow with each of them, not with their sum.  Elsewhere
+// |first| + |second| <= |first + second| + 2.  (A second of -infinity leaves no error.)
+__device__ __forceinline__ bool cancels(float first, float second) { return second < -1.0f && first > 1.0f && second > -INFINITY; }
+
 constexpr int ROUTE_WARPS = 4;
 
 // Choosing in 32 bits what the definition decides in 64.
@@ -250,9 +254,10 @@ constexpr int ROUTE_WARPS = 4;
 // exponential's argument is rounded by 2^-24 of its size z, z 2^-z <= 0.54, the exponential and the quotient
 // are good to 2^-22, a softmax's sum to (EPL + 5) 2^-24: in all below 2^-19 and 2^-24 for each of a lane's
 // scores, to which a bias adds 2^-24 of |c|.  Neighbours in the result no further apart than twice that
-// (`room` steps), and groups whose scores are as close, are told apart by
-// 64 bits (route_row_exactly), unless logit and bias are equal, a tie in either arithmetic.  Rows with
-// NaN, infinities or too few experts end there too, as they reach the lowest step.
+// (`room` steps), and groups whose scores are as close, are told apart by 64 bits (route_row_exactly), unless logit
+// and bias are equal, a tie in either arithmetic.  A group's score has the errors of its two terms, below 2^-18 and
+// 2^-23 for each of a lane's scores, and 2^-24 of |first| + |second| and of their sum: `slack` covers two groups'.
+// Rows with NaN, infinities, terms that cancel or too few experts end there too.
 //
 // A warp per row: 2.3 us for 13 rows of 64 experts, 20 us for 16384 x 256 float32 (0.9 TB/s), 36 us for
 // 16384 x 512 with a bias.  Bound by instructions (about 950 a row with 8 groups, 560 without).
@@ -360,6 +365,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, EPL <= 8 ? 8 : EPL <= 16 ? 5
                         first = fmaxf(first, f);
                     }
                     score[i] = p.group_max || size == 1 ? first : first + second;
+                    open |= !p.group_max && cancels(first, second);
                     if (expert(i * V) >= n) score[i] = -INFINITY;
                 }
                 // The best group top_groups times, and once more for the distance to the rest.
@@ -409,6 +415,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, EPL <= 8 ? 8 : EPL <= 16 ? 5
                     first = fmaxf(first, f);
                 }
                 const float score = p.group_max || size == 1 ? first : first + second;
+                open |= !p.group_max && cancels(first, second);
                 // Groups surely before this one, and groups that may be.
                 const float slack = 8e-6f + 5e-7f * EPL + fabsf(score) * 1e-6f;
                 int sure = 0, maybe = 0;
@@ -672,6 +679,7 @@ __global__ void __launch_bounds__(32, 24) povs_route_lanes_kernel(const __grid_c
             }
             if (GROUPED && (left -= 8) == 0) {
                 group_score[g * ROWS + place] = p.group_max ? first : first + second;
+                open |= !p.group_max && cancels(first, second);
                 group_first[g * ROWS + place] = first;
                 first = second = -INFINITY;
                 left = size;

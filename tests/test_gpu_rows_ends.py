@@ -67,6 +67,16 @@ def test_route_groups_with_nan_biases_and_masks():
     _same_route(x, 4, scoring="sigmoid", bias=bias, n_groups=groups, top_groups=12, group_score="max")
 
 
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("n,groups,top_groups,k,rows", [(64, 32, 9, 6, 2000), (96, 32, 9, 6, 2000), (256, 32, 9, 6, 9600)])
+def test_route_groups_whose_biases_cancel(n, groups, top_groups, k, rows, scoring):
+    """Two highest scores of +600 and -600: each is rounded by 2^-15, while groups' sums lie 10^-5 apart."""
+    x = _randn(rows, n, seed=n, sharp=0.01)
+    bias = torch.full((groups, n // groups), -2000.0, device=DEV)
+    bias[:, 0], bias[:, 1] = 600.0, -600.0
+    _same_route(x, k, scoring=scoring, bias=bias.reshape(-1), n_groups=groups, top_groups=top_groups)
+
+
 @pytest.mark.parametrize("score", [0.0, 0.3, 0.235038429])
 @pytest.mark.parametrize("width", [131072, 16384])
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
