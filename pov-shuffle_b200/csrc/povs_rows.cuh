@@ -242,6 +242,10 @@ constexpr float LOG2E = 1.44269504f;
 // |first| + |second| <= |first + second| + 2.  (A second of -infinity leaves no error.)
 __device__ __forceinline__ bool cancels(float first, float second) { return second < -1.0f && first > 1.0f && second > -INFINITY; }
 
+// Chosen scores that sum to less are divided in 64 bits: 32 bits flush scores below 2^-126 to 0, which above
+// this is 2^-86 of the sum and less.
+constexpr float LEAST_TOTAL = 0x1p-40f;
+
 constexpr int ROUTE_WARPS = 4;
 
 // Choosing in 32 bits what the definition decides in 64.
@@ -511,13 +515,17 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, EPL <= 8 ? 8 : EPL <= 16 ? 5
         }
         float s = 0.0f;
         if (active) s = p.sigmoid ? 1.0f / (1.0f + exp2_fast(logit * -LOG2E)) : exp2_fast((logit - top_logit) * LOG2E) * inv;
-        float w = s * p.scale;
         if (p.renormalize) {
             float total = s;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(FULL_WARP, total, o);
-            w = total == 0.0f ? 0.0f : w / total;
+            if (!(total >= LEAST_TOTAL)) {
+                route_row_exactly<T, EPL>(p, row);
+                continue;
+            }
+            s /= total;
         }
+        const float w = s * p.scale;
         if (active) {
             p.experts[row * p.top_k + lane] = e;
             p.weights[row * p.top_k + lane] = w;
@@ -781,8 +789,8 @@ __global__ void __launch_bounds__(32, 24) povs_route_lanes_kernel(const __grid_c
             chosen[j] = e;
         }
     }
-    float factor = p.scale;
-    if (p.renormalize) factor = total == 0.0f ? 0.0f : factor / total;
+    open |= p.renormalize && !(total >= LEAST_TOTAL);
+    const float part = p.renormalize ? 1.0f / total : 1.0f;
     if (active && !open && share == 0) {
         int32_t* experts = p.experts + row * p.top_k;
         float* weights = p.weights + row * p.top_k;
@@ -790,7 +798,7 @@ __global__ void __launch_bounds__(32, 24) povs_route_lanes_kernel(const __grid_c
         for (int j = 0; j < ROUTE_LIST; ++j)
             if (j < p.top_k) {
                 experts[j] = chosen[j];
-                weights[j] = score[j] * factor;
+                weights[j] = score[j] * part * p.scale;
             }
     }
     for (unsigned rest = __ballot_sync(FULL_WARP, active && open && share == 0); rest != 0; rest &= rest - 1) {

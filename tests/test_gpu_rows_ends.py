@@ -77,6 +77,57 @@ def test_route_groups_whose_biases_cancel(n, groups, top_groups, k, rows, scorin
     _same_route(x, k, scoring=scoring, bias=bias.reshape(-1), n_groups=groups, top_groups=top_groups)
 
 
+def _weight_bound(x: np.ndarray, n: int) -> float:
+    """Relative error of a weight in 32 bits: the exponential's argument, rounded twice relative to its
+    size (a logit, or its difference from the highest), the exponential and the quotients (16 steps), and
+    sums over n scores by one lane and over up to 32 chosen ones."""
+    finite = x[np.isfinite(x)]
+    return (2 * (np.abs(finite).max() + finite.max() - finite.min()) + n + 32 + 16) * U32
+
+
+@pytest.mark.parametrize("rows", FEW_AND_MANY)
+@pytest.mark.parametrize("level", [-27.0, -87.0, -100.0, -300.0])
+@pytest.mark.parametrize("dtype,bias", [(torch.float32, False), (torch.float32, True), (torch.bfloat16, False)], ids=str)
+def test_route_renormalizes_scores_below_32_bits(dtype, bias, level, rows):
+    """Sigmoid scores that 32 bits flush to 0 still have quotients, which sum to the scale.  Where the
+    chosen scores' sum is 2^-40 or more, a flushed score is below 2^-86 of it."""
+    n, k, scale = 64, 6, 16.0
+    x = (_randn(rows, n, seed=5) + level).to(dtype)
+    kw = dict(scoring="sigmoid", renormalize=True, scale=scale)
+    if bias:
+        kw["bias"] = _randn(n, seed=6, sharp=0.1)
+    got = povs.route(x, k, **kw)
+    experts, weights = oracle.route(_host(x), k, **{**kw, "bias": _host(kw["bias"]) if bias else None})
+    np.testing.assert_array_equal(_host(got.experts), experts)
+    np.testing.assert_allclose(_host(got.weights), weights, rtol=_weight_bound(_host(x), n), atol=2.0**-86 * scale)
+    assert np.abs(_host(got.weights).sum(1) / scale - 1).max() < 1e-4
+
+
+@pytest.mark.parametrize("rows", FEW_AND_MANY)
+def test_route_renormalizes_softmax_scores_below_32_bits(rows):
+    """A bias brings experts forward whose softmax scores are e^-100 and less."""
+    n, k = 64, 4
+    x = _randn(rows, n, seed=7)
+    x[:, :8] += 120.0
+    bias = _randn(n, seed=8, sharp=0.1)  # so far apart that 32 bits decide
+    bias[:8] = -3.0
+    got = povs.route(x, k, bias=bias, renormalize=True)
+    experts, weights = oracle.route(_host(x), k, bias=_host(bias), renormalize=True)
+    assert (experts >= 8).all()
+    np.testing.assert_array_equal(_host(got.experts), experts)
+    np.testing.assert_allclose(_host(got.weights), weights, rtol=_weight_bound(_host(x), n))
+
+
+def test_route_scales_of_any_size():
+    """Renormalised weights are quotients times the scale, also where score times scale or scale by sum would
+    leave 32 bits."""
+    x = _randn(200, 32, seed=8) - 20.0
+    for scale in (1e-30, 1e36):
+        got = povs.route(x, 4, scoring="sigmoid", renormalize=True, scale=scale)
+        _, weights = oracle.route(_host(x), 4, scoring="sigmoid", renormalize=True, scale=scale)
+        np.testing.assert_allclose(_host(got.weights), weights, rtol=_weight_bound(_host(x), 32))
+
+
 @pytest.mark.parametrize("score", [0.0, 0.3, 0.235038429])
 @pytest.mark.parametrize("width", [131072, 16384])
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
