@@ -812,7 +812,7 @@ __global__ void __launch_bounds__(32, 24) povs_route_lanes_kernel(const __grid_c
 // chosen scores, S their sum (1 without renormalisation) and g the weights' gradient:
 //   df_j = scale (g_j - sum_i g_i f_i / S [renormalised]) / S
 //   softmax: dx_i = s_i (df_i - sum_j f_j df_j);  sigmoid: dx_i = s_i (1 - s_i) df_i
-// (df is 0 outside the chosen experts).  The logits are read twice, the second time from cache.
+// (df is 0 outside the chosen experts).  The logits are read up to three times, all but the first from cache.
 template <typename T>
 __global__ void __launch_bounds__(128) povs_route_backward_kernel(const __grid_constant__ RouteParams p)
 {
@@ -849,19 +849,25 @@ __global__ void __launch_bounds__(128) povs_route_backward_kernel(const __grid_c
         for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(FULL_WARP, a, o);
         return a;
     };
-    float df = g * p.scale;
+    float df = g * p.scale, mine, common = 0.0f;
     if (p.renormalize) {
-        const float total = warp_sum(f);
-        const float w = total == 0.0f ? 0.0f : f / total;
-        const float mean = warp_sum(g * w);
-        df = e < 0 || total == 0.0f ? 0.0f : (g - mean) * p.scale / total;
-    }
-    float mine, common = 0.0f;
-    if (p.sigmoid) {
+        // Quotients of the scores over a common factor, the highest chosen one's, so that none is lost where 32 bits
+        // flush the scores themselves to 0.  They do not depend on that factor: common is 0 exactly.
+        float most = e < 0 ? -INFINITY : v;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(FULL_WARP, most, o));
+        if (most == -INFINITY || (p.sigmoid && most > 0.0f)) most = 0.0f;
+        const float part = e < 0 ? 0.0f : !p.sigmoid ? expf(v - most) : v > 0.0f ? f : expf(v - most) / (1.0f + expf(v));
+        const float total = warp_sum(part);
+        const float w = total == 0.0f ? 0.0f : part / total;
+        const float mean = warp_sum(df * w);
+        mine = w * (df - mean);
+        if (p.sigmoid) mine *= 1.0f - f;
+        else if (inv != inv) mine = inv; // a row with NaN or +infinity has no scores
+    } else if (p.sigmoid) {
         mine = f * (1.0f - f) * df;
     } else {
-        // Renormalised weights do not depend on a common factor of the scores: the sum is 0 exactly.
-        common = p.renormalize ? 0.0f : warp_sum(f * df);
+        common = warp_sum(f * df);
         mine = f * (df - common);
     }
     for (int i = lane; i < n; i += 32) {

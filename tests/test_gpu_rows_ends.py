@@ -128,6 +128,76 @@ def test_route_scales_of_any_size():
         np.testing.assert_allclose(_host(got.weights), weights, rtol=_weight_bound(_host(x), 32))
 
 
+def _gradient(x, experts, g, scoring, renormalize, scale):
+    """(gradient of the logits, the size of the terms whose sum each of its numbers is), in 64 bits.
+
+    With f the scores, w the weights before scaling and j a chosen expert, without a difference of large
+    numbers: dx_j = f_j (g_j U + sum_i f_i (g_j - g_i)) for a softmax, U the scores of those not chosen (0
+    for quotients); dx_j = f_j (1 - f_j) g_j for a sigmoid, w_j (1 - f_j) sum_i w_i (g_j - g_i) for its
+    quotients; dx_i = -s_i sum_j f_j g_j elsewhere in a softmax's row."""
+    x, g = x.astype(np.float64), g.astype(np.float64)
+    out, size = np.zeros_like(x), np.zeros_like(x)
+    for r in range(len(x)):
+        e = experts[r][experts[r] >= 0]
+        up = g[r][experts[r] >= 0] * scale
+        if scoring == "softmax":
+            s = np.exp(x[r] - x[r].max())
+            s /= s.sum()
+            other = np.delete(s, e).sum()
+        else:
+            s, complement = 1 / (1 + np.exp(-x[r])), 1 / (1 + np.exp(x[r]))
+        f = s[e]
+        w = f / f.sum() if renormalize else f
+        apart = up[:, None] - up[None, :]
+        if renormalize:
+            d, m = w * (apart @ w), w * (np.abs(apart) @ w)
+            if scoring == "sigmoid":
+                d, m = d * complement[e], m * complement[e]
+        elif scoring == "softmax":
+            out[r], size[r] = -s * (f * up).sum(), s * (f * np.abs(up)).sum()
+            d, m = f * (up * other + apart @ f), f * (np.abs(up) * other + np.abs(apart) @ f)
+        else:
+            d = f * complement[e] * up
+            m = np.abs(d)
+        out[r, e], size[r, e] = d, m
+    return out, size
+
+
+def _gradient_bound(size, want, dtype, x, n):
+    """One rounding to the type; in 32 bits each term is a product of up to three scores or weights (each
+    with a weight's error) and a difference, summed over up to 32 chosen ones."""
+    tiny = {torch.float32: 2.0**-126, torch.bfloat16: 2.0**-126, torch.float16: 2.0**-24}[dtype]
+    return torch.finfo(dtype).eps / 2 * np.abs(want) + (3 * _weight_bound(x, n) + 40 * U32) * size + tiny
+
+
+def _check_gradient(x, k, seed, **kw):
+    x = x.detach().requires_grad_()
+    experts, weights = povs.route(x, k, **kw)
+    g = _randn(*weights.shape, seed=seed)
+    (dx,) = torch.autograd.grad(weights, x, g)
+    want, size = _gradient(_host(x), _host(experts), _host(g), kw.get("scoring", "softmax"),
+                           kw.get("renormalize", False), kw.get("scale", 1.0))
+    assert (np.abs(_host(dx) - want) <= _gradient_bound(size, want, x.dtype, _host(x), x.shape[1])).all()
+    return dx
+
+
+@pytest.mark.parametrize("level", [-10.0, -87.0, -100.0, -300.0])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_route_gradient_of_scores_below_32_bits(dtype, level):
+    x = (_randn(60, 40, seed=9) + level).to(dtype)
+    dx = _check_gradient(x, 5, seed=1, scoring="sigmoid", renormalize=True, scale=2.5)
+    assert ((dx != 0).sum(1) >= 4).all()
+
+
+def test_route_gradient_of_softmax_scores_below_32_bits():
+    x = _randn(60, 40, seed=10)
+    x[:, :8] += 120.0
+    bias = torch.zeros(40, device=DEV)
+    bias[:8] = -3.0
+    dx = _check_gradient(x, 5, seed=2, bias=bias, renormalize=True)
+    assert ((dx != 0).sum(1) >= 4).all()
+
+
 @pytest.mark.parametrize("score", [0.0, 0.3, 0.235038429])
 @pytest.mark.parametrize("width", [131072, 16384])
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
