@@ -198,6 +198,26 @@ def test_route_gradient_of_softmax_scores_below_32_bits():
     assert ((dx != 0).sum(1) >= 4).all()
 
 
+@pytest.mark.parametrize("renormalize", [False, True])
+@pytest.mark.parametrize("level", [10.0, 17.0, 30.0])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16], ids=str)
+def test_route_gradient_of_sigmoid_scores_near_one(dtype, level, renormalize):
+    """The factor 1 - s keeps its relative accuracy where s is rounded to 1."""
+    x = (_randn(60, 40, seed=11) + level).to(dtype)
+    _check_gradient(x, 5, seed=3, scoring="sigmoid", renormalize=renormalize)
+
+
+@pytest.mark.parametrize("renormalize", [False, True])
+@pytest.mark.parametrize("k", [1, 8])
+@pytest.mark.parametrize("level", [5.0, 40.0])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_route_gradient_of_softmax_scores_near_one(dtype, level, k, renormalize):
+    """One expert far above the rest: its gradient is a small difference, and is summed without one."""
+    x = _randn(60, 48, seed=12)
+    x[torch.arange(60), torch.arange(60) % 48] += level
+    _check_gradient(x.to(dtype), k, seed=4, renormalize=renormalize)
+
+
 @pytest.mark.parametrize("score", [0.0, 0.3, 0.235038429])
 @pytest.mark.parametrize("width", [131072, 16384])
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
