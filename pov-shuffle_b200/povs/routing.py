@@ -4,7 +4,7 @@
 the rows of an expert together, ``dispatch_rows`` moves rows into that order and ``combine_rows`` sums
 them back, weighted.  As in the shuffle, a row is one instance: everything behind axis 0.  All run
 on the tensors' current stream, give the same result on every run, and have gradients (of first
-order).  All can be captured into CUDA graphs; as for any PyTorch backward pass, capture one with
+order, by backward passes: tangents of forward-mode differentiation are refused).  All can be captured into CUDA graphs; as for any PyTorch backward pass, capture one with
 leaves of its own, not those of an eager graph that is still alive.
 """
 
@@ -14,6 +14,7 @@ import math
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 
@@ -90,6 +91,7 @@ def route(
         if not isinstance(bias, torch.Tensor) or bias.device != logits.device or bias.dtype != torch.float32:
             raise TypeError(f"bias must be a float32 tensor on the device of logits ({logits.device})")
         assert bias.shape == (n,) and bias.is_contiguous(), f"bias must be contiguous with shape ({n},), got {tuple(bias.shape)}"
+    _no_tangents(logits)
     spec = (int(top_k), SCORINGS[scoring], int(n_groups), int(top_groups), GROUP_SCORES[group_score], bool(renormalize),
             float(scale))
     if logits.requires_grad and torch.is_grad_enabled():
@@ -142,6 +144,7 @@ def dispatch_rows(data: torch.Tensor, plan: RowPlan) -> torch.Tensor:
     """
     _check_moved(data, plan, "dispatch_rows")
     assert data.shape[0] == plan.slots.shape[0], f"data has {data.shape[0]} rows, the plan {plan.slots.shape[0]}"
+    _no_tangents(data)
     if data.requires_grad and torch.is_grad_enabled():
         _native.score_dtype(data)
         return _Dispatch.apply(data, plan.slots, plan.offsets)
@@ -180,6 +183,7 @@ def combine_rows(data: torch.Tensor, plan: RowPlan, weights: torch.Tensor | None
             raise TypeError(f"weights must be a float32 tensor on the device of data ({data.device})")
         assert weights.shape == slots.shape, f"weights must have shape {tuple(slots.shape)}, got {tuple(weights.shape)}"
         assert weights.is_contiguous(), "weights must be contiguous"
+    _no_tangents(data, weights)
     if torch.is_grad_enabled() and (data.requires_grad or (weights is not None and weights.requires_grad)):
         return _Combine.apply(data, weights, slots, plan.offsets)
     return _native.combine_rows(data, slots, weights)
@@ -204,6 +208,14 @@ def _first_order() -> None:
     pass runs with gradients enabled."""
     if torch.is_grad_enabled():
         raise RuntimeError("povs gradients are once differentiable: call backward without create_graph=True")
+
+
+def _no_tangents(*tensors: torch.Tensor | None) -> None:
+    """Refuse dual tensors: the kernels would return their outputs without a tangent."""
+    if forward_ad._current_level >= 0:  # inside a dual_level
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("povs gradients are for backward passes: forward-mode differentiation is not supported")
 
 
 def _check_moved(data: torch.Tensor, plan: RowPlan, what: str) -> None:

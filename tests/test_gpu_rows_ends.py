@@ -303,3 +303,20 @@ def test_sample_small_weights_of_a_wide_row(width):
     for kw in ({"top_k": k}, {"min_p": 1e-12}):
         got = povs.sample(row.to(DEV).expand(len(picks), -1), u.to(DEV), **kw).cpu()
         assert torch.equal(got, at[picks])
+
+
+def test_forward_mode_differentiation_is_refused():
+    """A tangent is refused, as a second-order gradient is, and not dropped."""
+    plan = povs.plan_rows(torch.zeros(4, 2, dtype=torch.int32, device=DEV), 3)
+    x, y, w = _randn(4, 8, seed=1), _randn(8, 5, seed=2), torch.rand(4, 2, device=DEV)
+    with torch.autograd.forward_ad.dual_level():
+        def dual(t):
+            return torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: povs.route(dual(x), 2), lambda: povs.dispatch_rows(dual(x), plan),
+                     lambda: povs.combine_rows(dual(y), plan), lambda: povs.combine_rows(y, plan, dual(w)),
+                     lambda: povs.route(dual(x).requires_grad_(), 2)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        assert torch.equal(povs.combine_rows(y, plan, w), povs.combine_rows(y.clone(), plan, w))
+        assert povs.route(x, 2).weights.shape == (4, 2)
