@@ -435,19 +435,22 @@ def combine_rows(data: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor 
     return out
 
 
-def combine_backward(grad: torch.Tensor, data: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor | None,
+def combine_backward(grad: torch.Tensor, data: torch.Tensor | None, slots: torch.Tensor, weights: torch.Tensor | None,
                      offsets: torch.Tensor, need_data: bool, need_weights: bool):
-    """``povs_combine_backward_v1``: the gradients of ``data`` and ``weights`` (None where not needed)."""
+    """``povs_combine_backward_v1``: the gradients of ``data`` and ``weights`` (None where not needed; ``data`` is
+    read for the weights' alone)."""
     dev = grad.device
     rows, k = slots.shape
-    grad_data = data.new_empty(data.shape) if need_data else None
-    grad_weights = data.new_empty((rows, k), dtype=torch.float32) if need_weights else None
+    n, width = rows * k, _row_elements(grad)
+    grad_data = grad.new_empty((n, *grad.shape[1:])) if need_data else None
+    grad_weights = grad.new_empty((rows, k), dtype=torch.float32) if need_weights else None
     check(
         load().povs_combine_backward_v1(
-            grad.data_ptr(), data.data_ptr(), _SCORE_DTYPES[data.dtype], data.shape[0], _row_elements(data),
-            data.stride(0), slots.data_ptr(), rows, k, None if weights is None else weights.data_ptr(),
-            offsets.data_ptr() + 4 * (offsets.numel() - 1), None if grad_data is None else grad_data.data_ptr(),
-            None if grad_weights is None else grad_weights.data_ptr(), dev.index, current_stream_handle(dev),
+            grad.data_ptr(), data.data_ptr() if need_weights else None, _SCORE_DTYPES[grad.dtype], n, width,
+            data.stride(0) if need_weights else width, slots.data_ptr(), rows, k,
+            None if weights is None else weights.data_ptr(), offsets.data_ptr() + 4 * (offsets.numel() - 1),
+            None if grad_data is None else grad_data.data_ptr(), None if grad_weights is None else grad_weights.data_ptr(),
+            dev.index, current_stream_handle(dev),
         ),
         "povs_combine_backward_v1",
     )

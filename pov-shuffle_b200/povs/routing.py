@@ -192,7 +192,8 @@ def combine_rows(data: torch.Tensor, plan: RowPlan, weights: torch.Tensor | None
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, data, weights, slots, offsets):
-        ctx.save_for_backward(data, weights, slots, offsets)
+        # The rows are read again for the weights' gradient alone.
+        ctx.save_for_backward(data if ctx.needs_input_grad[1] else None, weights, slots, offsets)
         return _native.combine_rows(data, slots, weights)
 
     @staticmethod

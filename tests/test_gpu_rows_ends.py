@@ -320,3 +320,21 @@ def test_forward_mode_differentiation_is_refused():
                 call()
         assert torch.equal(povs.combine_rows(y, plan, w), povs.combine_rows(y.clone(), plan, w))
         assert povs.route(x, 2).weights.shape == (4, 2)
+
+
+def test_combine_keeps_rows_for_the_weights_gradient_alone():
+    plan = povs.plan_rows(torch.randint(0, 3, (16, 2), device=DEV), 3)
+    y = _randn(32, 5, seed=1).requires_grad_()
+    w = torch.rand(16, 2, device=DEV)
+    for weights, kept in ((None, False), (w, False), (w.clone().requires_grad_(), True)):
+        rows = y * 1.0
+        out = povs.combine_rows(rows, plan, weights)
+        assert any(t is not None and t.shape == y.shape for t in out.grad_fn.saved_tensors) == kept
+        if not kept:
+            rows.detach().add_(1.0)  # so it may change before the backward pass
+        up = _randn(16, 5, seed=2)
+        (dy,) = torch.autograd.grad(out, y, up)
+        want = torch.zeros(32, 5, device=DEV)
+        share = torch.ones(16, 2, device=DEV) if weights is None else weights.detach()
+        want[plan.slots.long().reshape(-1)] = (share.unsqueeze(2) * up.unsqueeze(1)).reshape(32, 5)
+        assert torch.equal(dy, want)
