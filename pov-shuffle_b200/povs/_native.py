@@ -321,6 +321,11 @@ def score_dtype(t: torch.Tensor) -> int:
     return code
 
 
+def plain(t: torch.Tensor) -> torch.Tensor:
+    """The tensor, or a copy where its numbers are not its bytes (a lazy conjugate or negative)."""
+    return t.resolve_conj().resolve_neg() if t.is_conj() or t.is_neg() else t
+
+
 def _row_elements(data: torch.Tensor) -> int:
     n = 1
     for d in data.shape[1:]:

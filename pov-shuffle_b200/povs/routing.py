@@ -75,6 +75,7 @@ def route(
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise TypeError("route takes a CUDA tensor of logits")
     _native.score_dtype(logits)
+    logits = _native.plain(logits)
     assert logits.dim() == 2, f"logits must have shape (rows, n_experts), got {tuple(logits.shape)}"
     n = logits.shape[1]
     assert 1 <= n <= _native.MAX_ROUTE_EXPERTS, f"number of experts ({n}) must be in [1, {_native.MAX_ROUTE_EXPERTS}]"
@@ -90,6 +91,7 @@ def route(
     if bias is not None:
         if not isinstance(bias, torch.Tensor) or bias.device != logits.device or bias.dtype != torch.float32:
             raise TypeError(f"bias must be a float32 tensor on the device of logits ({logits.device})")
+        bias = _native.plain(bias)
         assert bias.shape == (n,) and bias.is_contiguous(), f"bias must be contiguous with shape ({n},), got {tuple(bias.shape)}"
     _no_tangents(logits)
     spec = (int(top_k), SCORINGS[scoring], int(n_groups), int(top_groups), GROUP_SCORES[group_score], bool(renormalize),
@@ -116,7 +118,7 @@ class _Route(torch.autograd.Function):
             return None, None, None
         logits, experts = ctx.saved_tensors
         top_k, scoring, _, _, _, renormalize, scale = ctx.spec
-        return _native.route_backward(logits, experts, grad_weights.contiguous(), scoring, renormalize, scale), None, None
+        return _native.route_backward(logits, experts, _native.plain(grad_weights).contiguous(), scoring, renormalize, scale), None, None
 
 
 def plan_rows(experts: torch.Tensor, n_experts: int) -> RowPlan:
@@ -142,7 +144,7 @@ def dispatch_rows(data: torch.Tensor, plan: RowPlan) -> torch.Tensor:
     :param data: CUDA tensor (rows, ...) of any dtype (rows are moved as bytes; a gradient needs float32,
         bfloat16 or float16).  Each row is contiguous; any row stride.
     """
-    _check_moved(data, plan, "dispatch_rows")
+    data = _check_moved(data, plan, "dispatch_rows")
     assert data.shape[0] == plan.slots.shape[0], f"data has {data.shape[0]} rows, the plan {plan.slots.shape[0]}"
     _no_tangents(data)
     if data.requires_grad and torch.is_grad_enabled():
@@ -161,7 +163,7 @@ class _Dispatch(torch.autograd.Function):
     def backward(ctx, grad):
         _first_order()
         (slots,) = ctx.saved_tensors
-        return _native.combine_rows(grad.contiguous(), slots, None), None, None
+        return _native.combine_rows(_native.plain(grad).contiguous(), slots, None), None, None
 
 
 def combine_rows(data: torch.Tensor, plan: RowPlan, weights: torch.Tensor | None = None) -> torch.Tensor:
@@ -174,13 +176,14 @@ def combine_rows(data: torch.Tensor, plan: RowPlan, weights: torch.Tensor | None
         row is contiguous; any row stride.
     :param weights: float32 (rows, top_k), contiguous, on the same device; None sums without weights.
     """
-    _check_moved(data, plan, "combine_rows")
+    data = _check_moved(data, plan, "combine_rows")
     _native.score_dtype(data)
     slots = plan.slots
     assert data.shape[0] == slots.numel(), f"data has {data.shape[0]} rows, the plan {slots.numel()} places"
     if weights is not None:
         if not isinstance(weights, torch.Tensor) or weights.device != data.device or weights.dtype != torch.float32:
             raise TypeError(f"weights must be a float32 tensor on the device of data ({data.device})")
+        weights = _native.plain(weights)
         assert weights.shape == slots.shape, f"weights must have shape {tuple(slots.shape)}, got {tuple(weights.shape)}"
         assert weights.is_contiguous(), "weights must be contiguous"
     _no_tangents(data, weights)
@@ -200,7 +203,7 @@ class _Combine(torch.autograd.Function):
     def backward(ctx, grad):
         _first_order()
         data, weights, slots, offsets = ctx.saved_tensors
-        return (*_native.combine_backward(grad.contiguous(), data, slots, weights, offsets, *ctx.needs_input_grad[:2]),
+        return (*_native.combine_backward(_native.plain(grad).contiguous(), data, slots, weights, offsets, *ctx.needs_input_grad[:2]),
                 None, None)
 
 
@@ -219,9 +222,10 @@ def _no_tangents(*tensors: torch.Tensor | None) -> None:
                 raise RuntimeError("povs gradients are for backward passes: forward-mode differentiation is not supported")
 
 
-def _check_moved(data: torch.Tensor, plan: RowPlan, what: str) -> None:
+def _check_moved(data: torch.Tensor, plan: RowPlan, what: str) -> torch.Tensor:
     if not isinstance(data, torch.Tensor) or not data.is_cuda:
         raise TypeError(f"{what} takes a CUDA tensor of rows")
+    data = _native.plain(data)
     assert data.dim() >= 1, f"data must have at least one dimension, but has {data.dim()}"
     assert data.is_contiguous() or data[:1].is_contiguous(), "rows of data must be contiguous"
     slots, offsets = plan.slots, plan.offsets
@@ -230,3 +234,4 @@ def _check_moved(data: torch.Tensor, plan: RowPlan, what: str) -> None:
     assert slots.is_contiguous() and offsets.is_contiguous(), "plan.slots and plan.offsets must be contiguous"
     assert slots.dim() == 2 and slots.shape[1] >= 1, f"plan.slots must have shape (rows, top_k), got {tuple(slots.shape)}"
     assert offsets.dim() == 1 and offsets.numel() >= 2, "plan.offsets must have shape (n_experts + 1,)"
+    return data

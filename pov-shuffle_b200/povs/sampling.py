@@ -47,15 +47,17 @@ def sample(
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise TypeError("sample takes a CUDA tensor of scores")
     _native.score_dtype(logits)
+    logits = _native.plain(logits)
     assert logits.dim() == 2, f"logits must have shape (rows, width), got {tuple(logits.shape)}"
     rows, width = logits.shape
     assert width >= 1, "logits must have at least one id per row"
     assert width == 1 or logits.stride(1) == 1, "ids of a row must be contiguous"
-    _check_per_row("uniforms", uniforms, logits, (torch.float32, torch.float64))
+    uniforms = _per_row("uniforms", uniforms, logits, (torch.float32, torch.float64))
     given = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
     for name, value in given.items():
         if isinstance(value, torch.Tensor):
-            _check_per_row(name, value, logits, (torch.int32 if name == "top_k" else torch.float32,))
+            given[name] = _per_row(name, value, logits, (torch.int32 if name == "top_k" else torch.float32,))
+    temperature, top_k, top_p, min_p = given.values()
     if not isinstance(temperature, torch.Tensor):
         assert temperature >= 0 and math.isfinite(temperature), f"temperature ({temperature}) must be finite and at least 0"
     if not isinstance(top_k, torch.Tensor):
@@ -68,10 +70,11 @@ def sample(
     return _native.sample(logits, uniforms, temperature, top_k, top_p, min_p)
 
 
-def _check_per_row(name: str, value: torch.Tensor, logits: torch.Tensor, dtypes: tuple) -> None:
+def _per_row(name: str, value: torch.Tensor, logits: torch.Tensor, dtypes: tuple) -> torch.Tensor:
     if not isinstance(value, torch.Tensor) or value.device != logits.device:
         raise TypeError(f"{name} must be a tensor on the device of logits ({logits.device})")
     if value.dtype not in dtypes:
         raise TypeError(f"{name} must have dtype {' or '.join(map(str, dtypes))}, got {value.dtype}")
     assert value.shape == (logits.shape[0],), f"{name} must have shape ({logits.shape[0]},), got {tuple(value.shape)}"
     assert value.is_contiguous(), f"{name} must be contiguous"
+    return _native.plain(value)

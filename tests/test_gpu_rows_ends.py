@@ -338,3 +338,25 @@ def test_combine_keeps_rows_for_the_weights_gradient_alone():
         share = torch.ones(16, 2, device=DEV) if weights is None else weights.detach()
         want[plan.slots.long().reshape(-1)] = (share.unsqueeze(2) * up.unsqueeze(1)).reshape(32, 5)
         assert torch.equal(dy, want)
+
+
+def test_rows_of_lazily_conjugated_and_negated_tensors():
+    """A conjugate or an imaginary part of one is a view whose numbers differ from its bytes."""
+    plan = povs.plan_rows(torch.tensor([[1], [0], [1]], dtype=torch.int32, device=DEV), 2)
+    z = torch.complex(_randn(3, 4, seed=1), _randn(3, 4, seed=2)).conj()
+    assert z.is_conj()
+    order = [1, 0, 2]
+    assert torch.equal(povs.dispatch_rows(z, plan), z.resolve_conj()[order])
+    line = z.imag[:, 0]
+    assert line.is_neg()
+    assert torch.equal(povs.dispatch_rows(line, plan), line.resolve_neg()[order])
+    back = [1, 0, 2]
+    assert torch.equal(povs.combine_rows(line, plan), line.resolve_neg()[back])
+    column = z.imag[:, :1]
+    u = torch.tensor([0.1, 0.2, 0.3], device=DEV)
+    assert torch.equal(povs.route(column, 1).weights, torch.ones(3, 1, device=DEV))
+    assert torch.equal(povs.route(column, 1, scoring="sigmoid").weights,
+                       povs.route(column.resolve_neg(), 1, scoring="sigmoid").weights)
+    flat = torch._neg_view(_randn(3, 50, seed=3))
+    assert torch.equal(povs.sample(flat, u, top_k=1), povs.sample(flat.resolve_neg(), u, top_k=1))
+    assert torch.equal(povs.route(flat, 3).experts, povs.route(flat.resolve_neg(), 3).experts)
