@@ -546,6 +546,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, EPL <= 8 ? 8 : EPL <= 16 ? 5
 // bound of 80 registers that lets 24 warps in, 63), 32 us by the logits alone; 32749 x 128 bfloat16 in 11 us (a
 // warp per row: 17).  Bound by instructions (530 a row with groups).
 constexpr int ROUTE_LIST = 8;
+constexpr int ROUTE_LANES_EXPERTS = 256; // at most
 
 __device__ __forceinline__ void exchange(uint32_t& a, uint32_t& b)
 {
@@ -801,11 +802,8 @@ __global__ void __launch_bounds__(32, 24) povs_route_lanes_kernel(const __grid_c
                 weights[j] = score[j] * part * p.scale;
             }
     }
-    for (unsigned rest = __ballot_sync(FULL_WARP, active && open && share == 0); rest != 0; rest &= rest - 1) {
-        const int64_t r = first_row + __ffs(rest) - 1;
-        if (n <= 256) route_row_exactly<T, 8>(p, r);
-        else route_row_exactly<T, 16>(p, r);
-    }
+    for (unsigned rest = __ballot_sync(FULL_WARP, active && open && share == 0); rest != 0; rest &= rest - 1)
+        route_row_exactly<T, ROUTE_LANES_EXPERTS / 32>(p, first_row + __ffs(rest) - 1);
 }
 
 // Gradient of the weights with respect to the scores' logits, one warp per row.  With f_j the
@@ -948,7 +946,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) povs_plan_count_kernel(const __g
 // blocks before, of the warps before and of the lanes before with the same expert.  Each warp takes
 // a contiguous run of the block's chunk, so the order within an expert is the entries' order
 // whatever the timing.  3 us for up to 4096 entries (one block, one launch); 12 us for 131072 entries and 256
-// experts (64 blocks), most of it the latency of two launches and of reading the blocks' counts.  `warps` warps count (each holds a row of n_experts counters).
+// experts (64 blocks), most of it the latency of two launches and of reading the blocks' counts.  `warps` warps
+// count (each holds a row of n_experts counters).
 __global__ void __launch_bounds__(PLAN_THREADS) povs_plan_place_kernel(const __grid_constant__ PlanRowsParams p, int warps)
 {
     extern __shared__ int32_t smem[];

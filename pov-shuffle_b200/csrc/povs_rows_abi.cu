@@ -125,23 +125,22 @@ template <typename T, int EPL> void launch_route_of(const povs::RouteParams& p, 
     else povs::povs_route_kernel<T, EPL, false><<<grid, 32 * povs::ROUTE_WARPS, 0, s>>>(p);
 }
 
-template <typename T, int L, bool SIGMOID, bool BY_LOGIT, bool GROUPED> int launch_route_lanes(const povs::RouteParams& p, cudaStream_t s)
+// Up to 41 KB of shared memory (248 experts in 31 groups, float32).
+template <typename T, int L, bool SIGMOID, bool BY_LOGIT, bool GROUPED> void launch_route_lanes(const povs::RouteParams& p, cudaStream_t s)
 {
     constexpr int ROWS = 32 / L;
     const int floats = (BY_LOGIT ? 0 : p.n_experts) + (GROUPED ? 2 * ROWS * p.n_groups : 0);
     const int smem = ROWS * povs::route_pitch(p.n_experts * static_cast<int>(sizeof(T))) + 4 * floats;
-    auto* kernel = povs::povs_route_lanes_kernel<T, L, SIGMOID, BY_LOGIT, GROUPED>;
-    if (smem > 48 * 1024) POVS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    kernel<<<static_cast<unsigned>((p.rows + ROWS - 1) / ROWS), 32, smem, s>>>(p);
-    return POVS_OK;
+    povs::povs_route_lanes_kernel<T, L, SIGMOID, BY_LOGIT, GROUPED>
+        <<<static_cast<unsigned>((p.rows + ROWS - 1) / ROWS), 32, smem, s>>>(p);
 }
 
-template <typename T, int L> int launch_route_lanes_of(const povs::RouteParams& p, cudaStream_t s)
+template <typename T, int L> void launch_route_lanes_of(const povs::RouteParams& p, cudaStream_t s)
 {
     const bool grouped = p.top_groups < p.n_groups, by_logit = p.bias == nullptr && !grouped;
-    if (by_logit) return p.sigmoid ? launch_route_lanes<T, L, true, true, false>(p, s) : launch_route_lanes<T, L, false, true, false>(p, s);
-    if (grouped) return p.sigmoid ? launch_route_lanes<T, L, true, false, true>(p, s) : launch_route_lanes<T, L, false, false, true>(p, s);
-    return p.sigmoid ? launch_route_lanes<T, L, true, false, false>(p, s) : launch_route_lanes<T, L, false, false, false>(p, s);
+    if (by_logit) p.sigmoid ? launch_route_lanes<T, L, true, true, false>(p, s) : launch_route_lanes<T, L, false, true, false>(p, s);
+    else if (grouped) p.sigmoid ? launch_route_lanes<T, L, true, false, true>(p, s) : launch_route_lanes<T, L, false, false, true>(p, s);
+    else p.sigmoid ? launch_route_lanes<T, L, true, false, false>(p, s) : launch_route_lanes<T, L, false, false, false>(p, s);
 }
 
 // Lanes per row: as many (1, 2, 4 or 8) as bring a warp's rows below 9 KB, in whole pieces of experts and groups.
@@ -159,12 +158,12 @@ int route_lanes(const povs::RouteParams& p, int element)
 // 16384 x 256 13 against 20, but 8192 x 256 20 against 14 and 16384 x 512 58 against 36.
 bool route_by_lanes(const povs::RouteParams& p, int element, int sms)
 {
-    return p.rows >= 64 * static_cast<int64_t>(sms) && p.top_k <= povs::ROUTE_LIST && p.n_experts <= 256 && p.n_experts % 8 == 0 &&
+    return p.rows >= 64 * static_cast<int64_t>(sms) && p.top_k <= povs::ROUTE_LIST && p.n_experts <= povs::ROUTE_LANES_EXPERTS && p.n_experts % 8 == 0 &&
            (p.top_groups == p.n_groups || p.n_experts / p.n_groups % 8 == 0) && p.n_experts * element % 16 == 0 &&
            p.row_stride * element % 16 == 0 && address(p.logits) % 16 == 0;
 }
 
-template <typename T> int launch_route(const povs::RouteParams& p, int sms, cudaStream_t s)
+template <typename T> void launch_route(const povs::RouteParams& p, int sms, cudaStream_t s)
 {
     if (route_by_lanes(p, sizeof(T), sms)) {
         switch (route_lanes(p, sizeof(T))) {
@@ -181,7 +180,6 @@ template <typename T> int launch_route(const povs::RouteParams& p, int sms, cuda
     else if (epl <= 8) launch_route_of<T, 8>(p, sms, s);
     else if (epl <= 16) launch_route_of<T, 16>(p, sms, s);
     else launch_route_of<T, 32>(p, sms, s);
-    return POVS_OK;
 }
 
 int check_rows(int64_t rows, int32_t top_k, int64_t n_slots)
@@ -387,10 +385,10 @@ extern "C" int povs_route_v1(const void* logits, int32_t dtype, int64_t rows, in
     r = enter(dg, device, &sms);
     if (r != POVS_OK) return r;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (dtype == POVS_FLOAT32) r = launch_route<float>(p, sms, s);
-    else if (dtype == POVS_BFLOAT16) r = launch_route<__nv_bfloat16>(p, sms, s);
-    else r = launch_route<__half>(p, sms, s);
-    return r == POVS_OK ? launched("route kernel") : r;
+    if (dtype == POVS_FLOAT32) launch_route<float>(p, sms, s);
+    else if (dtype == POVS_BFLOAT16) launch_route<__nv_bfloat16>(p, sms, s);
+    else launch_route<__half>(p, sms, s);
+    return launched("route kernel");
 }
 
 extern "C" int povs_route_backward_v1(const void* logits, int32_t dtype, int64_t rows, int32_t n_experts,

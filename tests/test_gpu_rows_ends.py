@@ -360,3 +360,20 @@ def test_rows_of_lazily_conjugated_and_negated_tensors():
     flat = torch._neg_view(_randn(3, 50, seed=3))
     assert torch.equal(povs.sample(flat, u, top_k=1), povs.sample(flat.resolve_neg(), u, top_k=1))
     assert torch.equal(povs.route(flat, 3).experts, povs.route(flat.resolve_neg(), 3).experts)
+
+
+@pytest.mark.parametrize("n,groups,top_groups,k", [(248, 31, 9, 8), (240, 30, 4, 8), (240, 3, 2, 5), (8, 1, 1, 8),
+                                                   (256, 32, 8, 8), (200, 1, 1, 3)])
+@pytest.mark.parametrize("scoring,bias", [("softmax", False), ("sigmoid", True)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_route_of_many_rows_of_every_shape_of_the_tile(dtype, scoring, bias, n, groups, top_groups, k):
+    """Rows that one lane, or two to eight, walk, up to the largest tile of shared memory."""
+    rows = 9477
+    x = _randn(rows, n, seed=n, sharp=1.5, dtype=dtype)
+    kw = dict(scoring=scoring, n_groups=groups, top_groups=top_groups)
+    if bias:
+        kw["bias"] = _randn(n, seed=1, sharp=0.1)
+    got = povs.route(x, k, **kw)
+    experts, weights = oracle.route(_host(x), k, **{**kw, "bias": _host(kw["bias"]) if bias else None})
+    np.testing.assert_array_equal(_host(got.experts), experts)
+    np.testing.assert_allclose(_host(got.weights), weights, rtol=_weight_bound(_host(x), n), atol=1e-37)
