@@ -509,23 +509,19 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, EPL <= 8 ? 8 : EPL <= 16 ? 5
                     break;
                 }
             }
+        float s = 0.0f, total = 1.0f;
+        if (active) s = p.sigmoid ? 1.0f / (1.0f + exp2_fast(logit * -LOG2E)) : exp2_fast((logit - top_logit) * LOG2E) * inv;
+        if (p.renormalize) {
+            total = s;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(FULL_WARP, total, o);
+            close |= !(total >= LEAST_TOTAL);
+        }
         if (__any_sync(FULL_WARP, close)) {
             route_row_exactly<T, EPL>(p, row);
             continue;
         }
-        float s = 0.0f;
-        if (active) s = p.sigmoid ? 1.0f / (1.0f + exp2_fast(logit * -LOG2E)) : exp2_fast((logit - top_logit) * LOG2E) * inv;
-        if (p.renormalize) {
-            float total = s;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(FULL_WARP, total, o);
-            if (!(total >= LEAST_TOTAL)) {
-                route_row_exactly<T, EPL>(p, row);
-                continue;
-            }
-            s /= total;
-        }
-        const float w = s * p.scale;
+        const float w = s / total * p.scale;
         if (active) {
             p.experts[row * p.top_k + lane] = e;
             p.weights[row * p.top_k + lane] = w;
