@@ -1148,8 +1148,9 @@ template <typename T> struct SampleRow {
         const Whole ties_before = warp_inclusive(two_ties, lane) - two_ties;
         part_mass[0] += tied(ties_before, part_ties[0], cut_weight);
         part_mass[1] += tied(ties_before + part_ties[0], part_ties[1], cut_weight);
-        // A part of nothing but scores left out would be one without an id to draw.
-        const double least = warp_sum(part_mass[0] + part_mass[1]) * 0x1p-200;
+        // A part of nothing but scores left out would be one without an id to draw.  (A draw at 0 counts every
+        // score with a weight in 64 bits, and its sums are above 0 where there is one.)
+        const double least = u == 0.0 ? 0.0 : warp_sum(part_mass[0] + part_mass[1]) * 0x1p-200;
 #pragma unroll
         for (int h = 0; h < 2; ++h) part_mass[h] = part_mass[h] > least ? part_mass[h] : 0.0;
         const double two = part_mass[0] + part_mass[1];
@@ -1216,23 +1217,6 @@ template <typename T> struct SampleRow {
         p.ids[row] = id;
     }
 
-    // The draw at 0: the lowest id kept, however small its weight.
-    __device__ __forceinline__ void draw_first(int64_t row)
-    {
-        Entry first = ~0ull, unused = 0;
-        each([&](float, uint32_t k, uint32_t id) {
-            if (k >= lowest && k >= cut) first = min(first, static_cast<Entry>(id));
-        });
-        block_range(first, unused);
-        if (blocks > 1) {
-            if (t == 0) sh.exchange[parity] = first;
-            cluster.sync();
-            for (int r = 0; r < blocks; ++r) first = min(first, block_at(r).exchange[parity]);
-            cluster.sync(); // the last look at the other blocks
-        }
-        if (rank == 0 && t == 0) p.ids[row] = static_cast<int64_t>(first);
-    }
-
     __device__ __forceinline__ void run(int64_t row)
     {
         if (t == 0) {
@@ -1294,7 +1278,7 @@ template <typename T> struct SampleRow {
         lowest = lowest_counted();
         if (u == 0.0 && !lone) lowest = lowest_of(fmax(min_p, 4.9406564584124654e-324));
         else if (floor_p && !lone) lowest = max(lowest, lowest_of(min_p));
-        bool summed = !filtered && !lone; // part_mass and part_ties hold what each part's ids keep
+        bool summed = !filtered && !lone && u != 0.0; // part_mass and part_ties hold what each part's ids keep
         if (lone) {
             Whole c = 0;
             each([&](float, uint32_t k, uint32_t) { c += k == top_key; });
@@ -1316,15 +1300,11 @@ template <typename T> struct SampleRow {
         } else if (nucleus) {
             const double need = top_p * total;
             if (border_in_window(need, listed_mass, below)) {
-                summed = !floor_p;
+                summed = !floor_p && u != 0.0;
             } else {
                 const double want = ceil(need * unit);
                 narrow<true>(want > 1.0 ? static_cast<Whole>(want) : Whole{1});
             }
-        }
-        if (u == 0.0) {
-            draw_first(row);
-            return;
         }
         if (!summed) sum_parts();
         everyone(); // the last look at the other blocks
