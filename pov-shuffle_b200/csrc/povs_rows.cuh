@@ -808,8 +808,9 @@ __global__ void __launch_bounds__(32, 24) povs_route_lanes_kernel(const __grid_c
 //   softmax: dx_i = s_i (df_i - sum_j f_j df_j);  sigmoid: dx_i = s_i (1 - s_i) df_i
 // (df is 0 outside the chosen experts).  For a chosen expert, df_i - sum_j f_j df_j
 //   = df_i (1 - sum_j f_j) + sum_j f_j (df_i - df_j), 1 - sum_j f_j the sum of the others,
-// keeps its accuracy where the first form is a difference of near numbers.  The logits are read three times (up to four,
-// or twice where weights are renormalised), all but the first from cache.
+// keeps its accuracy where the first form is a difference of near numbers.  The logits are read three or four times (once
+// for renormalised weights, a sigmoid's chosen ones alone), all but the first from cache.  B200: 26 us with the forward
+// pass for 32749 x 128 bfloat16, 72 for 65536 x 256 float32.
 template <typename T>
 __global__ void __launch_bounds__(128) povs_route_backward_kernel(const __grid_constant__ RouteParams p)
 {
@@ -835,7 +836,11 @@ __global__ void __launch_bounds__(128) povs_route_backward_kernel(const __grid_c
         return a;
     };
     float top = -INFINITY, sum = 0.0f;
-    if (!p.sigmoid) {
+    bool no_scores = false; // a softmax's row with NaN or +infinity
+    if (!p.sigmoid && p.renormalize) {
+        for (int i = lane; i < n; i += 32) no_scores |= !(to_float(x[i]) < INFINITY);
+        no_scores = __any_sync(FULL_WARP, no_scores);
+    } else if (!p.sigmoid) {
         for (int i = lane; i < n; i += 32) top = fmaxf(top, to_float(x[i]));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL_WARP, top, o));
@@ -844,18 +849,24 @@ __global__ void __launch_bounds__(128) povs_route_backward_kernel(const __grid_c
         sum = warp_sum(sum);
     }
     const float inv = 1.0f / sum;
-    const float f = e < 0 ? 0.0f : p.sigmoid ? 1.0f / (1.0f + expf(-v)) : expf(v - top) * inv;
-    // 1 - f of a sigmoid, from the logit: f may be rounded to 1.
-    auto complement = [&] { return v > 0.0f ? expf(-v) / (1.0f + expf(-v)) : 1.0f / (1.0f + expf(v)); };
-    float df = g * p.scale, mine, common = 0.0f;
-    // Where the chosen scores make most of the sum, df less its mean is a small difference of two near numbers: it is
-    // then summed from the differences (33 us against 25 for a training step of 32749 x 128, were it always).
-    constexpr float MOST = 0.75f;
-    auto apart = [&](float weight) {
-        float a = 0.0f;
-        for (int j = 0; j < p.top_k; ++j) a = fmaf(__shfl_sync(FULL_WARP, weight, j), df - __shfl_sync(FULL_WARP, df, j), a);
-        return a;
+    // Score f of a chosen expert; 1 - f of a sigmoid, from the logit too, as f may be rounded to 1.
+    float f = 0.0f, complement = 1.0f;
+    if (p.sigmoid) {
+        const float t = expf(-fabsf(v)), r = 1.0f / (1.0f + t);
+        complement = v > 0.0f ? t * r : r;
+        f = e < 0 ? 0.0f : v > 0.0f ? r : t * r;
+    } else if (!p.renormalize) {
+        f = e < 0 ? 0.0f : expf(v - top) * inv;
+    }
+    // sum_j weight_j (g - g_j) with the weights' sum.  Gradients are taken relative to that of the highest weight, which
+    // differs from the others by no more than top_k times such a sum: near gradients, or one weight near the sum, cost
+    // no accuracy.
+    auto apart = [&](float weight, float weights) {
+        const unsigned most = __reduce_max_sync(FULL_WARP, __float_as_uint(weight));
+        const float from = __shfl_sync(FULL_WARP, g, __ffs(__ballot_sync(FULL_WARP, __float_as_uint(weight) == most)) - 1);
+        return fmaf(weights, g - from, -warp_sum(weight * (g - from)));
     };
+    float mine, common = 0.0f;
     if (p.renormalize) {
         // Quotients of the scores over a common factor, the highest chosen one's, so that none is lost where 32 bits
         // flush the scores themselves to 0.  They do not depend on that factor: common is 0 exactly.
@@ -863,17 +874,19 @@ __global__ void __launch_bounds__(128) povs_route_backward_kernel(const __grid_c
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(FULL_WARP, most, o));
         if (most == -INFINITY || (p.sigmoid && most > 0.0f)) most = 0.0f;
-        const float part = e < 0 ? 0.0f : !p.sigmoid ? expf(v - most) : v > 0.0f ? f : expf(v - most) / (1.0f + expf(v));
+        const float part = e < 0 ? 0.0f : p.sigmoid && v > 0.0f ? f : expf(v - most) * complement;
         const float total = warp_sum(part);
         const float w = total == 0.0f ? 0.0f : part / total;
-        mine = w * (__any_sync(FULL_WARP, w > MOST) ? apart(w) : df - warp_sum(df * w));
-        if (p.sigmoid) mine *= complement();
-        else if (inv != inv) mine = inv; // a row with NaN or +infinity has no scores
+        mine = w * complement * apart(w, 1.0f);
+        if (no_scores) mine = NAN;
     } else if (p.sigmoid) {
-        mine = f * complement() * df;
+        mine = f * complement * g;
     } else {
-        common = warp_sum(f * df);
-        float away = df - common;
+        common = warp_sum(f * g);
+        // Where the others make a quarter of the sum, g less the mean is not small beside both (34 us for a training
+        // step of 32749 x 128 with the others' sum always, against 26).
+        constexpr float MOST = 0.75f;
+        float away = g - common;
         if (__reduce_add_sync(FULL_WARP, __float2uint_rn(f * 0x1p20f)) > static_cast<unsigned>(MOST * 0x1p20f)) {
             unsigned out = 0; // bit m: expert lane + 32 m is chosen
             for (int j = 0; j < p.top_k; ++j) {
@@ -882,10 +895,13 @@ __global__ void __launch_bounds__(128) povs_route_backward_kernel(const __grid_c
             }
             float rest = 0.0f; // the others' sum
             for (int i = lane; i < n; i += 32, out >>= 1) rest += out & 1 ? 0.0f : expf(to_float(x[i]) - top);
-            away = fmaf(df, warp_sum(rest) * inv, apart(f));
+            away = fmaf(g, warp_sum(rest) * inv, apart(f, warp_sum(f)));
         }
         mine = f * away;
     }
+    // The scale comes last: differences of the given numbers are exact where those are near.
+    mine *= p.scale;
+    common *= p.scale;
     for (int i = lane; i < n; i += 32) {
         const float xi = to_float(x[i]);
         dx[i] = from_float<T>(common == 0.0f || xi == -INFINITY ? 0.0f : -expf(xi - top) * inv * common);

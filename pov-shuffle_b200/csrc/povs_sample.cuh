@@ -10,8 +10,8 @@
 //
 // Ids have to be those of exact arithmetic, and two borders of a row of 10^5 ids can lie 10^-10 of its sum
 // apart: weights and sums have 64 bits.  B200, 512 rows of 131072 float32 (41 us to read at the copy rate):
-// 55 us for the reading alone, 75 with top-k 50 (the list), 117 without a filter (the weights: nine 64-bit
-// operations a score), 165 for narrow nuclei (both), 290 where one row in five has a nucleus of thousands.
+// 55 us for the reading alone, 75 with top-k 50 (the list), 114 without a filter (the weights: nine 64-bit
+// operations a score), 165 for narrow nuclei (both), 285 where one row in five has a nucleus of thousands.
 // One row of 50021 with top-k and top-p: 15 us, the latency of about ten steps between barriers.
 #pragma once
 

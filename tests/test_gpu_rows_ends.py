@@ -377,3 +377,16 @@ def test_route_of_many_rows_of_every_shape_of_the_tile(dtype, scoring, bias, n, 
     experts, weights = oracle.route(_host(x), k, **{**kw, "bias": _host(kw["bias"]) if bias else None})
     np.testing.assert_array_equal(_host(got.experts), experts)
     np.testing.assert_allclose(_host(got.weights), weights, rtol=_weight_bound(_host(x), n), atol=1e-37)
+
+
+@pytest.mark.parametrize("renormalize", [False, True])
+def test_route_gradient_of_weights_whose_gradients_are_near(renormalize):
+    """A softmax over all chosen experts passes on the differences of the weights' gradients alone."""
+    x = _randn(60, 4, seed=13)
+    x[:, 0] += 5.0
+    x = x.requires_grad_()
+    experts, weights = povs.route(x, 4, renormalize=renormalize, scale=2.3)
+    g = 1.0 + _randn(60, 4, seed=14, sharp=1e-3)
+    (dx,) = torch.autograd.grad(weights, x, g)
+    want, size = _gradient(_host(x), _host(experts), _host(g), "softmax", renormalize, 2.3)
+    assert (np.abs(_host(dx) - want) <= _gradient_bound(size, want, torch.float32, _host(x), 4)).all()
