@@ -397,7 +397,7 @@ int povs_sample_v1(const void* logits, int32_t dtype, int64_t rows, int64_t widt
  * choice scores (POVS_GROUP_TOP2) or its highest (POVS_GROUP_MAX), and only the top_groups best
  * groups' experts can be chosen.  experts[r * top_k + j]: the j-th highest c, equal ones by the lowest
  * index; weights[r * top_k + j] = scale * s of it, divided by the sum of the row's chosen s with
- * renormalize.  Without bias and groups the order is the logits'; else choices are made on scores
+ * renormalize (also where those are too small for 32 bits).  Without bias and groups the order is the logits'; else choices are made on scores
  * computed in 64 bits.  An expert whose logit or choice
  * score is -infinity is never chosen; a row with fewer than top_k others ends with experts -1 of
  * weight 0.  A NaN score ranks below every number.  No reference counterpart.
@@ -437,8 +437,10 @@ int povs_plan_rows_v1(const void* experts, int32_t id_bytes, int64_t n_entries, 
 /*
  * Copy rows to their slots (device memory; asynchronous on `stream`): row r (row_bytes opaque bytes
  * at data + r * row_stride, bytes) to out + slot * row_bytes for each of slots[r * top_k ..
- * + top_k - 1] in 0 .. n_slots-1.  The rows of `out` from *used (device) on are zeroed.  `out`
- * must not overlap `data`.  No reference counterpart (its moves are in place).
+ * + top_k - 1] in 0 .. n_slots-1.  The rows of `out` from *used (device) on are zeroed.  Slots as
+ * povs_plan_rows_v1 writes them name each place below *used once; with others, a place named twice holds pieces of
+ * either row, and one named by none is left as it was.  `out` must not overlap `data`.  No reference counterpart (its moves
+ * are in place).
  */
 int povs_dispatch_rows_v1(const void* data, int64_t rows, int64_t row_bytes, int64_t row_stride,
                           const int32_t* slots, int32_t top_k, const int32_t* used, void* out, int64_t n_slots,
@@ -456,7 +458,8 @@ int povs_combine_rows_v1(const void* data, int32_t dtype, int64_t n_slots, int64
                          int32_t device, void* stream);
 
 /* Gradients of povs_combine_rows_v1 from grad (rows, width), contiguous: grad_data (n_slots, width),
- * contiguous, or NULL, where the slots from *used on are zeroed; grad_weights (rows, top_k), or NULL. */
+ * contiguous, or NULL, where the slots from *used on are zeroed (each place below is named once, as by
+ * povs_plan_rows_v1); grad_weights (rows, top_k), or NULL, for which alone `data` is read. */
 int povs_combine_backward_v1(const void* grad, const void* data, int32_t dtype, int64_t n_slots, int64_t width,
                              int64_t data_stride, const int32_t* slots, int64_t rows, int32_t top_k,
                              const float* weights, const int32_t* used, void* grad_data, float* grad_weights,

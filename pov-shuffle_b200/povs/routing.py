@@ -35,6 +35,9 @@ class RowPlan(NamedTuple):
     ``slots`` int32 (rows, top_k): the place of each entry, -1 for an entry without an expert.
     ``sources`` int32 (rows * top_k,): the entry (row * top_k + j) at each place; -1 behind the last one.
     ``offsets`` int32 (n_experts + 1,): the first place of each expert, and the number of places in use.
+
+    ``plan_rows`` names every place in use once.  With a plan made by hand that does not, a place named twice holds
+    pieces of either row (or gradient), and a place below ``offsets[-1]`` that no entry names holds anything.
     """
 
     slots: torch.Tensor
